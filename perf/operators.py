@@ -7,10 +7,14 @@ A cache page holds `block` tokens of one KV head: codes [pages, kv_heads, block,
 power-of-two scale per page and head. A block table [batch, max_blocks] names each sequence's pages in order.
 """
 import math
+import os
+import sys
 
 import torch
 
 own = False
+
+PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "whisper-blaze_b200")
 
 DT = {"float16": torch.float16, "bfloat16": torch.bfloat16, "float32": torch.float32}
 F8 = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
@@ -310,6 +314,8 @@ def _plain_sample(s):
 def run(s):
     case = s["case"]
     if own:
+        if PACKAGE not in sys.path:
+            sys.path.insert(0, PACKAGE)
         from whisper_blaze_b200 import ops
         if case["op"] == "attention":
             return ops.attention_kv8(s["q"], s["k_cache"], s["v_cache"], s["k_scale"], s["v_scale"], s["table"],
