@@ -39,6 +39,11 @@ typedef struct CUstream_st* wbk_stream_t;
 #define WBK_FMT_E4M3 0
 #define WBK_FMT_E5M2 1
 
+/* element types of the 16- and 32-bit inputs that a call names by number */
+#define WBK_DT_F16  0   /* IEEE binary16 */
+#define WBK_DT_BF16 1   /* bfloat16 */
+#define WBK_DT_F32  2   /* IEEE binary32 */
+
 /* GEMM epilogues */
 #define WBK_EPI_NONE          0   /* out = fp16(acc*descale [+ bias]) */
 #define WBK_EPI_GELU          1   /* out = fp16(gelu_erf(acc*descale + bias)) */
@@ -295,6 +300,90 @@ int wbk_linear_fp8_f16(const void* A16, int64_t M, int64_t N, int64_t K, int a_f
                        const void* bias, const void* residual, void* out,
                        int epilogue, uint32_t* out_amax_bits,
                        void* workspace, int64_t workspace_bytes, wbk_stream_t stream);
+
+/* -------------------------------------------------- 8-bit key/value cache
+ *
+ * The cache of a decoder layer: codes [pages, kv_heads, block, head_dim] in the
+ * fp8 format `fmt`, contiguous, one array for keys and one for values, and one
+ * fp32 scale per page and head, [pages, kv_heads]; a value is code * scale.
+ * block (tokens per page) is 16, 32, 64 or 128; head_dim 64 or 128. Row b of
+ * block_table (int32, row stride table_stride elements, max_blocks entries)
+ * names the pages of sequence b in order: token t of it lies in page
+ * block_table[b][t / block], at t % block. Lengths, table and scales are read on
+ * the device, so no call synchronises. Lengths beyond the table are held to it,
+ * and a table entry outside [0, pages) names no page: nothing is written there,
+ * and attention leaves its tokens out.
+ * Scales are powers of two, as wbk_kv8_append writes them; attention takes any
+ * positive finite scale. No reference counterpart (the reference caches fp16 keys
+ * and values inside Hugging Face's decoder, whisper_blaze/model.py).
+ */
+
+/* Append `tokens` new tokens (new_lens[b] of them where new_lens is not NULL) of
+ * each sequence behind the seq_lens[b] that its cache holds.
+ * k, v: [batch, kv_heads, tokens, head_dim] views of dtype WBK_DT_F16 or
+ * WBK_DT_BF16 with the head_dim values contiguous and element strides in the
+ * HOST array strides[6] = {k_b, k_h, k_s, v_b, v_h, v_s}, each a multiple of 8;
+ * pointers 16-byte aligned.
+ * Of each touched page and head: scale = 2^E with the least E >= -64 for which
+ * max|x| <= max_fp8 * 2^E over the page's tokens (NaN and infinities left out of
+ * the maximum), never less than the scale of the tokens that the page held
+ * already; code = fp8_rn_satfinite(x / scale), NaN -> -max_fp8. Where the scale
+ * of a partly filled page grows, its older codes become
+ * fp8_rn_satfinite(code * old_scale / scale). Places behind the last token keep
+ * what they held. A page must not be appended to for two sequences in one call.
+ * seq_lens and new_lens are not changed. */
+int wbk_kv8_append(const void* k, const void* v, int dtype, int64_t batch, int64_t kv_heads, int64_t tokens,
+                   int64_t head_dim, const int64_t* strides, int fmt, void* k_cache, void* v_cache,
+                   float* k_scale, float* v_scale, int64_t pages, int64_t block, const int32_t* block_table,
+                   int64_t max_blocks, int64_t table_stride, const int32_t* seq_lens, const int32_t* new_lens,
+                   wbk_stream_t stream);
+
+/* Attention of `queries` query rows per sequence over the cache:
+ *   out[b,h,i,:] = sum_j softmax_j(scale * q[b,h,i,:] . k[j]) v[j],  j < visible
+ * with n = q_lens[b] (queries where q_lens is NULL) real rows in sequence b and
+ * visible = seq_lens[b] - n + i + 1 where causal is not 0 (the n rows are the
+ * sequence's last n tokens), seq_lens[b] otherwise. A row that sees no token,
+ * and a row i >= n, is 0. Query head h reads KV head h / (heads / kv_heads).
+ * q, out: [batch, heads, queries, head_dim] views of dtype WBK_DT_F16 or
+ * WBK_DT_BF16, head_dim values contiguous, element strides in the HOST array
+ * strides[6] = {q_b, q_h, q_s, o_b, o_h, o_s}, each a multiple of 8; pointers
+ * 16-byte aligned. Scores, softmax and sums in fp32; the softmax weights are
+ * rounded to fp16 before they multiply the (exact) fp16 values of the codes.
+ * What lies in the cache behind a sequence's length is never used, whatever its
+ * codes. A NaN code among the visible tokens makes its head's rows NaN.
+ * workspace: wbk_attention_kv8_ws_bytes(...) bytes of device memory, 256-byte
+ * aligned, zero-filled before first use and left reusable by each call, not used
+ * by two calls at once; may be NULL where that is 0. */
+int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
+                      int64_t queries, int64_t head_dim, const int64_t* strides, int fmt, const void* k_cache,
+                      const void* v_cache, const float* k_scale, const float* v_scale, int64_t pages,
+                      int64_t block, const int32_t* block_table, int64_t max_blocks, int64_t table_stride,
+                      const int32_t* seq_lens, const int32_t* q_lens, int causal, float scale, void* workspace,
+                      int64_t workspace_bytes, wbk_stream_t stream);
+int64_t wbk_attention_kv8_ws_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t queries,
+                                   int64_t head_dim);
+
+/* --------------------------------------------------------------- sampling */
+
+/* One token for each of `rows` rows of logits (dtype WBK_DT_F16, _BF16 or _F32;
+ * row stride logits_stride elements). With M the row's largest logit and
+ * p_i = exp((l_i - M) / temperature), tokens ordered by logit (larger first,
+ * ties by lower index), a token is kept iff its place is below top_k, the mass
+ * before it is below top_p * (mass of the first top_k), and p_i >= min_p; the
+ * first token is always kept. The answer is the kept token with the largest
+ * p_i / noise_i, ties to the lower index; noise: fp32 [rows, vocab] (row stride
+ * noise_stride), independent Exp(1) numbers, which makes it a draw from the kept
+ * tokens' softmax. temperature <= 0: the first token of the order. top_k <= 0 or
+ * >= vocab, top_p >= 1, min_p <= 0: no such filter. NaN logits count as -inf, which is never drawn,
+ * +inf as the largest finite fp32; noise below 2^-126 counts as 2^-126.
+ * temperature, top_k, top_p, min_p: device arrays [rows], or NULL: the *_all value for every row.
+ * tokens_out[row] = the token, logprobs_out[row] = log softmax(l)[token] of the
+ * logits as given (temperature 1, nothing filtered); a row with no logit above
+ * -inf gives -1 and -inf. Equal inputs give equal outputs, bit for bit. */
+int wbk_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t logits_stride,
+               const float* noise, int64_t noise_stride, const float* temperature, const int32_t* top_k,
+               const float* top_p, const float* min_p, float temperature_all, int top_k_all, float top_p_all,
+               float min_p_all, int64_t* tokens_out, float* logprobs_out, wbk_stream_t stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -37,9 +37,12 @@ UNITS = {
     "wbk_norm.cu": [],
     "wbk_gemm.cu": [],
     "wbk_attn.cu": [],
+    "wbk_kv8.cu": [],
+    "wbk_sample.cu": [],
 }
 HEADERS = [os.path.join(HERE, "wbk_common.cuh"), os.path.join(HERE, "wbk_sm100.cuh"),
-           os.path.join(HERE, "wbk_fp8_quant.cuh"), os.path.join(INCLUDE, "wbk.h")]
+           os.path.join(HERE, "wbk_fp8_quant.cuh"), os.path.join(HERE, "wbk_kv8.cuh"),
+           os.path.join(INCLUDE, "wbk.h")]
 
 
 def nvcc() -> str:

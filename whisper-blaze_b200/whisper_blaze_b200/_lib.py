@@ -25,6 +25,10 @@ WBK_ERR_DEVICE_TIMEOUT = 4
 FMT_E4M3 = 0
 FMT_E5M2 = 1
 
+DT_F16 = 0
+DT_BF16 = 1
+DT_F32 = 2
+
 EPI_NONE = 0
 EPI_GELU = 1
 EPI_RESIDUAL = 2
@@ -59,6 +63,13 @@ _PROTOTYPES = {
     "wbk_gemm_fp8_ws_bytes": (_i64, [_i64, _i64, _i64]),
     "wbk_linear_fp8_f16": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _f32, _vp, _vp, _vp,
                                   _i32, _vp, _vp, _i64, _vp]),
+    "wbk_kv8_append": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _vp,
+                              _i64, _i64, _vp, _vp, _vp]),
+    "wbk_attention_kv8": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i64,
+                                 _i64, _vp, _i64, _i64, _vp, _vp, _i32, _f32, _vp, _i64, _vp]),
+    "wbk_attention_kv8_ws_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "wbk_sample": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _f32, _i32, _f32, _f32, _vp, _vp,
+                          _vp]),
 }
 
 _lock = threading.Lock()

@@ -13,8 +13,8 @@ from typing import Optional, Sequence, Union
 import torch
 
 from . import _lib
-from ._lib import (EPI_BIAS_MAXKEY, EPI_GELU, EPI_NONE, EPI_RESIDUAL, EPI_RESIDUAL_CLAMP, FMT_E4M3, FMT_E5M2,
-                   check, lib, ptr, stream_of)
+from ._lib import (DT_BF16, DT_F16, DT_F32, EPI_BIAS_MAXKEY, EPI_GELU, EPI_NONE, EPI_RESIDUAL, EPI_RESIDUAL_CLAMP,
+                   FMT_E4M3, FMT_E5M2, check, lib, ptr, stream_of)
 
 Scale = Union[float, torch.Tensor]
 
@@ -470,3 +470,203 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[t
                                       strides, sc, ptr(out_amax), stream_of(q)), "attention")
     _count()
     return o
+
+
+# ------------------------------------------------------ 8-bit key/value cache
+
+_DT16 = {torch.float16: DT_F16, torch.bfloat16: DT_BF16}
+_F8_DTYPE = {FMT_E4M3: torch.float8_e4m3fn, FMT_E5M2: torch.float8_e5m2}
+
+
+def _require_int32(t: torch.Tensor, name: str, numel: int) -> None:
+    require_input(t, name)
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != numel:
+        raise RuntimeError(f"{name} must be int32 with shape [{numel}]")
+
+
+def _require_bhsd(t: torch.Tensor, name: str) -> int:
+    """The dtype number of a [B, H, S, D] fp16 or bf16 CUDA view with a contiguous last dimension."""
+    require_cuda(t, name)
+    if t.dtype not in _DT16:
+        raise RuntimeError(f"{name} must be fp16 or bf16, got {t.dtype}")
+    if t.dim() != 4:
+        raise RuntimeError(f"{name} must be 4D: [B, H, S, D]")
+    if t.stride(-1) != 1:
+        raise RuntimeError(f"{name} must have a contiguous last dimension")
+    return _DT16[t.dtype]
+
+
+def _strides3(t: torch.Tensor) -> list:
+    """Batch, head and position strides; 0 where a dimension has one entry, whose stride says nothing."""
+    return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
+
+
+def _require_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, batch: int, kv_heads, head_dim: int, fmt):
+    """Checks a cache against the batch that uses it; (format, pages, block, max_blocks, table stride)."""
+    f = fmt_code(fmt)
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        require_input(t, name)
+        if t.dtype not in (torch.uint8, torch.int8, _F8_DTYPE[f]):
+            raise RuntimeError(f"{name} must hold {fmt} codes (uint8, int8 or {_F8_DTYPE[f]}), got {t.dtype}")
+        if t.dim() != 4:
+            raise RuntimeError(f"{name} must be 4D: [pages, kv_heads, block, head_dim]")
+    if k_cache.shape != v_cache.shape:
+        raise RuntimeError("k_cache and v_cache must have the same shape")
+    pages, heads, block, d = k_cache.shape
+    if d != head_dim or (kv_heads is not None and heads != kv_heads):
+        raise RuntimeError(f"the cache holds {heads} heads of {d}; the call has {kv_heads or heads} of {head_dim}")
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        require_input(t, name)
+        if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads):
+            raise RuntimeError(f"{name} must be fp32 with shape {(pages, heads)}")
+    require_cuda(block_table, "block_table")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
+        raise RuntimeError(f"block_table must be int32 with shape [{batch}, max_blocks]")
+    width = block_table.shape[1]
+    if width > 1 and block_table.stride(1) != 1:
+        raise RuntimeError("block_table must have contiguous rows")
+    _require_int32(seq_lens, "seq_lens", batch)
+    return f, pages, block, width, max(block_table.stride(0), width) if batch > 1 else width
+
+
+def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+               v_scale: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+               new_lens: Optional[torch.Tensor] = None, fmt="e4m3") -> None:
+    """Write new tokens' keys and values into the pages of an 8-bit cache, in place.
+
+    k, v [B, Hkv, T, D] fp16 or bf16 CUDA views (strides multiples of 8 elements,
+    last dimension contiguous); k_cache, v_cache [pages, Hkv, block, D] fp8 codes
+    (uint8 or the float8 dtype of `fmt`), block 16 / 32 / 64 / 128, D 64 / 128;
+    k_scale, v_scale [pages, Hkv] fp32; block_table [B, max_blocks] int32;
+    seq_lens [B] int32: tokens each sequence holds BEFORE this call; new_lens [B]
+    int32: how many of the T tokens are real (default: all).
+    A page and head share one power-of-two scale; where a new token needs a larger
+    one, the page's older codes are rescaled. Tokens past the table, or whose page
+    is outside the pool, are not stored. seq_lens is not changed.
+    """
+    dt = _require_bhsd(k, "k")
+    if _require_bhsd(v, "v") != dt or v.shape != k.shape:
+        raise RuntimeError("k and v must have the same shape and dtype")
+    B, H, T, D = k.shape
+    f, pages, block, width, ts = _require_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, B, H, D, fmt)
+    if new_lens is not None:
+        _require_int32(new_lens, "new_lens", B)
+    require_same_device(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, new_lens)
+    strides = (ctypes.c_int64 * 6)(*(_strides3(k) + _strides3(v)))
+    with torch.cuda.device(k.device):
+        check(lib().wbk_kv8_append(k.data_ptr(), v.data_ptr(), dt, B, H, T, D, strides, f, k_cache.data_ptr(),
+                                   v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, block,
+                                   block_table.data_ptr(), width, ts, seq_lens.data_ptr(), ptr(new_lens),
+                                   stream_of(k)), "kv8_append")
+    _count()
+
+
+def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                  v_scale: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                  q_lens: Optional[torch.Tensor] = None, causal: bool = True, scale: Optional[float] = None,
+                  fmt="e4m3", out: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(q k^T * scale) v over the pages of an 8-bit cache.
+
+    q [B, Hq, T, D] fp16 or bf16 CUDA view, Hq a multiple of the cache's heads; the
+    cache, block_table as for kv8_append; seq_lens [B] int32: tokens each sequence
+    holds now (the T queries' own included where causal); q_lens [B] int32: how
+    many of the T rows are real (default: all). Causal row i of n sees the first
+    seq_len - n + i + 1 tokens, otherwise all seq_len; a row that sees none, and a
+    padding row, is 0. scale defaults to 1/sqrt(D). `out` (default: a new
+    contiguous [B, Hq, T, D] tensor) takes the output in q's dtype.
+    Long caches are split over the SMs through `workspace` (a zero-filled uint8
+    CUDA tensor of at least wbk_attention_kv8_ws_bytes bytes) or the device's
+    shared one, so such calls must not run concurrently on different streams
+    without a workspace of their own.
+    """
+    dt = _require_bhsd(q, "q")
+    B, H, T, D = q.shape
+    f, pages, block, width, ts = _require_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, B, None, D, fmt)
+    kv_heads = k_cache.shape[1]
+    if kv_heads == 0 or H % kv_heads != 0:
+        raise RuntimeError(f"{H} query heads do not share {kv_heads} KV heads evenly")
+    if q_lens is not None:
+        _require_int32(q_lens, "q_lens", B)
+    o = torch.empty((B, H, T, D), dtype=q.dtype, device=q.device) if out is None else out
+    if o.shape != q.shape or _require_bhsd(o, "out") != dt:
+        raise RuntimeError(f"out must be a {q.dtype} view of shape {tuple(q.shape)}")
+    require_same_device(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, q_lens, o, workspace)
+    strides = (ctypes.c_int64 * 6)(*(_strides3(q) + _strides3(o)))
+    sc = float(scale) if scale is not None else D ** -0.5
+    with torch.cuda.device(q.device):
+        need = lib().wbk_attention_kv8_ws_bytes(B, H, kv_heads, T, D)
+        ws = workspace if workspace is not None else splitk_workspace(q.device, need)
+        check(lib().wbk_attention_kv8(q.data_ptr(), o.data_ptr(), dt, B, H, kv_heads, T, D, strides, f,
+                                      k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                      pages, block, block_table.data_ptr(), width, ts, seq_lens.data_ptr(),
+                                      ptr(q_lens), int(bool(causal)), sc, ptr(ws),
+                                      0 if ws is None else ws.numel() * ws.element_size(), stream_of(q)),
+              "attention_kv8")
+    _count()
+    return o
+
+
+# ----------------------------------------------------------------- sampling
+
+_DT_LOGITS = {torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.float32: DT_F32}
+
+
+def _per_row(value, name: str, dtype: torch.dtype, rows: int):
+    """(number for every row, device array or None)."""
+    if isinstance(value, torch.Tensor):
+        require_input(value, name)
+        if value.dtype != dtype or value.numel() != rows or value.dim() != 1:
+            raise RuntimeError(f"{name} must be a number or a {dtype} tensor of shape [{rows}]")
+        return 0, value
+    return value, None
+
+
+def sample(logits: torch.Tensor, noise: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+           tokens_out: Optional[torch.Tensor] = None,
+           logprobs_out: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Draw one token per row of logits; (tokens int64 [B], logprobs fp32 [B]).
+
+    logits [B, V] fp16, bf16 or fp32; noise [B, V] fp32 of independent Exp(1)
+    numbers (torch.Tensor.exponential_), both with contiguous rows. temperature,
+    top_p, min_p: a number or an fp32 CUDA tensor [B]; top_k: a number or an int32
+    CUDA tensor [B]. Filters apply in the order temperature, top_k, top_p (of what
+    top_k left), min_p (relative to the largest probability); temperature 0 is
+    greedy, top_k 0, top_p 1 and min_p 0 filter nothing. Ties go to the lowest
+    index; equal inputs give equal tokens. logprobs is the token's log-probability
+    under the unfiltered softmax of the logits as given. A row with no logit above
+    -inf gives token -1 and logprob -inf.
+    """
+    require_cuda(logits, "logits")
+    if logits.dtype not in _DT_LOGITS:
+        raise RuntimeError(f"logits must be fp16, bf16 or fp32, got {logits.dtype}")
+    if logits.dim() != 2:
+        raise RuntimeError("logits must be 2-D [B, V]")
+    B, V = logits.shape
+    require_cuda(noise, "noise")
+    if noise.dtype != torch.float32 or noise.shape != logits.shape:
+        raise RuntimeError(f"noise must be fp32 with shape {(B, V)}")
+    for t, name in ((logits, "logits"), (noise, "noise")):
+        if V > 1 and t.stride(1) != 1:
+            raise RuntimeError(f"{name} must have contiguous rows")
+    t_all, t_row = _per_row(temperature, "temperature", torch.float32, B)
+    k_all, k_row = _per_row(top_k, "top_k", torch.int32, B)
+    p_all, p_row = _per_row(top_p, "top_p", torch.float32, B)
+    m_all, m_row = _per_row(min_p, "min_p", torch.float32, B)
+    if not (t_all >= 0 and k_all >= 0 and p_all >= 0 and m_all >= 0):
+        raise ValueError("temperature, top_k, top_p and min_p must not be negative")
+    tok = torch.empty(B, dtype=torch.int64, device=logits.device) if tokens_out is None else tokens_out
+    lp = torch.empty(B, dtype=torch.float32, device=logits.device) if logprobs_out is None else logprobs_out
+    for t, name, dtype in ((tok, "tokens_out", torch.int64), (lp, "logprobs_out", torch.float32)):
+        require_input(t, name)
+        if t.dtype != dtype or tuple(t.shape) != (B,):
+            raise RuntimeError(f"{name} must be {dtype} with shape [{B}]")
+    require_same_device(logits, noise, t_row, k_row, p_row, m_row, tok, lp)
+    with torch.cuda.device(logits.device):
+        check(lib().wbk_sample(logits.data_ptr(), _DT_LOGITS[logits.dtype], B, V,
+                               max(logits.stride(0), V) if B > 1 else V, noise.data_ptr(),
+                               max(noise.stride(0), V) if B > 1 else V, ptr(t_row), ptr(k_row), ptr(p_row),
+                               ptr(m_row), float(t_all), min(int(k_all), 2 ** 31 - 1), float(p_all), float(m_all),
+                               tok.data_ptr(), lp.data_ptr(), stream_of(logits)), "sample")
+    _count()
+    return tok, lp
