@@ -1,5 +1,4 @@
-// The 8-bit key/value cache of a decoder: appending new tokens to its pages, and
-// attention over them.
+// The 8-bit key/value cache of a decoder: appending new tokens to its pages.
 //
 // A page holds `block` tokens of one KV head as fp8 codes with one fp32 scale, a
 // power of two. Scales are powers of two so that a page whose scale grows (a
@@ -145,88 +144,6 @@ int launch_append(const AppendParams& p, int head_dim, dim3 grid, cudaStream_t s
   return cuda_check(cudaGetLastError(), "kv8 append launch");
 }
 
-// --------------------------------------------------------------- attention
-
-struct Kv8AttnParams {
-  const void* q;
-  void* out;
-  int64_t q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;
-  Kv8Pages c;
-  const uint8_t *k_cache, *v_cache;
-  const float *k_scale, *v_scale;
-  const int32_t* lens;
-  const int32_t* q_lens;
-  int batch, heads, group, queries, causal;
-  float scale;
-};
-
-// One warp per query row: 32 tokens at a time, a lane per token for the scores, a
-// lane per head_dim / 32 channels for the sum.
-template <int kFmt, int kDtype, int kD>
-__global__ void __launch_bounds__(128) kv8_attention_kernel(const Kv8AttnParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= static_cast<int64_t>(p.batch) * p.heads * p.queries) return;
-  const int i = static_cast<int>(row % p.queries);
-  const int h = static_cast<int>(row / p.queries % p.heads);
-  const int b = static_cast<int>(row / p.queries / p.heads);
-  const int len = kv8_len(p.lens, b, p.c);
-  const int n = p.q_lens != nullptr ? min(max(p.q_lens[b], 0), p.queries) : p.queries;
-  const int visible = i >= n ? 0 : p.causal ? len - n + i + 1 : len;
-  const uint16_t* q = static_cast<const uint16_t*>(p.q) + b * p.q_sb + h * p.q_sh + i * p.q_ss;
-  constexpr int kPer = kD / 32;
-  float m = -INFINITY, l = 0.0f, acc[kPer] = {};
-  for (int j0 = 0; j0 < visible; j0 += 32) {
-    const int j = j0 + lane;
-    float score = -INFINITY, vs = 0.0f;
-    int64_t base = 0;
-    if (j < visible) {
-      const int64_t page = kv8_page(p.c, b, j >> p.c.block_log2);
-      if (page >= 0) {
-        const int64_t ph = page * p.c.kv_heads + h / p.group;
-        base = (ph * p.c.block + (j & (p.c.block - 1))) * kD;
-        vs = p.v_scale[ph];
-        float dot = 0.0f;
-        for (int d = 0; d < kD; d += 2) {
-          const float2 kf = __half22float2(kv8_half2<kFmt>(*reinterpret_cast<const uint16_t*>(p.k_cache + base + d)));
-          const float2 qf = pair_to_float2<kDtype>(*reinterpret_cast<const uint32_t*>(q + d));
-          dot = fmaf(kf.x, qf.x, fmaf(kf.y, qf.y, dot));
-        }
-        score = dot * p.k_scale[ph] * p.scale;
-      }
-    }
-    float mx = score;
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
-    mx = fmaxf(m, mx);
-    if (mx == -INFINITY) continue;
-    const float alpha = expf(m - mx), w = expf(score - mx);
-    m = mx;
-    l = l * alpha + warp_sum(w);
-    for (int c = 0; c < kPer; ++c) acc[c] *= alpha;
-    for (int t = 0; t < 32 && j0 + t < visible; ++t) {
-      const float wt = __shfl_sync(~0u, w * vs, t);
-      const int64_t bt = __shfl_sync(~0u, base, t);
-      if (wt == 0.0f) continue;
-      for (int c = 0; c < kPer; ++c)
-        acc[c] = fmaf(wt, __low2float(kv8_half2<kFmt>(p.v_cache[bt + lane + 32 * c])), acc[c]);
-    }
-  }
-  uint16_t* out = static_cast<uint16_t*>(p.out) + b * p.o_sb + h * p.o_sh + i * p.o_ss;
-  for (int c = 0; c < kPer; ++c)
-    out[lane + 32 * c] = static_cast<uint16_t>(float2_to_pair<kDtype>(l > 0.0f ? acc[c] / l : 0.0f, 0.0f));
-}
-
-template <int kFmt, int kDtype>
-int launch_attention(const Kv8AttnParams& p, int head_dim, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.queries;
-  const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
-  if (head_dim == 64) kv8_attention_kernel<kFmt, kDtype, 64><<<grid, 128, 0, stream>>>(p);
-  else kv8_attention_kernel<kFmt, kDtype, 128><<<grid, 128, 0, stream>>>(p);
-  return cuda_check(cudaGetLastError(), "kv8 attention launch");
-}
-
-bool kv8_stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s < (int64_t(1) << 40); }
-
 }  // namespace
 }  // namespace wbk
 
@@ -276,68 +193,6 @@ int wbk_kv8_append(const void* k, const void* v, int dtype, int64_t batch, int64
                                : launch_append<WBK_FMT_E4M3, WBK_DT_BF16>(p, d, grid, st);
   return dtype == WBK_DT_F16 ? launch_append<WBK_FMT_E5M2, WBK_DT_F16>(p, d, grid, st)
                              : launch_append<WBK_FMT_E5M2, WBK_DT_BF16>(p, d, grid, st);
-}
-
-int64_t wbk_attention_kv8_ws_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t queries, int64_t head_dim) {
-  (void)batch, (void)heads, (void)kv_heads, (void)queries, (void)head_dim;
-  return 0;
-}
-
-int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
-                      int64_t queries, int64_t head_dim, const int64_t* strides, int fmt, const void* k_cache,
-                      const void* v_cache, const float* k_scale, const float* v_scale, int64_t pages, int64_t block,
-                      const int32_t* block_table, int64_t max_blocks, int64_t table_stride, const int32_t* seq_lens,
-                      const int32_t* q_lens, int causal, float scale, void* workspace, int64_t workspace_bytes,
-                      wbk_stream_t stream) {
-  if (batch < 0 || heads < 0 || kv_heads < 0 || queries < 0)
-    return fail(WBK_ERR_INVALID_ARG, "wbk_attention_kv8: negative size");
-  if (dtype != WBK_DT_F16 && dtype != WBK_DT_BF16)
-    return fail(WBK_ERR_INVALID_ARG, "wbk_attention_kv8: dtype %d (WBK_DT_F16 or WBK_DT_BF16)", dtype);
-  if (batch == 0 || heads == 0 || queries == 0) return WBK_OK;
-  if (q == nullptr || out == nullptr || strides == nullptr)
-    return fail(WBK_ERR_INVALID_ARG, "wbk_attention_kv8: null pointer");
-  if (int e = kv8_check_pages("wbk_attention_kv8", k_cache, v_cache, k_scale, v_scale, pages, kv_heads, block, head_dim,
-                              fmt, block_table, max_blocks, table_stride, seq_lens))
-    return e;
-  if (heads % kv_heads != 0)
-    return fail(WBK_ERR_INVALID_ARG, "wbk_attention_kv8: %lld query heads do not share %lld KV heads evenly",
-                (long long)heads, (long long)kv_heads);
-  if (batch > 32767 || heads > 65535 || queries > (1 << 24))
-    return fail(WBK_ERR_UNSUPPORTED, "wbk_attention_kv8: size beyond batch 32767, heads 65535, queries 2^24");
-  if (q_lens != nullptr && !aligned(q_lens, 4))
-    return fail(WBK_ERR_INVALID_ARG, "wbk_attention_kv8: q_lens misaligned");
-  if (!aligned(q, 16) || !aligned(out, 16))
-    return fail(WBK_ERR_UNSUPPORTED, "wbk_attention_kv8: q and out must be 16-byte aligned");
-  for (int i = 0; i < 6; ++i)
-    if (!kv8_stride_ok(strides[i]))
-      return fail(WBK_ERR_UNSUPPORTED, "wbk_attention_kv8: stride[%d] = %lld is not a multiple of 8 elements", i,
-                  (long long)strides[i]);
-  (void)workspace, (void)workspace_bytes;
-  Kv8AttnParams p{};
-  p.q = q;
-  p.out = out;
-  p.q_sb = strides[0], p.q_sh = strides[1], p.q_ss = strides[2];
-  p.o_sb = strides[3], p.o_sh = strides[4], p.o_ss = strides[5];
-  p.c = kv8_pages(pages, kv_heads, block, block_table, max_blocks, table_stride);
-  p.k_cache = static_cast<const uint8_t*>(k_cache);
-  p.v_cache = static_cast<const uint8_t*>(v_cache);
-  p.k_scale = k_scale;
-  p.v_scale = v_scale;
-  p.lens = seq_lens;
-  p.q_lens = q_lens;
-  p.batch = static_cast<int>(batch);
-  p.heads = static_cast<int>(heads);
-  p.group = static_cast<int>(heads / kv_heads);
-  p.queries = static_cast<int>(queries);
-  p.causal = causal;
-  p.scale = scale;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int d = static_cast<int>(head_dim);
-  if (fmt == WBK_FMT_E4M3)
-    return dtype == WBK_DT_F16 ? launch_attention<WBK_FMT_E4M3, WBK_DT_F16>(p, d, st)
-                               : launch_attention<WBK_FMT_E4M3, WBK_DT_BF16>(p, d, st);
-  return dtype == WBK_DT_F16 ? launch_attention<WBK_FMT_E5M2, WBK_DT_F16>(p, d, st)
-                             : launch_attention<WBK_FMT_E5M2, WBK_DT_BF16>(p, d, st);
 }
 
 }  // extern "C"

@@ -101,6 +101,8 @@ __device__ __forceinline__ int kv8_len(const int32_t* lens, int b, const Kv8Page
 int kv8_check_pages(const char* what, const void* k_cache, const void* v_cache, const float* k_scale,
                     const float* v_scale, int64_t pages, int64_t kv_heads, int64_t block, int64_t head_dim, int fmt,
                     const int32_t* block_table, int64_t max_blocks, int64_t table_stride, const int32_t* seq_lens);
+// Element stride of a batch, head or position: TMA and 16-byte accesses need multiples of 8.
+inline bool kv8_stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s < (int64_t(1) << 40); }
 Kv8Pages kv8_pages(int64_t pages, int64_t kv_heads, int64_t block, const int32_t* block_table, int64_t max_blocks,
                    int64_t table_stride);
 

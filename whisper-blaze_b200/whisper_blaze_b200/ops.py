@@ -293,6 +293,7 @@ def _scale_arg(scale: Scale, name: str, device) -> tuple[float, Optional[int]]:
 
 
 _SPLITK_WS: dict = {}
+_KV8_WS: dict = {}
 
 
 @_lib.on_device_timeout
@@ -300,9 +301,10 @@ def _zero_shared_workspaces(device_index: int) -> None:
     """After a device-side timeout a kernel may have left the sync words or split-K tickets of
     the device's shared workspace non-zero; zero it again so the next call starts clean.
     (Workspaces passed by the caller are the caller's to zero, as wbk.h states.)"""
-    ws = _SPLITK_WS.get(torch.device("cuda", device_index))
-    if ws is not None:
-        ws.zero_()
+    for shared in (_SPLITK_WS, _KV8_WS):
+        ws = shared.get(torch.device("cuda", device_index))
+        if ws is not None:
+            ws.zero_()
 
 
 def splitk_workspace(device, nbytes: int) -> Optional[torch.Tensor]:
@@ -529,6 +531,16 @@ def _require_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, ba
     return f, pages, block, width, max(block_table.stride(0), width) if batch > 1 else width
 
 
+def kv8_workspace(device, nbytes: int) -> torch.Tensor:
+    """The per-device workspace of attention_kv8 (zero-filled once, grown on demand), shared by its calls on the
+    device: calls that may run at the same time need workspaces of their own."""
+    dev = torch.device(device)
+    ws = _KV8_WS.get(dev)
+    if ws is None or ws.numel() < nbytes:
+        ws = _KV8_WS[dev] = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+    return ws
+
+
 def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                v_scale: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                new_lens: Optional[torch.Tensor] = None, fmt="e4m3") -> None:
@@ -596,7 +608,7 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     sc = float(scale) if scale is not None else D ** -0.5
     with torch.cuda.device(q.device):
         need = lib().wbk_attention_kv8_ws_bytes(B, H, kv_heads, T, D)
-        ws = workspace if workspace is not None else splitk_workspace(q.device, need)
+        ws = workspace if workspace is not None else kv8_workspace(q.device, need)
         check(lib().wbk_attention_kv8(q.data_ptr(), o.data_ptr(), dt, B, H, kv_heads, T, D, strides, f,
                                       k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                       pages, block, block_table.data_ptr(), width, ts, seq_lens.data_ptr(),
