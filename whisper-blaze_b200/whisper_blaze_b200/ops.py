@@ -8,6 +8,7 @@ quantise -> GEMM -> norm -> quantise issues no host round trip.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Sequence, Union
 
 import torch
@@ -476,68 +477,107 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[t
 
 # ------------------------------------------------------ 8-bit key/value cache
 
+# The calls below are made once per layer and token, so what they do on the host is kept short: device indexes
+# instead of device objects, the raw stream, no device guard where the device is current already.
+
 _DT16 = {torch.float16: DT_F16, torch.bfloat16: DT_BF16}
 _F8_DTYPE = {FMT_E4M3: torch.float8_e4m3fn, FMT_E5M2: torch.float8_e5m2}
 
 
-def _require_int32(t: torch.Tensor, name: str, numel: int) -> None:
-    require_input(t, name)
-    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != numel:
+_I64X6 = ctypes.c_int64 * 6
+_BYTES8 = (torch.uint8, torch.int8)
+
+
+def _launch(fn, args: tuple, index: int, what: str) -> None:
+    """fn(*args, stream) on the current stream of CUDA device `index`."""
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status, what)
+    LAUNCHES[0] += 1
+
+
+def _require_on(index: int, t: torch.Tensor, name: str) -> None:
+    """t is a contiguous tensor on CUDA device `index`."""
+    if t.get_device() != index:
+        require_cuda(t, name)
+        raise RuntimeError(f"{name} is on {t.device}, expected cuda:{index}")
+    if not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+
+
+def _require_int32(index: int, t: torch.Tensor, name: str, numel: int) -> None:
+    _require_on(index, t, name)
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != numel:
         raise RuntimeError(f"{name} must be int32 with shape [{numel}]")
 
 
-def _require_bhsd(t: torch.Tensor, name: str) -> int:
-    """The dtype number of a [B, H, S, D] fp16 or bf16 CUDA view with a contiguous last dimension."""
-    require_cuda(t, name)
-    if t.dtype not in _DT16:
+def _require_bhsd(t: torch.Tensor, name: str) -> tuple:
+    """(dtype number, device index, shape, strides) of a [B, H, S, D] fp16 or bf16 CUDA view with a contiguous last
+    dimension; the stride of a dimension of one entry, which says nothing, is 0."""
+    index = t.get_device()
+    if index < 0:
+        require_cuda(t, name)
+    dt = _DT16.get(t.dtype)
+    if dt is None:
         raise RuntimeError(f"{name} must be fp16 or bf16, got {t.dtype}")
-    if t.dim() != 4:
+    shape = t.shape
+    if len(shape) != 4:
         raise RuntimeError(f"{name} must be 4D: [B, H, S, D]")
-    if t.stride(-1) != 1:
+    sb, sh, ss, sd = t.stride()
+    if sd != 1:
         raise RuntimeError(f"{name} must have a contiguous last dimension")
-    return _DT16[t.dtype]
+    b, h, s, _ = shape
+    return dt, index, shape, (sb if b > 1 else 0, sh if h > 1 else 0, ss if s > 1 else 0)
 
 
-def _strides3(t: torch.Tensor) -> list:
-    """Batch, head and position strides; 0 where a dimension has one entry, whose stride says nothing."""
-    return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
-
-
-def _require_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, batch: int, kv_heads, head_dim: int, fmt):
-    """Checks a cache against the batch that uses it; (format, pages, block, max_blocks, table stride)."""
+def _require_cache(index, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, batch, kv_heads, head_dim, fmt):
+    """Checks a cache against the batch that uses it; (format, pages, heads, block, max_blocks, table stride)."""
     f = fmt_code(fmt)
+    shape = k_cache.shape
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        require_input(t, name)
-        if t.dtype not in (torch.uint8, torch.int8, _F8_DTYPE[f]):
-            raise RuntimeError(f"{name} must hold {fmt} codes (uint8, int8 or {_F8_DTYPE[f]}), got {t.dtype}")
-        if t.dim() != 4:
+        _require_on(index, t, name)
+        dtype = t.dtype
+        if dtype is not _F8_DTYPE[f] and dtype not in _BYTES8:
+            raise RuntimeError(f"{name} must hold {fmt} codes (uint8, int8 or {_F8_DTYPE[f]}), got {dtype}")
+        if len(shape) != 4:
             raise RuntimeError(f"{name} must be 4D: [pages, kv_heads, block, head_dim]")
-    if k_cache.shape != v_cache.shape:
+    if shape != v_cache.shape:
         raise RuntimeError("k_cache and v_cache must have the same shape")
-    pages, heads, block, d = k_cache.shape
+    pages, heads, block, d = shape
     if d != head_dim or (kv_heads is not None and heads != kv_heads):
         raise RuntimeError(f"the cache holds {heads} heads of {d}; the call has {kv_heads or heads} of {head_dim}")
     for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        require_input(t, name)
-        if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads):
+        _require_on(index, t, name)
+        if t.dtype is not torch.float32 or t.shape != (pages, heads):
             raise RuntimeError(f"{name} must be fp32 with shape {(pages, heads)}")
-    require_cuda(block_table, "block_table")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
+    if block_table.get_device() != index:
+        _require_on(index, block_table, "block_table")
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
         raise RuntimeError(f"block_table must be int32 with shape [{batch}, max_blocks]")
     width = block_table.shape[1]
-    if width > 1 and block_table.stride(1) != 1:
+    stride, inner = block_table.stride()
+    if width > 1 and inner != 1:
         raise RuntimeError("block_table must have contiguous rows")
-    _require_int32(seq_lens, "seq_lens", batch)
-    return f, pages, block, width, max(block_table.stride(0), width) if batch > 1 else width
+    _require_int32(index, seq_lens, "seq_lens", batch)
+    return f, pages, heads, block, width, stride if batch > 1 else width
 
 
-def kv8_workspace(device, nbytes: int) -> torch.Tensor:
+@functools.lru_cache(maxsize=4096)
+def _kv8_ws_bytes(index: int, batch: int, heads: int, kv_heads: int, queries: int, head_dim: int) -> int:
+    with torch.cuda.device(index):
+        return int(lib().wbk_attention_kv8_ws_bytes(batch, heads, kv_heads, queries, head_dim))
+
+
+def kv8_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """The per-device workspace of attention_kv8 (zero-filled once, grown on demand), shared by its calls on the
     device: calls that may run at the same time need workspaces of their own."""
-    dev = torch.device(device)
-    ws = _KV8_WS.get(dev)
+    ws = _KV8_WS.get(device)
     if ws is None or ws.numel() < nbytes:
-        ws = _KV8_WS[dev] = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+        ws = _KV8_WS[device] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
     return ws
 
 
@@ -556,21 +596,19 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
     one, the page's older codes are rescaled. Tokens past the table, or whose page
     is outside the pool, are not stored. seq_lens is not changed.
     """
-    dt = _require_bhsd(k, "k")
-    if _require_bhsd(v, "v") != dt or v.shape != k.shape:
-        raise RuntimeError("k and v must have the same shape and dtype")
-    B, H, T, D = k.shape
-    f, pages, block, width, ts = _require_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, B, H, D, fmt)
+    dt, index, shape, ks3 = _require_bhsd(k, "k")
+    vdt, vindex, vshape, vs3 = _require_bhsd(v, "v")
+    if vdt != dt or vshape != shape or vindex != index:
+        raise RuntimeError("k and v must have the same shape and dtype, on one device")
+    B, H, T, D = shape
+    f, pages, _, block, width, ts = _require_cache(index, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, B, H,
+                                                   D, fmt)
     if new_lens is not None:
-        _require_int32(new_lens, "new_lens", B)
-    require_same_device(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, new_lens)
-    strides = (ctypes.c_int64 * 6)(*(_strides3(k) + _strides3(v)))
-    with torch.cuda.device(k.device):
-        check(lib().wbk_kv8_append(k.data_ptr(), v.data_ptr(), dt, B, H, T, D, strides, f, k_cache.data_ptr(),
-                                   v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, block,
-                                   block_table.data_ptr(), width, ts, seq_lens.data_ptr(), ptr(new_lens),
-                                   stream_of(k)), "kv8_append")
-    _count()
+        _require_int32(index, new_lens, "new_lens", B)
+    _launch(lib().wbk_kv8_append,
+            (k.data_ptr(), v.data_ptr(), dt, B, H, T, D, _I64X6(*ks3, *vs3), f, k_cache.data_ptr(), v_cache.data_ptr(),
+             k_scale.data_ptr(), v_scale.data_ptr(), pages, block, block_table.data_ptr(), width, ts,
+             seq_lens.data_ptr(), None if new_lens is None else new_lens.data_ptr()), index, "kv8_append")
 
 
 def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -592,30 +630,33 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     shared one, so such calls must not run concurrently on different streams
     without a workspace of their own.
     """
-    dt = _require_bhsd(q, "q")
-    B, H, T, D = q.shape
-    f, pages, block, width, ts = _require_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, B, None, D, fmt)
-    kv_heads = k_cache.shape[1]
+    dt, index, shape, qs3 = _require_bhsd(q, "q")
+    B, H, T, D = shape
+    f, pages, kv_heads, block, width, ts = _require_cache(index, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
+                                                          B, None, D, fmt)
     if kv_heads == 0 or H % kv_heads != 0:
         raise RuntimeError(f"{H} query heads do not share {kv_heads} KV heads evenly")
     if q_lens is not None:
-        _require_int32(q_lens, "q_lens", B)
-    o = torch.empty((B, H, T, D), dtype=q.dtype, device=q.device) if out is None else out
-    if o.shape != q.shape or _require_bhsd(o, "out") != dt:
-        raise RuntimeError(f"out must be a {q.dtype} view of shape {tuple(q.shape)}")
-    require_same_device(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, q_lens, o, workspace)
-    strides = (ctypes.c_int64 * 6)(*(_strides3(q) + _strides3(o)))
-    sc = float(scale) if scale is not None else D ** -0.5
-    with torch.cuda.device(q.device):
-        need = lib().wbk_attention_kv8_ws_bytes(B, H, kv_heads, T, D)
-        ws = workspace if workspace is not None else kv8_workspace(q.device, need)
-        check(lib().wbk_attention_kv8(q.data_ptr(), o.data_ptr(), dt, B, H, kv_heads, T, D, strides, f,
-                                      k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                      pages, block, block_table.data_ptr(), width, ts, seq_lens.data_ptr(),
-                                      ptr(q_lens), int(bool(causal)), sc, ptr(ws),
-                                      0 if ws is None else ws.numel() * ws.element_size(), stream_of(q)),
-              "attention_kv8")
-    _count()
+        _require_int32(index, q_lens, "q_lens", B)
+    if out is None:
+        o = torch.empty(shape, dtype=q.dtype, device=q.device)
+        os3 = (H * T * D, T * D, D)
+    else:
+        o = out
+        odt, oindex, oshape, os3 = _require_bhsd(o, "out")
+        if odt != dt or oindex != index or oshape != shape:
+            raise RuntimeError(f"out must be a {q.dtype} view of shape {tuple(shape)} on {q.device}")
+    need = _kv8_ws_bytes(index, B, H, kv_heads, T, D)
+    if workspace is None:
+        workspace = kv8_workspace(q.device, need)
+    else:
+        _require_on(index, workspace, "workspace")
+    _launch(lib().wbk_attention_kv8,
+            (q.data_ptr(), o.data_ptr(), dt, B, H, kv_heads, T, D, _I64X6(*qs3, *os3), f, k_cache.data_ptr(),
+             v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, block, block_table.data_ptr(), width, ts,
+             seq_lens.data_ptr(), None if q_lens is None else q_lens.data_ptr(), 1 if causal else 0,
+             D ** -0.5 if scale is None else float(scale), workspace.data_ptr(),
+             workspace.numel() * workspace.element_size()), index, "attention_kv8")
     return o
 
 
@@ -624,14 +665,26 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
 _DT_LOGITS = {torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.float32: DT_F32}
 
 
-def _per_row(value, name: str, dtype: torch.dtype, rows: int):
-    """(number for every row, device array or None)."""
+def _per_row(index: int, value, name: str, dtype: torch.dtype, rows: int):
+    """(number for every row, address of a device array or None)."""
     if isinstance(value, torch.Tensor):
-        require_input(value, name)
-        if value.dtype != dtype or value.numel() != rows or value.dim() != 1:
+        _require_on(index, value, name)
+        if value.dtype is not dtype or value.dim() != 1 or value.shape[0] != rows:
             raise RuntimeError(f"{name} must be a number or a {dtype} tensor of shape [{rows}]")
-        return 0, value
+        return 0, value.data_ptr()
+    if not value >= 0:
+        raise ValueError(f"{name} must not be negative, got {value}")
     return value, None
+
+
+def _require_rows(index: int, t: torch.Tensor, name: str) -> int:
+    """The row stride of a [B, V] tensor on CUDA device `index` whose rows are contiguous."""
+    if t.get_device() != index:
+        _require_on(index, t, name)
+    (rows, width), (stride, inner) = t.shape, t.stride()
+    if width > 1 and inner != 1:
+        raise RuntimeError(f"{name} must have contiguous rows")
+    return stride if rows > 1 else width
 
 
 def sample(logits: torch.Tensor, noise: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
@@ -649,36 +702,36 @@ def sample(logits: torch.Tensor, noise: torch.Tensor, temperature=1.0, top_k=0, 
     under the unfiltered softmax of the logits as given. A row with no logit above
     -inf gives token -1 and logprob -inf.
     """
-    require_cuda(logits, "logits")
-    if logits.dtype not in _DT_LOGITS:
+    index = logits.get_device()
+    if index < 0:
+        require_cuda(logits, "logits")
+    dt = _DT_LOGITS.get(logits.dtype)
+    if dt is None:
         raise RuntimeError(f"logits must be fp16, bf16 or fp32, got {logits.dtype}")
     if logits.dim() != 2:
         raise RuntimeError("logits must be 2-D [B, V]")
     B, V = logits.shape
-    require_cuda(noise, "noise")
-    if noise.dtype != torch.float32 or noise.shape != logits.shape:
+    if noise.dtype is not torch.float32 or noise.shape != logits.shape:
         raise RuntimeError(f"noise must be fp32 with shape {(B, V)}")
-    for t, name in ((logits, "logits"), (noise, "noise")):
-        if V > 1 and t.stride(1) != 1:
-            raise RuntimeError(f"{name} must have contiguous rows")
-    t_all, t_row = _per_row(temperature, "temperature", torch.float32, B)
-    k_all, k_row = _per_row(top_k, "top_k", torch.int32, B)
-    p_all, p_row = _per_row(top_p, "top_p", torch.float32, B)
-    m_all, m_row = _per_row(min_p, "min_p", torch.float32, B)
-    if not (t_all >= 0 and k_all >= 0 and p_all >= 0 and m_all >= 0):
-        raise ValueError("temperature, top_k, top_p and min_p must not be negative")
-    tok = torch.empty(B, dtype=torch.int64, device=logits.device) if tokens_out is None else tokens_out
-    lp = torch.empty(B, dtype=torch.float32, device=logits.device) if logprobs_out is None else logprobs_out
-    for t, name, dtype in ((tok, "tokens_out", torch.int64), (lp, "logprobs_out", torch.float32)):
-        require_input(t, name)
-        if t.dtype != dtype or tuple(t.shape) != (B,):
-            raise RuntimeError(f"{name} must be {dtype} with shape [{B}]")
-    require_same_device(logits, noise, t_row, k_row, p_row, m_row, tok, lp)
-    with torch.cuda.device(logits.device):
-        check(lib().wbk_sample(logits.data_ptr(), _DT_LOGITS[logits.dtype], B, V,
-                               max(logits.stride(0), V) if B > 1 else V, noise.data_ptr(),
-                               max(noise.stride(0), V) if B > 1 else V, ptr(t_row), ptr(k_row), ptr(p_row),
-                               ptr(m_row), float(t_all), min(int(k_all), 2 ** 31 - 1), float(p_all), float(m_all),
-                               tok.data_ptr(), lp.data_ptr(), stream_of(logits)), "sample")
-    _count()
-    return tok, lp
+    ls, ns = _require_rows(index, logits, "logits"), _require_rows(index, noise, "noise")
+    t_all, t_row = _per_row(index, temperature, "temperature", torch.float32, B)
+    k_all, k_row = _per_row(index, top_k, "top_k", torch.int32, B)
+    p_all, p_row = _per_row(index, top_p, "top_p", torch.float32, B)
+    m_all, m_row = _per_row(index, min_p, "min_p", torch.float32, B)
+    if tokens_out is None:
+        tokens_out = torch.empty(B, dtype=torch.int64, device=logits.device)
+    elif tokens_out.dtype is not torch.int64 or tokens_out.shape != (B,):
+        raise RuntimeError(f"tokens_out must be int64 with shape [{B}]")
+    else:
+        _require_on(index, tokens_out, "tokens_out")
+    if logprobs_out is None:
+        logprobs_out = torch.empty(B, dtype=torch.float32, device=logits.device)
+    elif logprobs_out.dtype is not torch.float32 or logprobs_out.shape != (B,):
+        raise RuntimeError(f"logprobs_out must be fp32 with shape [{B}]")
+    else:
+        _require_on(index, logprobs_out, "logprobs_out")
+    _launch(lib().wbk_sample,
+            (logits.data_ptr(), dt, B, V, ls, noise.data_ptr(), ns, t_row, k_row, p_row, m_row, t_all,
+             min(int(k_all), 2 ** 31 - 1), p_all, m_all, tokens_out.data_ptr(), logprobs_out.data_ptr()),
+            index, "sample")
+    return tokens_out, logprobs_out
