@@ -50,12 +50,14 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kSliceElems = 8192;       // per CTA, if a cluster of kMaxCluster allows
-constexpr int kSliceBytes = 100 * 1024; // most that is kept in shared memory (two CTAs per SM)
+constexpr int kCtasPerSm = 2;
+constexpr int kLeastSlice = 2048;       // tokens per CTA, below which a row is not split further
+constexpr int kSliceElems = 25600;      // most tokens per CTA kept in shared memory (two CTAs per SM)
 constexpr int kList = 2048;             // most tokens that one CTA sorts
 constexpr int kBins = kThreads;
 constexpr float kBinsPerUnit = 16.0f;
 constexpr int kRounds = 6;
+constexpr int kAhead = 8;               // loads in flight per thread
 // Error of the approximate race in log2 units: two roundings of a product up to 150 (tokens below 2^-149 have
 // p = 0), 1.8e-5, and of a logarithm up to 126, 0.8e-5, plus the approximate logarithm's 2^-22.
 constexpr float kNear = 1e-4f;
@@ -76,15 +78,14 @@ struct SampleParams {
   float* logprobs;
 };
 
-// Logit as an ordered fp32: NaN is never drawn (-inf), +inf is the largest finite
-// number, -0 is +0.
+// A logit as it is ordered: NaN is never drawn (-inf, fmaxf returns the operand that
+// is not NaN), +inf is the largest finite number, -0 is +0.
+__device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), 3.402823466e38f) + 0.0f; }
 template <int kDtype>
 __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
-  float x;
-  if constexpr (kDtype == WBK_DT_F32) x = static_cast<const float*>(p)[i];
-  else if constexpr (kDtype == WBK_DT_F16) x = __half2float(static_cast<const __half*>(p)[i]);
-  else x = __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return isnan(x) ? -INFINITY : fminf(x, 3.402823466e38f) + 0.0f;
+  if constexpr (kDtype == WBK_DT_F32) return clean(static_cast<const float*>(p)[i]);
+  else if constexpr (kDtype == WBK_DT_F16) return clean(__half2float(static_cast<const __half*>(p)[i]));
+  else return clean(__bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]));
 }
 
 // Order-preserving key of an fp32 and back, and the place of token i in its row's
@@ -118,45 +119,76 @@ __device__ __forceinline__ uint64_t warp_max_u64(uint64_t v) {
   return v;
 }
 
-// What a CTA tells its cluster in one exchange, and what it keeps for itself. All
-// sums run in a fixed order (thread, warp, rank), so equal inputs give equal bits.
+// What a CTA tells its cluster in one exchange. All sums run in a fixed order
+// (thread, warp, rank), so equal inputs give equal bits.
 struct Message {
-  uint64_t u;
-  float f, g;
-  int c;
+  uint64_t u;  // maximum
+  float f, g;  // sums
+  int c;       // sum
+  float l;     // the logit of the token that u names, filled in by the CTA
 };
 struct SampleSmem {
   Message warp[kWarps];
   Message said[2];          // exchanges alternate between the two
   int bins[kBins];          // this CTA's counts
-  int all[kBins];           // the row's
-  int count;
+  int all[kBins];           // the row's, summed up within each 32
+  int count;                // of rank 0: entries of its list
   float scan[kWarps];
   uint64_t list[kList];     // of rank 0: places
   float mass[kList];
 };
 
-// Joins every thread's (max u, sum f, sum g, sum c) over the CTA and the cluster.
-__device__ __forceinline__ Message exchange(Message m, SampleSmem& s, cg::cluster_group& cluster, int& turn) {
+// The key of a non-negative score above the index that breaks ties.
+__device__ __forceinline__ uint64_t score_place(float score, int i) {
+  return (static_cast<uint64_t>(__float_as_uint(score)) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(i));
+}
+
+// A row as one CTA of its cluster sees it: tokens [begin, end). x points at the
+// cleaned slice in shared memory, or at the row's own logits.
+template <int kDtype, bool kResident>
+struct Row {
+  const void* x;
+  const float* noise;  // the whole row's
+  int begin, end;
+  float top, temperature, scale;  // scale = log2(e) / temperature
+
+  __device__ __forceinline__ float logit(int i) const {
+    if constexpr (kResident) return static_cast<const float*>(x)[i - begin];
+    else return load_logit<kDtype>(x, i);
+  }
+  __device__ __forceinline__ float weight(float l) const { return expf((l - top) / temperature); }
+  __device__ __forceinline__ float score(float l, int i) const { return weight(l) / fmaxf(noise[i], kMinNoise); }
+};
+
+__device__ __forceinline__ Message warp_join(Message m) {
   m.u = warp_max_u64(m.u);
   m.f = warp_sum(m.f);
   m.g = warp_sum(m.g);
   m.c = __reduce_add_sync(~0u, m.c);
+  return m;
+}
+
+// Joins every thread's (max u, sum f, sum g, sum c) over the CTA, and says it to the
+// cluster: complete after the next cluster.sync().
+template <class R>
+__device__ __forceinline__ void say(Message m, const R& r, SampleSmem& s, int turn) {
+  m = warp_join(m);
   if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5] = m;
   __syncthreads();
   if (threadIdx.x < 32) {
-    m = threadIdx.x < kWarps ? s.warp[threadIdx.x] : Message{0, 0.0f, 0.0f, 0};
-    m.u = warp_max_u64(m.u);
-    m.f = warp_sum(m.f);
-    m.g = warp_sum(m.g);
-    m.c = __reduce_add_sync(~0u, m.c);
+    m = warp_join(threadIdx.x < kWarps ? s.warp[threadIdx.x] : Message{0, 0.0f, 0.0f, 0, 0.0f});
+    const int token = place_index(m.u);
+    m.l = token >= r.begin && token < r.end ? r.logit(token) : 0.0f;
     if (threadIdx.x == 0) s.said[turn] = m;
   }
-  cluster.sync();
-  Message r{0, 0.0f, 0.0f, 0};
+}
+// What the cluster said, joined. A message is overwritten two exchanges later, when
+// every CTA has passed the cluster.sync() in between.
+__device__ __forceinline__ Message hear(SampleSmem& s, cg::cluster_group& cluster, int& turn) {
+  Message r{0, 0.0f, 0.0f, 0, 0.0f};
   for (unsigned i = 0; i < cluster.num_blocks(); ++i) {
-    const Message& o = *cluster.map_shared_rank(&s.said[turn], i);
-    r.u = max(r.u, o.u);
+    const Message o = *cluster.map_shared_rank(&s.said[turn], i);
+    if (o.u > r.u) r.u = o.u, r.l = o.l;
     r.f += o.f;
     r.g += o.g;
     r.c += o.c;
@@ -164,58 +196,42 @@ __device__ __forceinline__ Message exchange(Message m, SampleSmem& s, cg::cluste
   turn ^= 1;
   return r;
 }
-
-// The key of a non-negative score above the index that breaks ties.
-__device__ __forceinline__ uint64_t score_place(float score, int i) {
-  return (static_cast<uint64_t>(__float_as_uint(score)) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(i));
+template <class R>
+__device__ __forceinline__ Message exchange(const Message& m, const R& r, SampleSmem& s, cg::cluster_group& cluster,
+                                            int& turn) {
+  say(m, r, s, turn);
+  cluster.sync();
+  return hear(s, cluster, turn);
 }
 
-// A row as its cluster sees it.
-template <int kDtype, bool kResident>
-struct Row {
-  const void* x;       // the CTA's slice: of shared memory, or of the row itself
-  const float* noise;  // the whole row's
-  int begin, end;      // the CTA's tokens
-  float top, temperature, scale;  // scale = log2(e) / temperature
-
-  __device__ __forceinline__ float logit(int i) const { return load_logit<kDtype>(x, i - begin); }
-  __device__ __forceinline__ float weight(float l) const { return expf((l - top) / temperature); }
-  __device__ __forceinline__ float score(float l, int i) const { return weight(l) / fmaxf(noise[i], kMinNoise); }
-};
-
-// The race among the tokens placed before (above) `limit`: score_place of the CTA's
-// winner in full evaluation, 0 if it has no token there; and per thread, where
-// asked, the sum of exp(l - top) and of exp((l - top) / temperature).
-template <int kDtype, bool kResident, bool kSums>
-__device__ __forceinline__ uint64_t race(const Row<kDtype, kResident>& r, uint64_t limit, float least, SampleSmem& s,
-                                         float& raw, float& all) {
+// The race among the tokens placed before (above) `limit` (0: all): score_place of
+// the CTA's winner in full evaluation, 0 if it has no token there. kFirst: also, per
+// thread, the sums of exp(l - top) and, if asked, of exp((l - top) / temperature).
+template <bool kFirst, int kDtype, bool kResident>
+__device__ __forceinline__ uint64_t race(const Row<kDtype, kResident>& r, uint64_t limit, float least, bool mass,
+                                         SampleSmem& s, float& raw, float& all) {
   float best = -INFINITY, second = -INFINITY;
-  int best_i = -1;
-  // groups of four that are 16-byte aligned in the random numbers
-  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(r.noise + r.begin) >> 2) & 3);
-  for (int i0 = r.begin - shift + 4 * static_cast<int>(threadIdx.x); i0 < r.end; i0 += 4 * kThreads) {
-    float e[4];
-    if (i0 >= r.begin && i0 + 4 <= r.end) {
-      const float4 v = *reinterpret_cast<const float4*>(r.noise + i0);
-      e[0] = v.x, e[1] = v.y, e[2] = v.z, e[3] = v.w;
-    } else {
+  int best_i = r.end;
+  for (int i0 = r.begin + static_cast<int>(threadIdx.x); i0 < r.end; i0 += kAhead * kThreads) {
+    float e[kAhead];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) e[j] = i0 + j >= r.begin && i0 + j < r.end ? r.noise[i0 + j] : 1.0f;
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * kThreads;
+      e[j] = i < r.end ? r.noise[i] : 1.0f;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j;
-      if (i < r.begin || i >= r.end) continue;
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * kThreads;
+      if (i >= r.end) break;
       const float l = r.logit(i), gap = l - r.top, power = gap * r.scale;
-      if (kSums) {
+      if constexpr (kFirst) {
         raw += ex2(gap * kLog2e);
-        all += ex2(power);
+        if (mass) all += ex2(power);
       }
-      const float t = power - lg2(fmaxf(e[j], kMinNoise));
-      if (t > second && power >= least && (limit == 0 || place_of(l, i) > limit)) {
-        if (t > best) second = best, best = t, best_i = i;
-        else second = t;
-      }
+      float t = power - lg2(fmaxf(e[j], kMinNoise));
+      if (power < least || (limit != 0 && place_of(l, i) <= limit)) t = -INFINITY;
+      second = fmaxf(second, fminf(t, best));
+      if (t > best) best = t, best_i = i;
     }
   }
   // the CTA's largest, then full evaluation of all that come near it
@@ -224,65 +240,67 @@ __device__ __forceinline__ uint64_t race(const Row<kDtype, kResident>& r, uint64
   if ((threadIdx.x & 31) == 0) s.scan[threadIdx.x >> 5] = top;
   __syncthreads();
   for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s.scan[i]);
-  __syncthreads();
   uint64_t won = 0;
-  if (best_i >= 0 && best >= top - kNear) {
+  if (best > -INFINITY && best >= top - kNear) {
     won = score_place(r.score(r.logit(best_i), best_i), best_i);
     if (second >= top - kNear) {  // two of this thread's tokens are near: look at all of them again
-      for (int i0 = r.begin - shift + 4 * static_cast<int>(threadIdx.x); i0 < r.end; i0 += 4 * kThreads)
-        for (int i = max(i0, r.begin); i < min(i0 + 4, r.end); ++i) {
-          const float l = r.logit(i), power = (l - r.top) * r.scale;
-          if (l > -INFINITY && power >= least && (limit == 0 || place_of(l, i) > limit))
-            won = max(won, score_place(r.score(l, i), i));
-        }
+      for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
+        const float l = r.logit(i);
+        if (l > -INFINITY && (l - r.top) * r.scale >= least && place_of(l, i) > limit)
+          won = max(won, score_place(r.score(l, i), i));
+      }
     }
   }
   return won;
 }
 
-// The CTAs' counts in s.bins, added over the cluster: the first bin up to which they reach `least` (kBins where
-// none does), the sum up to there and the sum before it. Ends with the cluster in step.
+// The CTAs' counts in s.bins, added over the cluster: the first bin up to which they
+// reach `least` (kBins where none does), the sum up to there and the sum before it.
+// The counts were completed before a cluster.sync().
 struct Cut {
   int bin, upto, before;
 };
 __device__ __forceinline__ Cut cut_bins(int least, SampleSmem& s, cg::cluster_group& cluster) {
-  cluster.sync();
   int c = 0;
   for (unsigned i = 0; i < cluster.num_blocks(); ++i) c += *cluster.map_shared_rank(&s.bins[threadIdx.x], i);
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(~0u, c, o);
     if ((threadIdx.x & 31) >= o) c += y;
   }
-  s.all[threadIdx.x] = c;  // up to this bin, within its 32
-  cluster.sync();
+  s.all[threadIdx.x] = c;
+  __syncthreads();
   Cut r{kBins, 0, 0};
   for (int b0 = 0; b0 < kBins && r.bin == kBins; b0 += 32) {
     const int upto = r.upto + s.all[b0 + (threadIdx.x & 31)];
     const uint32_t enough = __ballot_sync(~0u, upto >= least);
     const int at = enough != 0 ? __ffs(enough) - 1 : 31;
-    r.before = enough != 0 && at > 0 ? __shfl_sync(~0u, upto, max(at - 1, 0)) : enough != 0 ? r.upto : 0;
+    const int prior = __shfl_sync(~0u, upto, max(at - 1, 0));
+    r.before = at > 0 ? prior : r.upto;
     r.upto = __shfl_sync(~0u, upto, at);
     if (enough != 0) r.bin = b0 + at;
   }
   return r;
 }
 
-// A place that the first top_k tokens lie before (above), and the number of tokens before it: top_k, or for
-// small top_k at most kList. By counts of the range that the last of them lies in, kBins-fold smaller each time.
+// A place that the first top_k tokens lie before (above), and the number of tokens
+// before it: top_k, or for small top_k at most kList. By counts of the range that the
+// last of them lies in, kBins-fold smaller each time.
 template <int kDtype, bool kResident>
-__device__ __forceinline__ uint64_t kth_limit(const Row<kDtype, kResident>& r, int top_k, uint64_t first, SampleSmem& s,
+__device__ __forceinline__ uint64_t kth_limit(const Row<kDtype, kResident>& r, int top_k, SampleSmem& s,
                                               cg::cluster_group& cluster, int& left) {
-  uint64_t lo = 0, hi = first;  // the last of the first top_k lies in (lo, hi]
-  int above = 0;                // tokens above hi
+  uint64_t lo = 0, hi = place_of(r.top, 0);  // the last of the first top_k lies in (lo, hi]
+  int above = 0;                             // tokens above hi
   for (;;) {
     int shift = 0;
     while (((hi - lo - 1) >> shift) >= kBins) ++shift;
+    cluster.sync();  // the counts of the step before were read
     s.bins[threadIdx.x] = 0;
     __syncthreads();
-    for (int i = r.begin + threadIdx.x; i < r.end; i += kThreads) {
+    for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
       const uint64_t place = place_of(r.logit(i), i);
       if (place > lo && place <= hi) atomicAdd(&s.bins[(hi - place) >> shift], 1);
     }
+    cluster.sync();
     const Cut cut = cut_bins(top_k - above, s, cluster);
     const uint64_t to = hi - (static_cast<uint64_t>(cut.bin) << shift);
     const uint64_t step = 1ull << shift;
@@ -298,12 +316,64 @@ __device__ __forceinline__ uint64_t kth_limit(const Row<kDtype, kResident>& r, i
 template <int kDtype, bool kResident>
 __device__ __forceinline__ Message before(const Row<kDtype, kResident>& r, uint64_t limit, SampleSmem& s,
                                           cg::cluster_group& cluster, int& turn) {
-  Message m{0, 0.0f, 0.0f, 0};
-  for (int i = r.begin + threadIdx.x; i < r.end; i += kThreads) {
+  Message m{0, 0.0f, 0.0f, 0, 0.0f};
+  for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
     const float l = r.logit(i);
     if (place_of(l, i) > limit) ++m.c, m.f += r.weight(l);
   }
-  return exchange(m, s, cluster, turn);
+  return exchange(m, r, s, cluster, turn);
+}
+
+// Bitonic sort of kPer * kThreads places, larger first, place m * kThreads + t in
+// v[m] of thread t: partners in other warps meet in shared memory, others in registers.
+template <int kPer>
+__device__ __forceinline__ void sort_places(uint64_t (&v)[kPer], int size, uint64_t* list) {
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      if (j >= kThreads) {
+        if constexpr (kPer > 1) {
+#pragma unroll
+          for (int m = 0; m < kPer; ++m) {
+            const int o = m ^ (j / kThreads);
+            if (o > m) {
+              const bool down = ((m * kThreads + static_cast<int>(threadIdx.x)) & k) == 0;
+              const uint64_t x = v[m];
+#pragma unroll
+              for (int q = 0; q < kPer; ++q)  // v[o], without an index that the compiler does not know
+                if (q == o && (x < v[q]) == down) v[m] = v[q], v[q] = x;
+            }
+          }
+        }
+        continue;
+      }
+      if (j >= 32) {
+#pragma unroll
+        for (int m = 0; m < kPer; ++m) list[m * kThreads + threadIdx.x] = v[m];
+        __syncthreads();
+      }
+#pragma unroll
+      for (int m = 0; m < kPer; ++m) {
+        const int i = m * kThreads + static_cast<int>(threadIdx.x);
+        const uint64_t y = j >= 32 ? list[i ^ j] : __shfl_xor_sync(~0u, v[m], j);
+        const bool larger = ((i & k) == 0) == ((i & j) == 0);
+        v[m] = larger ? max(v[m], y) : min(v[m], y);
+      }
+      if (j >= 32) __syncthreads();
+    }
+}
+template <int kPer>
+__device__ __forceinline__ void sort_list(int n, int size, uint64_t* list) {
+  uint64_t v[kPer];
+#pragma unroll
+  for (int m = 0; m < kPer; ++m) {
+    const int i = m * kThreads + static_cast<int>(threadIdx.x);
+    v[m] = i < n ? list[i] : 0;
+  }
+  __syncthreads();
+  sort_places<kPer>(v, size, list);
+#pragma unroll
+  for (int m = 0; m < kPer; ++m) list[m * kThreads + threadIdx.x] = v[m];
+  __syncthreads();
 }
 
 // Rank 0's list of n places, sorted, then every filter and the race among the kept:
@@ -314,20 +384,12 @@ __device__ __forceinline__ uint64_t finish(const Row<kDtype, kResident>& r, int 
                                            float whole, SampleSmem& s) {
   int size = 32;
   while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = 0;
-  __syncthreads();
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int t = threadIdx.x; t < size / 2; t += kThreads) {
-        const int a = 2 * t - (t & (j - 1)), b = a + j;
-        const uint64_t x = s.list[a], y = s.list[b];
-        if ((x < y) == ((a & k) == 0)) s.list[a] = y, s.list[b] = x;  // larger (earlier) first
-      }
-      __syncthreads();
-    }
+  if (size <= kThreads) sort_list<1>(n, size, s.list);
+  else if (size <= 2 * kThreads) sort_list<2>(n, size, s.list);
+  else sort_list<4>(n, size, s.list);
   const int kept = min(n, top_k);
   // running masses: each thread a run of the list, then over the threads
-  const int run = (kept + kThreads - 1) / kThreads, i0 = threadIdx.x * run, i1 = min(i0 + run, kept);
+  const int run = (kept + kThreads - 1) / kThreads, i0 = static_cast<int>(threadIdx.x) * run, i1 = min(i0 + run, kept);
   float own = 0.0f;
   for (int i = i0; i < i1; ++i) {
     s.mass[i] = r.weight(place_logit(s.list[i]));
@@ -346,35 +408,29 @@ __device__ __forceinline__ uint64_t finish(const Row<kDtype, kResident>& r, int 
     total += s.scan[i];
   }
   const double cut = static_cast<double>(top_p) * (whole >= 0.0f ? whole : total);
-  uint64_t won = 0;
+  uint64_t won = 0, place = 0;
   for (int i = i0; i < i1; ++i) {
     const float w = s.mass[i];
     if (i == 0 || ((top_p >= 1.0f || static_cast<double>(mass) < cut) && w >= min_p && place_logit(s.list[i]) > -INFINITY)) {
       const int token = place_index(s.list[i]);
-      won = max(won, score_place(w / fmaxf(r.noise[token], kMinNoise), token));
+      const uint64_t mine = score_place(w / fmaxf(r.noise[token], kMinNoise), token);
+      if (mine > won) won = mine, place = s.list[i];
     }
     mass += w;
   }
+  const uint64_t own_won = won;
   won = warp_max_u64(won);
   if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5].u = won;
   __syncthreads();
   for (int i = 0; i < kWarps; ++i) won = max(won, s.warp[i].u);
-  const int token = place_index(won);
-  // back to the place, for its logit
-  uint64_t place = 0;
-  for (int i = i0; i < i1; ++i)
-    if (place_index(s.list[i]) == token) place = s.list[i];
-  place = warp_max_u64(place);
+  if (own_won == won) s.list[0] = place;  // one thread: a token's score_place is its own
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5].u = place;
-  __syncthreads();
-  for (int i = 0; i < kWarps; ++i) place = max(place, s.warp[i].u);
-  return place;
+  return s.list[0];
 }
 
 // One cluster per row.
 template <int kDtype, bool kResident>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   SampleSmem& s = *reinterpret_cast<SampleSmem*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
@@ -387,108 +443,121 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   r.noise = p.noise + row * p.noise_stride;
   r.begin = min(rank * p.slice, p.vocab);
   r.end = min(r.begin + p.slice, p.vocab);
+
+  // ---- 1. the row's largest logit; the cleaned slice goes to shared memory
+  // whole 16-byte vectors [v0, v1) of the slice, and the few tokens before and after them
+  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(logits + static_cast<int64_t>(r.begin) * kItem) & 15) / kItem);
+  const int head = min((kVec - shift) % kVec, r.end - r.begin);
+  const int vecs = (r.end - r.begin - head) / kVec;
+  float* held = reinterpret_cast<float*>(smem_raw + (sizeof(SampleSmem) + 15) / 16 * 16) + (kVec - head) % kVec;
+  const uint8_t* from = logits + static_cast<int64_t>(r.begin + head) * kItem;
+  float top = -INFINITY;
+  for (int v0 = threadIdx.x; v0 < vecs; v0 += kAhead / 2 * kThreads) {
+    uint4 v[kAhead / 2];
+#pragma unroll
+    for (int j = 0; j < kAhead / 2; ++j)
+      if (v0 + j * kThreads < vecs) v[j] = reinterpret_cast<const uint4*>(from)[v0 + j * kThreads];
+#pragma unroll
+    for (int j = 0; j < kAhead / 2; ++j) {
+      if (v0 + j * kThreads >= vecs) break;
+      float f[kVec];
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        f[i] = load_logit<kDtype>(&v[j], i);
+        top = fmaxf(top, f[i]);
+      }
+      if constexpr (kResident) {
+        float4* to = reinterpret_cast<float4*>(held + head + (v0 + j * kThreads) * kVec);
+        to[0] = make_float4(f[0], f[1], f[2], f[3]);
+        if constexpr (kVec == 8) to[1] = make_float4(f[4], f[5], f[6], f[7]);
+      }
+    }
+  }
+  const int rest = r.end - r.begin - vecs * kVec;  // fewer than 2 * kVec tokens, the first `head` of them in front
+  if (static_cast<int>(threadIdx.x) < rest) {
+    const int i = static_cast<int>(threadIdx.x) < head ? threadIdx.x : vecs * kVec + threadIdx.x;
+    const float f = load_logit<kDtype>(logits, r.begin + i);
+    top = fmaxf(top, f);
+    if constexpr (kResident) held[i] = f;
+  }
+  r.x = kResident ? static_cast<const void*>(held) : logits;
+  s.bins[threadIdx.x] = 0;
+  if (threadIdx.x == 0) s.count = 0;
   const float temperature = p.temperature != nullptr ? p.temperature[row] : p.temperature_all;
   const float top_p = p.top_p != nullptr ? p.top_p[row] : p.top_p_all;
   const float min_p = p.min_p != nullptr ? p.min_p[row] : p.min_p_all;
   const int k_given = p.top_k != nullptr ? p.top_k[row] : p.top_k_all;
   const int top_k = k_given > 0 && k_given < p.vocab ? k_given : p.vocab;
-
-  // ---- 1. the first token of the order; the slice goes to shared memory
-  const uint8_t* slice = logits + static_cast<int64_t>(r.begin) * kItem;
-  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(slice) & 15) / kItem);  // slice begins so far into a vector
-  uint8_t* held = smem_raw + (sizeof(SampleSmem) + 15) / 16 * 16;
-  r.x = kResident ? static_cast<const void*>(held + shift * kItem) : slice;
-  Message m{0, 0.0f, 0.0f, 0};
-  for (int i0 = r.begin - shift + kVec * static_cast<int>(threadIdx.x); i0 < r.end; i0 += kVec * kThreads) {
-    if (i0 >= r.begin && i0 + kVec <= r.end) {
-      const uint4 v = *reinterpret_cast<const uint4*>(logits + static_cast<int64_t>(i0) * kItem);
-      if (kResident) *reinterpret_cast<uint4*>(held + (i0 - r.begin + shift) * kItem) = v;
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) m.u = max(m.u, place_of(load_logit<kDtype>(&v, j), i0 + j));
-    } else {
-      for (int i = max(i0, r.begin); i < min(i0 + kVec, r.end); ++i) {
-        if (kResident) {
-          if constexpr (kItem == 4) reinterpret_cast<float*>(held)[i - r.begin + shift] = reinterpret_cast<const float*>(logits)[i];
-          else reinterpret_cast<uint16_t*>(held)[i - r.begin + shift] = reinterpret_cast<const uint16_t*>(logits)[i];
-        }
-        m.u = max(m.u, place_of(load_logit<kDtype>(logits, i), i));
-      }
-    }
-  }
-  for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins[i] = 0;
-  if (threadIdx.x == 0) s.count = 0;
-  m = exchange(m, s, cluster, turn);
-  const uint64_t first = m.u;
-  r.top = place_logit(first);
   r.temperature = temperature;
   r.scale = fminf(kLog2e / temperature, 3e38f);
+  const Message none{0, 0.0f, 0.0f, 0, 0.0f};
+  Message m = none;
+  m.u = place_of(top, -1);  // no token's place
+  r.top = place_logit(exchange(m, r, s, cluster, turn).u);
 
-  uint64_t winner = first;  // a place
-  float raw = 0.0f;
+  uint64_t winner = 0;  // a place
+  float raw = 0.0f;     // sum of exp(l - top)
   const bool empty = r.top == -INFINITY;
   if (!empty && !(temperature > 0.0f)) {
-    for (int i = r.begin + threadIdx.x; i < r.end; i += kThreads) raw += ex2((r.logit(i) - r.top) * kLog2e);
-    raw = exchange(Message{0, raw, 0.0f, 0}, s, cluster, turn).f;
+    m = none;
+    for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
+      const float gap = r.logit(i) - r.top;
+      m.f += ex2(gap * kLog2e);
+      if (gap == 0.0f) m.u = max(m.u, place_of(r.top, i));
+    }
+    m = exchange(m, r, s, cluster, turn);
+    winner = m.u;
+    raw = m.f;
   } else if (!empty) {
-    const bool few = top_k <= kList && top_k < p.vocab;
-    const float least = min_p > 0.0f ? lg2(min_p) - kNear : -INFINITY;  // of log2 p, for the race
-    uint64_t limit = 0;       // every token at or after this place is out
-    int left = p.vocab;       // tokens before it
-    float whole = -1.0f;      // the mass top_p refers to
-    int cut_bin = -1;         // or: what is left are the tokens of the bins up to this
-    bool gather = false;      // what is left fits one CTA's list
-    if (few) {
+    const float least = min_p > 0.0f ? lg2(fminf(min_p, 1.0f)) - kNear : -INFINITY;  // of log2 p, for the race
+    uint64_t limit = 0;    // every token at or after this place is out
+    int left = p.vocab;    // tokens before it
+    float whole = -1.0f;   // the mass top_p refers to
+    int cut_bin = -1;      // or: what is left are the tokens of the bins up to this
+    bool gather = false;   // what is left fits one CTA's list
+    if (top_k <= kList && top_k < p.vocab) {
       // ---- 2a. count by distance from the maximum
-      for (int i = r.begin + threadIdx.x; i < r.end; i += kThreads) {
+      m = none;
+      for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
         const float gap = r.top - r.logit(i);
-        raw += ex2(-gap * kLog2e);
+        m.f += ex2(-gap * kLog2e);
         const float bin = gap * kBinsPerUnit;
         if (bin < kBins) atomicAdd(&s.bins[static_cast<int>(bin)], 1);
       }
-      raw = exchange(Message{0, raw, 0.0f, 0}, s, cluster, turn).f;
+      raw = exchange(m, r, s, cluster, turn).f;
       const Cut cut = cut_bins(top_k, s, cluster);
       gather = true;
       if (cut.bin < kBins && cut.upto <= kList) cut_bin = cut.bin, left = cut.upto;
-      else limit = kth_limit(r, top_k, first, s, cluster, left);  // far from the maximum, or many ties
-    }
-    if (!gather) {
+      else limit = kth_limit(r, top_k, s, cluster, left);  // far from the maximum, or many ties
+    } else {
       if (top_k < p.vocab) {
-        limit = kth_limit(r, top_k, first, s, cluster, left);
+        limit = kth_limit(r, top_k, s, cluster, left);
         whole = before(r, limit, s, cluster, turn).f;
       }
       // ---- 2b. rounds
-      uint64_t lo = 0, hi = first;  // the cut lies between these places, once halving has begun
       for (int round = 0;; ++round) {
-        float all = 0.0f, dummy = 0.0f;
-        Message w{0, 0.0f, 0.0f, 0};
+        float all = 0.0f;
+        Message w = none;
         if (round == 0) {
-          raw = 0.0f;
-          w.u = race<kDtype, kResident, true>(r, limit, least, s, raw, all);
-          w.f = raw;
-          w.g = all;
-          w = exchange(w, s, cluster, turn);
+          w.u = race<true>(r, limit, least, top_p < 1.0f && whole < 0.0f, s, w.f, w.g);
+          w = exchange(w, r, s, cluster, turn);
           raw = w.f;
           if (whole < 0.0f) whole = w.g;
         } else {
-          w.u = race<kDtype, kResident, false>(r, limit, least, s, dummy, dummy);
-          w = exchange(w, s, cluster, turn);
+          w.u = race<false>(r, limit, least, false, s, all, all);
+          w = exchange(w, r, s, cluster, turn);
         }
-        // the winner's place: its logit is with the CTA that has it
-        const int token = place_index(w.u);
-        Message mine{0, 0.0f, 0.0f, 0};
-        if (threadIdx.x == 0 && token >= r.begin && token < r.end) mine.u = place_of(r.logit(token), token);
-        winner = exchange(mine, s, cluster, turn).u;
-        if (winner == first) break;
-        const bool likely = r.weight(place_logit(winner)) >= min_p;
-        if (top_p >= 1.0f && likely) break;
+        winner = place_of(w.l, place_index(w.u));
+        if (top_p >= 1.0f && r.weight(w.l) >= min_p) break;
         const Message b = before(r, winner, s, cluster, turn);
-        if (likely && static_cast<double>(b.f) < static_cast<double>(top_p) * whole) break;
+        if (b.c == 0) break;  // the first token of the order is always kept
+        if (r.weight(w.l) >= min_p && (top_p >= 1.0f || static_cast<double>(b.f) < static_cast<double>(top_p) * whole)) break;
         limit = winner;
         left = b.c;
         gather = left <= kList;
         if (gather) break;
         if (round >= kRounds) {
-          lo = limit;
+          uint64_t lo = limit, hi = place_of(r.top, 0);  // the cut lies between these places
           while (hi - lo > 1 && left > kList) {
             const uint64_t mid = lo + (hi - lo) / 2;
             const Message c = before(r, mid, s, cluster, turn);
@@ -502,34 +571,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           gather = left <= kList;
           if (gather) break;
           // every token before `limit` is kept: one more race decides
-          w = Message{0, 0.0f, 0.0f, 0};
-          w.u = race<kDtype, kResident, false>(r, limit, -INFINITY, s, dummy, dummy);
-          w = exchange(w, s, cluster, turn);
-          const int last = place_index(w.u);
-          mine = Message{0, 0.0f, 0.0f, 0};
-          if (threadIdx.x == 0 && last >= r.begin && last < r.end) mine.u = place_of(r.logit(last), last);
-          winner = exchange(mine, s, cluster, turn).u;
+          w = none;
+          w.u = race<false>(r, limit, -INFINITY, false, s, all, all);
+          w = exchange(w, r, s, cluster, turn);
+          winner = place_of(w.l, place_index(w.u));
           break;
         }
       }
     }
     if (gather) {
-      // ---- gather what is left at rank 0: a run of its list for each CTA
-      Message mine{0, 0.0f, 0.0f, 0};
-      for (int i = r.begin + threadIdx.x; i < r.end; i += kThreads) {
-        const float l = r.logit(i);
-        if (cut_bin >= 0 ? (r.top - l) * kBinsPerUnit < cut_bin + 1 : place_of(l, i) > limit) ++mine.c;
-      }
-      exchange(mine, s, cluster, turn);  // said[turn ^ 1].c of each rank
-      int base = 0;
-      for (int i = 0; i < rank; ++i) base += cluster.map_shared_rank(&s.said[turn ^ 1], i)->c;
+      // ---- what is left goes to rank 0, in any order
       uint64_t* list = cluster.map_shared_rank(&s.list[0], 0);
-      for (int i = r.begin + threadIdx.x; i < r.end; i += kThreads) {
-        const float l = r.logit(i);
-        if (cut_bin >= 0 ? (r.top - l) * kBinsPerUnit < cut_bin + 1 : place_of(l, i) > limit) {
-          const int at = base + atomicAdd(&s.count, 1);
-          if (at < kList) list[at] = place_of(l, i);
-        }
+      int* count = cluster.map_shared_rank(&s.count, 0);
+      for (int i0 = r.begin; i0 < r.end; i0 += kThreads) {
+        const int i = i0 + static_cast<int>(threadIdx.x);
+        const float l = i < r.end ? r.logit(i) : 0.0f;
+        const bool in = i < r.end && (cut_bin >= 0 ? (r.top - l) * kBinsPerUnit < cut_bin + 1 : place_of(l, i) > limit);
+        const uint32_t who = __ballot_sync(~0u, in);
+        if (who == 0) continue;
+        const int lane = threadIdx.x & 31;
+        int at = 0;
+        if (lane == __ffs(who) - 1) at = atomicAdd(count, __popc(who));
+        at = __shfl_sync(~0u, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
+        if (in && at < kList) list[at] = place_of(l, i);
       }
       cluster.sync();
       if (rank == 0) winner = finish(r, min(left, kList), top_k, top_p, min_p, whole, s);
@@ -544,7 +608,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
 
 template <int kDtype, bool kResident>
 int launch_sample(const SampleParams& p, int64_t rows, int ctas, cudaStream_t stream) {
-  constexpr int kItem = kDtype == WBK_DT_F32 ? 4 : 2;
   constexpr int kFixed = (sizeof(SampleSmem) + 15) / 16 * 16;
   static std::mutex mu;
   static std::vector<char> configured;
@@ -555,7 +618,7 @@ int launch_sample(const SampleParams& p, int64_t rows, int ctas, cudaStream_t st
     if (static_cast<int>(configured.size()) <= dev) configured.resize(dev + 1, 0);
     if (!configured[dev]) {
       if (int e = cuda_check(cudaFuncSetAttribute(sample_kernel<kDtype, kResident>,
-                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + kSliceBytes + 32),
+                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + kSliceElems * 4 + 32),
                              "sample smem attribute"))
         return e;
       configured[dev] = 1;
@@ -564,7 +627,7 @@ int launch_sample(const SampleParams& p, int64_t rows, int ctas, cudaStream_t st
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = kFixed + (kResident ? p.slice * kItem + 32 : 0);
+  cfg.dynamicSmemBytes = kFixed + (kResident ? p.slice * 4 + 32 : 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -578,13 +641,17 @@ int launch_sample(const SampleParams& p, int64_t rows, int ctas, cudaStream_t st
 
 template <int kDtype>
 int dispatch_sample(SampleParams p, int64_t rows, cudaStream_t stream) {
-  constexpr int kItem = kDtype == WBK_DT_F32 ? 4 : 2;
+  // A row is split as far as keeps every CTA of all rows resident at once (a row alone is a chain of latencies, which
+  // smaller slices shorten: 51866 logits, one row: 8 CTAs), and as far as its slices need to fit shared memory.
+  const int64_t room = static_cast<int64_t>(sm_count() > 0 ? sm_count() : 148) * kCtasPerSm;
   int ctas = 1;
-  while (ctas < kMaxCluster && (p.vocab + ctas - 1) / ctas > kSliceElems) ctas *= 2;
+  while (ctas < kMaxCluster && ((p.vocab + ctas - 1) / ctas > kSliceElems ||
+                                (p.vocab / (2 * ctas) >= kLeastSlice && rows * 2 * ctas <= room)))
+    ctas *= 2;
   p.slice = ((p.vocab + ctas - 1) / ctas + 7) / 8 * 8;
   if (rows * ctas > (int64_t(1) << 31) - 1) return fail(WBK_ERR_UNSUPPORTED, "wbk_sample: too many rows");
-  return static_cast<int64_t>(p.slice) * kItem <= kSliceBytes ? launch_sample<kDtype, true>(p, rows, ctas, stream)
-                                                              : launch_sample<kDtype, false>(p, rows, ctas, stream);
+  return p.slice <= kSliceElems ? launch_sample<kDtype, true>(p, rows, ctas, stream)
+                                : launch_sample<kDtype, false>(p, rows, ctas, stream);
 }
 
 }  // namespace
