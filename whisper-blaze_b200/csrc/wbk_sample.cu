@@ -20,12 +20,12 @@
 //   2. sum of exp(l - M), for the log-probability, and either
 //      a. top_k up to kList: a count of the tokens by floor((M - l) * 16); the bins that
 //         hold the first top_k tokens (found by finer counts where these are not
-//         enough) are gathered and sorted by one CTA, which
-//         applies every filter and runs the race among the few kept (the random
-//         numbers of all other tokens are not read); or
+//         enough) are gathered by one CTA, which applies every filter and runs the
+//         race among the few kept (the random numbers of all other tokens are not
+//         read); or
 //      b. the race among all tokens. Its winner is the answer if it is kept. If it
 //         is not, nothing after it in the order is kept either, so the race is run
-//         again among the tokens before it: gathered and sorted as in a. once they
+//         again among the tokens before it: gathered by one CTA as in a. once they
 //         are few, otherwise another round. A round throws away a random share of
 //         what is left, so rounds are few; after kRounds of them (random numbers
 //         made to defeat this) the cut is found by halving instead.
@@ -53,9 +53,10 @@ constexpr int kMaxCluster = 8;
 constexpr int kCtasPerSm = 2;
 constexpr int kLeastSlice = 2048;       // tokens per CTA, below which a row is not split further
 constexpr int kSliceElems = 25600;      // most tokens per CTA kept in shared memory (two CTAs per SM)
-constexpr int kList = 2048;             // most tokens that one CTA sorts
+constexpr int kList = 2048;             // most tokens that one CTA gathers
 constexpr int kBins = kThreads;
 constexpr float kBinsPerUnit = 16.0f;
+constexpr int kNearBins = 128;          // of the first count: tokens within 8 of the maximum
 constexpr int kRounds = 6;
 constexpr int kAhead = 8;               // loads in flight per thread
 // Error of the approximate race in log2 units: two roundings of a product up to 150 (tokens below 2^-149 have
@@ -135,7 +136,6 @@ struct SampleSmem {
   int count;                // of rank 0: entries of its list
   float scan[kWarps];
   uint64_t list[kList];     // of rank 0: places
-  float mass[kList];
 };
 
 // The key of a non-negative score above the index that breaks ties.
@@ -254,15 +254,13 @@ __device__ __forceinline__ uint64_t race(const Row<kDtype, kResident>& r, uint64
   return won;
 }
 
-// The CTAs' counts in s.bins, added over the cluster: the first bin up to which they
-// reach `least` (kBins where none does), the sum up to there and the sum before it.
-// The counts were completed before a cluster.sync().
+// Of a count per thread (cut_sums), or the CTAs' counts in s.bins added over the
+// cluster, completed before a cluster.sync() (cut_bins): the first bin up to which
+// they reach `least` (kBins where none does), the sum up to it and the sum before it.
 struct Cut {
   int bin, upto, before;
 };
-__device__ __forceinline__ Cut cut_bins(int least, SampleSmem& s, cg::cluster_group& cluster) {
-  int c = 0;
-  for (unsigned i = 0; i < cluster.num_blocks(); ++i) c += *cluster.map_shared_rank(&s.bins[threadIdx.x], i);
+__device__ __forceinline__ Cut cut_sums(int c, int least, SampleSmem& s) {
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(~0u, c, o);
     if ((threadIdx.x & 31) >= o) c += y;
@@ -280,6 +278,11 @@ __device__ __forceinline__ Cut cut_bins(int least, SampleSmem& s, cg::cluster_gr
     if (enough != 0) r.bin = b0 + at;
   }
   return r;
+}
+__device__ __forceinline__ Cut cut_bins(int least, SampleSmem& s, cg::cluster_group& cluster) {
+  int c = 0;
+  for (unsigned i = 0; i < cluster.num_blocks(); ++i) c += *cluster.map_shared_rank(&s.bins[threadIdx.x], i);
+  return cut_sums(c, least, s);
 }
 
 // A place that the first top_k tokens lie before (above), and the number of tokens
@@ -324,108 +327,94 @@ __device__ __forceinline__ Message before(const Row<kDtype, kResident>& r, uint6
   return exchange(m, r, s, cluster, turn);
 }
 
-// Bitonic sort of kPer * kThreads places, larger first, place m * kThreads + t in
-// v[m] of thread t: partners in other warps meet in shared memory, others in registers.
-template <int kPer>
-__device__ __forceinline__ void sort_places(uint64_t (&v)[kPer], int size, uint64_t* list) {
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      if (j >= kThreads) {
-        if constexpr (kPer > 1) {
-#pragma unroll
-          for (int m = 0; m < kPer; ++m) {
-            const int o = m ^ (j / kThreads);
-            if (o > m) {
-              const bool down = ((m * kThreads + static_cast<int>(threadIdx.x)) & k) == 0;
-              const uint64_t x = v[m];
-#pragma unroll
-              for (int q = 0; q < kPer; ++q)  // v[o], without an index that the compiler does not know
-                if (q == o && (x < v[q]) == down) v[m] = v[q], v[q] = x;
-            }
-          }
-        }
-        continue;
-      }
-      if (j >= 32) {
-#pragma unroll
-        for (int m = 0; m < kPer; ++m) list[m * kThreads + threadIdx.x] = v[m];
-        __syncthreads();
-      }
-#pragma unroll
-      for (int m = 0; m < kPer; ++m) {
-        const int i = m * kThreads + static_cast<int>(threadIdx.x);
-        const uint64_t y = j >= 32 ? list[i ^ j] : __shfl_xor_sync(~0u, v[m], j);
-        const bool larger = ((i & k) == 0) == ((i & j) == 0);
-        v[m] = larger ? max(v[m], y) : min(v[m], y);
-      }
-      if (j >= 32) __syncthreads();
-    }
+__device__ __forceinline__ uint64_t block_max(uint64_t v, SampleSmem& s) {
+  v = warp_max_u64(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5].u = v;
+  __syncthreads();
+  for (int i = 0; i < kWarps; ++i) v = max(v, s.warp[i].u);
+  return v;
 }
-template <int kPer>
-__device__ __forceinline__ void sort_list(int n, int size, uint64_t* list) {
-  uint64_t v[kPer];
+__device__ __forceinline__ float block_sum(float v, SampleSmem& s) {
+  v = warp_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s.scan[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0f;
+  for (int i = 0; i < kWarps; ++i) v += s.scan[i];
+  return v;
+}
+
+// Every filter and the race among the n places of rank 0's list: the winner's place.
+// The last of the first top_k lies in (lo, hi]. `whole` is the mass that top_p refers to, or < 0: that of the first top_k.
+template <int kDtype, bool kResident>
+__device__ __forceinline__ uint64_t finish(const Row<kDtype, kResident>& r, int n, int top_k, uint64_t lo, uint64_t hi,
+                                           float top_p, float min_p, float whole, SampleSmem& s) {
+  constexpr int kPer = kList / kThreads;
+  uint64_t v[kPer];  // 0: none, or out
 #pragma unroll
   for (int m = 0; m < kPer; ++m) {
     const int i = m * kThreads + static_cast<int>(threadIdx.x);
-    v[m] = i < n ? list[i] : 0;
+    v[m] = i < n ? s.list[i] : 0;
   }
-  __syncthreads();
-  sort_places<kPer>(v, size, list);
+  if (n > top_k) {
+    // the place that top_k tokens lie above, as in kth_limit
+    int above = 0;
 #pragma unroll
-  for (int m = 0; m < kPer; ++m) list[m * kThreads + threadIdx.x] = v[m];
-  __syncthreads();
-}
-
-// Rank 0's list of n places, sorted, then every filter and the race among the kept:
-// the winner's place. `whole` is the mass that top_p refers to, or < 0: that of
-// the first top_k in the list.
-template <int kDtype, bool kResident>
-__device__ __forceinline__ uint64_t finish(const Row<kDtype, kResident>& r, int n, int top_k, float top_p, float min_p,
-                                           float whole, SampleSmem& s) {
-  int size = 32;
-  while (size < n) size <<= 1;
-  if (size <= kThreads) sort_list<1>(n, size, s.list);
-  else if (size <= 2 * kThreads) sort_list<2>(n, size, s.list);
-  else sort_list<4>(n, size, s.list);
-  const int kept = min(n, top_k);
-  // running masses: each thread a run of the list, then over the threads
-  const int run = (kept + kThreads - 1) / kThreads, i0 = static_cast<int>(threadIdx.x) * run, i1 = min(i0 + run, kept);
-  float own = 0.0f;
-  for (int i = i0; i < i1; ++i) {
-    s.mass[i] = r.weight(place_logit(s.list[i]));
-    own += s.mass[i];
-  }
-  float upto = own;
-  for (int o = 1; o < 32; o <<= 1) {
-    const float y = __shfl_up_sync(~0u, upto, o);
-    if ((threadIdx.x & 31) >= o) upto += y;
-  }
-  if ((threadIdx.x & 31) == 31) s.scan[threadIdx.x >> 5] = upto;
-  __syncthreads();
-  float total = 0.0f, mass = upto - own;
-  for (int i = 0; i < kWarps; ++i) {
-    if (i == static_cast<int>(threadIdx.x >> 5)) mass += total;
-    total += s.scan[i];
-  }
-  const double cut = static_cast<double>(top_p) * (whole >= 0.0f ? whole : total);
-  uint64_t won = 0, place = 0;
-  for (int i = i0; i < i1; ++i) {
-    const float w = s.mass[i];
-    if (i == 0 || ((top_p >= 1.0f || static_cast<double>(mass) < cut) && w >= min_p && place_logit(s.list[i]) > -INFINITY)) {
-      const int token = place_index(s.list[i]);
-      const uint64_t mine = score_place(w / fmaxf(r.noise[token], kMinNoise), token);
-      if (mine > won) won = mine, place = s.list[i];
+    for (int m = 0; m < kPer; ++m) above += __syncthreads_count(v[m] > hi);
+    for (int shift = 64; shift > 0;) {
+      for (shift = 0; ((hi - lo - 1) >> shift) >= kBins;) ++shift;
+      __syncthreads();
+      s.bins[threadIdx.x] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int m = 0; m < kPer; ++m)
+        if (v[m] > lo && v[m] <= hi) atomicAdd(&s.bins[(hi - v[m]) >> shift], 1);
+      __syncthreads();
+      const Cut cut = cut_sums(s.bins[threadIdx.x], top_k - above, s);
+      const uint64_t to = hi - (static_cast<uint64_t>(cut.bin) << shift), step = 1ull << shift;
+      lo = to - lo > step ? to - step : lo;
+      hi = to;
+      if (above + cut.upto == top_k) break;
+      above += cut.before;
     }
-    mass += w;
+#pragma unroll
+    for (int m = 0; m < kPer; ++m)
+      if (v[m] <= lo) v[m] = 0;
   }
-  const uint64_t own_won = won;
-  won = warp_max_u64(won);
-  if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5].u = won;
-  __syncthreads();
-  for (int i = 0; i < kWarps; ++i) won = max(won, s.warp[i].u);
-  if (own_won == won) s.list[0] = place;  // one thread: a token's score_place is its own
-  __syncthreads();
-  return s.list[0];
+  float w[kPer], own = 0.0f;
+  uint64_t score[kPer];
+#pragma unroll
+  for (int m = 0; m < kPer; ++m) {
+    w[m] = v[m] != 0 ? r.weight(place_logit(v[m])) : 0.0f;
+    own += w[m];
+    score[m] = 0;
+    if (v[m] != 0 && w[m] >= min_p && place_logit(v[m]) > -INFINITY) {
+      const int token = place_index(v[m]);
+      score[m] = score_place(w[m] / fmaxf(r.noise[token], kMinNoise), token);
+    }
+  }
+  if (whole < 0.0f && top_p < 1.0f) whole = block_sum(own, s);
+  const double cut = static_cast<double>(top_p) * whole;
+  for (uint64_t limit = 0;;) {
+    uint64_t best = 0;
+#pragma unroll
+    for (int m = 0; m < kPer; ++m)
+      if (v[m] > limit) best = max(best, score[m]);
+    best = block_max(best, s);
+#pragma unroll
+    for (int m = 0; m < kPer; ++m)
+      if (score[m] == best && v[m] > limit) s.list[0] = v[m];  // one thread: a token's score_place is its own
+    __syncthreads();
+    const uint64_t winner = s.list[0];
+    if (top_p >= 1.0f) return winner;
+    float mass = 0.0f;
+#pragma unroll
+    for (int m = 0; m < kPer; ++m)
+      if (v[m] > winner) mass += w[m];
+    if (static_cast<double>(block_sum(mass, s)) < cut) return winner;
+    limit = winner;
+  }
 }
 
 // One cluster per row.
@@ -498,7 +487,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
   uint64_t winner = 0;  // a place
   float raw = 0.0f;     // sum of exp(l - top)
   const bool empty = r.top == -INFINITY;
-  if (!empty && !(temperature > 0.0f)) {
+  const bool first_only = !(temperature > 0.0f) || !(top_p > 0.0f) || !(min_p <= 1.0f);  // nothing else is kept
+  if (!empty && first_only) {
     m = none;
     for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
       const float gap = r.logit(i) - r.top;
@@ -509,26 +499,35 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
     winner = m.u;
     raw = m.f;
   } else if (!empty) {
-    const float least = min_p > 0.0f ? lg2(fminf(min_p, 1.0f)) - kNear : -INFINITY;  // of log2 p, for the race
+    const float least = min_p > 0.0f ? lg2(min_p) - kNear : -INFINITY;  // of log2 p, for the race
     uint64_t limit = 0;    // every token at or after this place is out
     int left = p.vocab;    // tokens before it
     float whole = -1.0f;   // the mass top_p refers to
-    int cut_bin = -1;      // or: what is left are the tokens of the bins up to this
+    Cut cut{kBins, 0, 0};  // or: what is left are the tokens of the bins up to this, cut.before of them in the bins before
     bool gather = false;   // what is left fits one CTA's list
     if (top_k <= kList && top_k < p.vocab) {
-      // ---- 2a. count by distance from the maximum
+      // ---- 2a. count by distance from the maximum; the few tokens near it are enough as a rule
       m = none;
       for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
         const float gap = r.top - r.logit(i);
         m.f += ex2(-gap * kLog2e);
         const float bin = gap * kBinsPerUnit;
-        if (bin < kBins) atomicAdd(&s.bins[static_cast<int>(bin)], 1);
+        if (bin < kNearBins) atomicAdd(&s.bins[static_cast<int>(bin)], 1);
       }
       raw = exchange(m, r, s, cluster, turn).f;
-      const Cut cut = cut_bins(top_k, s, cluster);
+      cut = cut_bins(top_k, s, cluster);
+      if (cut.bin == kBins) {  // the tokens further away, too
+        cluster.sync();
+        for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
+          const float bin = (r.top - r.logit(i)) * kBinsPerUnit;
+          if (bin >= kNearBins && bin < kBins) atomicAdd(&s.bins[static_cast<int>(bin)], 1);
+        }
+        cluster.sync();
+        cut = cut_bins(top_k, s, cluster);
+      }
       gather = true;
-      if (cut.bin < kBins && cut.upto <= kList) cut_bin = cut.bin, left = cut.upto;
-      else limit = kth_limit(r, top_k, s, cluster, left);  // far from the maximum, or many ties
+      if (cut.bin < kBins && cut.upto <= kList) left = cut.upto;
+      else cut.bin = kBins, limit = kth_limit(r, top_k, s, cluster, left);  // still further, or many ties
     } else {
       if (top_k < p.vocab) {
         limit = kth_limit(r, top_k, s, cluster, left);
@@ -550,7 +549,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
         winner = place_of(w.l, place_index(w.u));
         if (top_p >= 1.0f && r.weight(w.l) >= min_p) break;
         const Message b = before(r, winner, s, cluster, turn);
-        if (b.c == 0) break;  // the first token of the order is always kept
         if (r.weight(w.l) >= min_p && (top_p >= 1.0f || static_cast<double>(b.f) < static_cast<double>(top_p) * whole)) break;
         limit = winner;
         left = b.c;
@@ -586,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
       for (int i0 = r.begin; i0 < r.end; i0 += kThreads) {
         const int i = i0 + static_cast<int>(threadIdx.x);
         const float l = i < r.end ? r.logit(i) : 0.0f;
-        const bool in = i < r.end && (cut_bin >= 0 ? (r.top - l) * kBinsPerUnit < cut_bin + 1 : place_of(l, i) > limit);
+        const bool in = i < r.end && (cut.bin < kBins ? (r.top - l) * kBinsPerUnit < cut.bin + 1 : place_of(l, i) > limit);
         const uint32_t who = __ballot_sync(~0u, in);
         if (who == 0) continue;
         const int lane = threadIdx.x & 31;
@@ -596,7 +594,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
         if (in && at < kList) list[at] = place_of(l, i);
       }
       cluster.sync();
-      if (rank == 0) winner = finish(r, min(left, kList), top_k, top_p, min_p, whole, s);
+      if (rank == 0) {
+        uint64_t hi = place_of(r.top, 0);
+        if (cut.bin < kBins) {  // the last of the first top_k lies in the last bin; one bin more on both sides covers rounding
+          if (cut.bin > 1) hi = place_of(r.top - (cut.bin - 1) / kBinsPerUnit, 0);
+          limit = static_cast<uint64_t>(order_key(r.top - (cut.bin + 2) / kBinsPerUnit)) << 32;
+        }
+        winner = finish(r, min(left, kList), top_k, limit, hi, top_p, min_p, whole, s);
+      }
     }
   }
   if (rank == 0 && threadIdx.x == 0) {
