@@ -4,21 +4,21 @@
 // What bounds it: 2 * head_dim bytes of codes per token and KV head, each used by
 // group * queries rows only, so HBM; nothing else may wait.
 //
-//   * The work is the list of 64-token tiles of all (sequence, KV head, block of
-//     rows) items, in that order. Every CTA takes an equal, contiguous share of the
+//   * The work is the list of 32-token tiles of all (sequence, KV head, block of 8
+//     rows) items, in that order. Every warp takes an equal, contiguous share of the
 //     list, whatever the lengths are -- they are read on the device -- so ragged
-//     batches and one long sequence fill the SMs alike. An item that lies in several
-//     CTAs is joined by the last of them to finish, in the order of the list.
-//   * One producer warp per CTA keeps a ring of tiles in flight with TMA (swizzled,
-//     so that the fragment loads below have no bank conflicts), looks pages and
-//     scales up 32 at a time and one batch ahead, and hands each 16 tokens their
-//     factors through shared memory.
-//   * Four compute warps share a tile's 16-token groups and the rows' 16-row groups.
-//     Scores and outputs are m16n8k16 fp16 products of the codes (exact in fp16)
-//     with fp32 sums: with at most 64 rows a 128-row tcgen05 tile would
-//     be mostly padding, and the tensor pipe is not what bounds this. The order of
-//     the channels within a product is free, so a lane's fragments of K are 16 or 32
-//     consecutive bytes of one token, and so are its outputs.
+//     batches and one long sequence fill the SMs alike. Warps share nothing but the
+//     items that lie in several of them: such an item is joined first by the last warp
+//     of a CTA to finish, through shared memory, then by the last of its CTAs, through
+//     global memory, always in the order of the list.
+//   * Each warp keeps a ring of tiles in flight with TMA (swizzled, so that the
+//     fragment loads below have no bank conflicts) and looks pages and scales up 32
+//     at a time and one batch ahead.
+//   * Scores and outputs are m16n8k16 fp16 products of the codes (exact in fp16) with
+//     fp32 sums, transposed: tokens (then channels) are the 16 rows, queries the 8
+//     columns. With 8 columns a 128-row tcgen05 tile would be mostly padding, and the
+//     tensor pipe is not what bounds this. The order of the channels within a
+//     product is free, so a lane's fragments are consecutive bytes of one token.
 //
 // Softmax in powers of two: with x_j = log2(e) * scale * q.k_j and a page's value
 // scale vs, the weight that meets the codes of V is w_j = 2^(x_j + log2 vs - m),
@@ -36,17 +36,20 @@
 namespace wbk {
 namespace {
 
-constexpr int kTile = 64;          // tokens per ring stage
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 32;          // tokens per ring stage
+constexpr int kTileLog2 = 5;
 constexpr int kGroups = kTile / 16;
-constexpr int kComputeWarps = 4;
-constexpr int kStepThreads = kComputeWarps * 32 + 32;
-constexpr int kMinTiles = 2;       // of a CTA's share, where the SMs are not full
+constexpr int kRows = 8;           // query rows per item
+constexpr int kSlots = 6;          // partial results that the warps of a CTA can have for one another
+constexpr int kMaxStages = 4;
+constexpr int kMinShare = 256;     // tokens of a CTA's share, where the SMs are not full: two tiles per warp
 constexpr float kRaise = 8.0f;     // log2 units
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint64_t kDrainNs = 100000000ull;  // limit of the waits for copies in flight after a wait gave up
 
-constexpr uint64_t kDrainNs = 100000000ull;  // limit of the waits for copies in flight at a CTA's end
-
-enum : uint32_t { KSITE_PRODUCER = 41, KSITE_COMPUTE = 42, KSITE_DRAIN = 43 };
+enum : uint32_t { KSITE_TILE = 41, KSITE_DRAIN = 42 };
 
 struct Kv8AttnParams {
   const void* q;
@@ -57,7 +60,9 @@ struct Kv8AttnParams {
   const int32_t* lens;
   const int32_t* q_lens;
   int batch, group, queries, rows;  // rows = group * queries of one KV head
-  int row_blocks;                   // blocks of 16 * kWR rows
+  int row_blocks;                   // blocks of kRows rows
+  int part_rows;                    // rows of a partial result: min(rows, kRows)
+  int stages;                       // of a warp's ring
   int causal, bf16;
   float scale_log2;  // scale * log2(e)
   uint32_t* tickets;
@@ -65,27 +70,16 @@ struct Kv8AttnParams {
   uint64_t timeout_ns;
 };
 
-template <int kD, int kWR>
-struct StepCfg {
-  static constexpr int kRows = 16 * kWR;
-  static constexpr int kCtasPerSm = kD == 64 ? 3 : 2;  // what the registers of a lane's fragments allow
-  static constexpr int kStages = kD == 64 ? 6 : kWR == 2 ? 5 : 6;  // and what then fits into shared memory
-  static constexpr int kTileBytes = kTile * kD;
-  static constexpr int kPartFloats = kRows * (kD + 2);  // one partial result: sums, maxima, totals
-};
-
-template <int kD, int kWR>
+// Shared memory: the rings (kWarps * stages tiles, 1024-byte aligned for the swizzle),
+// then this, then kSlots partial results.
 struct StepSmem {
-  static constexpr int kStages = StepCfg<kD, kWR>::kStages;
-  uint8_t k[kStages][kTile * kD];  // 1024-byte aligned (swizzle atoms)
-  uint8_t v[kStages][kTile * kD];
-  float4 factor[kStages][kGroups];  // of 16 tokens: key factor, log2 of the value scale, its inverse, 1 if there
-  float sum[kWR < 4 ? 16 * kWR * kD : 4];  // joins the compute warps of one row group
-  float max[kComputeWarps][16], total[kComputeWarps][16];
-  uint64_t full[kStages], empty[kStages];
-  int last;
+  float4 factor[kWarps][kMaxStages][kGroups];  // of 16 tokens: key factor, log2 of the value scale, its inverse, 1 if there
+  uint64_t full[kWarps][kMaxStages];
+  uint32_t tickets[kWarps];
   int abort_flag;
 };
+// A partial result: sums [part_rows][kD], then maxima and totals [part_rows], in whole 16-byte units.
+__host__ __device__ constexpr int part_floats(int rows, int d) { return rows * d + (2 * rows + 3) / 4 * 4; }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -100,29 +94,41 @@ __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Four codes -> two packed fp16 pairs (exact).
 template <int kFmt>
-__device__ __forceinline__ uint32_t half2_bits(uint32_t codes) {
-  const __half2 h = kv8_half2<kFmt>(codes);
-  return *reinterpret_cast<const uint32_t*>(&h);
+__device__ __forceinline__ uint2 codes_to_half(uint32_t w) {
+  uint2 r;
+  if constexpr (kFmt == WBK_FMT_E4M3)
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(r.x), "=r"(r.y) : "r"(w));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e5m2x2 %0, l;\n\tcvt.rn.f16x2.e5m2x2 %1, h;\n\t}"
+        : "=r"(r.x), "=r"(r.y) : "r"(w));
+  return r;
 }
 
 __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 __device__ __forceinline__ uint2 lds8(const uint8_t* p) { return *reinterpret_cast<const uint2*>(p); }
 
-__device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kComputeWarps * 32) : "memory"); }
+// The transposed 8 x 8 matrix of 16-bit values (row lane / 4, columns 2 * (lane % 4) and the next).
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 
-// One item of the work list: KV head h of sequence b, rows 16 * kWR * rb onwards.
+// One item of the work list: KV head h of sequence b, rows kRows * rb onwards.
 struct Item {
   int b, h, rb;
   int len, n;  // cached tokens, real query rows
-  int tiles;   // 64-token tiles, at least 1 (an item without tokens still writes its zeros)
+  int tiles;   // at least 1 (an item without tokens still writes its zeros)
 };
 
 __device__ __forceinline__ int tiles_of(const Kv8AttnParams& p, int b, int& len, int& n) {
   len = kv8_len(p.lens, b, p.c);
   n = p.q_lens != nullptr ? min(max(p.q_lens[b], 0), p.queries) : p.queries;
   if (n == 0) len = 0;
-  return max((len + kTile - 1) / kTile, 1);
+  return max((len + kTile - 1) >> kTileLog2, 1);
 }
 
 // Tiles of the whole list, by a converged warp.
@@ -198,421 +204,459 @@ __device__ __forceinline__ float log2_scale(float s) {
   return frac == 0 ? static_cast<float>(e) : log2f(s);
 }
 
-template <int kFmt, int kD, int kWR, bool kHalf>
-__global__ void __launch_bounds__(kStepThreads, StepCfg<kD, kWR>::kCtasPerSm)
+// A warp's loads: the place in its share that the next tile comes from, and the pages there.
+struct Loader {
+  Item it;
+  int tile, t1;       // next tile of the item, end of this warp's tiles of it
+  int blk0, te;       // cur covers the tiles up to te; its first page
+  int64_t x, x1;      // place in the list, end of the share
+  PageLane cur, nxt;  // this and the next batch of 32 pages
+
+  __device__ __forceinline__ int first_blk(const Kv8AttnParams& p, int t) const { return (t * kTile) >> p.c.block_log2; }
+  __device__ __forceinline__ void take(const Kv8AttnParams& p, const PageLane& pages) {
+    const int lane = threadIdx.x & 31;
+    cur = pages;
+    blk0 = first_blk(p, tile);
+    const int covered = ((blk0 + 32) << p.c.block_log2) >> kTileLog2;
+    te = min(t1, covered);
+    if (te < t1) {
+      nxt = fetch_page(p, it, first_blk(p, te) + lane);
+    } else if (x + (t1 - tile) < x1) {
+      Item n = it;
+      next_item(p, n);
+      nxt = fetch_page(p, n, lane);
+    }
+  }
+  __device__ __forceinline__ void start(const Kv8AttnParams& p, const Item& first, int t, int64_t begin, int64_t end) {
+    it = first;
+    tile = t;
+    x = begin;
+    x1 = end;
+    t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
+    nxt = PageLane{-1, 0.0f, 1.0f};
+    take(p, fetch_page(p, it, first_blk(p, tile) + (threadIdx.x & 31)));
+  }
+  // Loads the next tile into a stage of the ring.
+  template <int kD>
+  __device__ __forceinline__ void issue(const Kv8AttnParams& p, const CUtensorMap* tk, const CUtensorMap* tv, uint8_t* stage,
+                                        float4* factor, uint64_t* full) {
+    const int lane = threadIdx.x & 31;
+    const int pos = tile * kTile + (lane & (kGroups - 1)) * 16;  // of a 16-token group
+    const int from = ((pos >> p.c.block_log2) - blk0) & 31;
+    const int64_t page = __shfl_sync(~0u, cur.page, from);
+    const float ks = __shfl_sync(~0u, cur.ks, from), vs = __shfl_sync(~0u, cur.vs, from);
+    const bool there = page >= 0 && pos < it.len;
+    if (lane < kGroups)
+      factor[lane] = make_float4(ks * p.scale_log2, log2_scale(vs), there ? 1.0f / vs : 0.0f, 0.0f);
+    // one box per page of the tile; the first 16-token group of it stands for it
+    const int sub = min(p.c.block_log2, kTileLog2);
+    const bool load = lane < kGroups && there && (lane & ((1 << (sub - 4)) - 1)) == 0;
+    const uint32_t loads = __popc(__ballot_sync(~0u, load));
+    if (lane == 0) mbar_arrive_expect_tx(full, loads * 2u * (static_cast<uint32_t>(kD) << sub));
+    __syncwarp();
+    if (load) {
+      const int y = (it.h << p.c.block_log2) + (pos & (p.c.block - 1));
+      tma_load_3d(tk, full, stage + lane * 16 * kD, 0, y, static_cast<int>(page));
+      tma_load_3d(tv, full, stage + (kTile + lane * 16) * kD, 0, y, static_cast<int>(page));
+    }
+    ++tile;
+    ++x;
+    if (x < x1) {
+      if (tile == t1) {
+        next_item(p, it);
+        tile = 0;
+        t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), x1 - x));
+        take(p, nxt);
+      } else if (tile == te) {
+        take(p, nxt);
+      }
+    }
+  }
+};
+
+// Where a row's output goes; r counts the rows of one KV head.
+__device__ __forceinline__ uint16_t* out_row(const Kv8AttnParams& p, const Item& it, int r) {
+  const int gi = r / p.queries, i = r - gi * p.queries;
+  return static_cast<uint16_t*>(p.out) + it.b * p.o_sb + (it.h * p.group + gi) * p.o_sh + i * p.o_ss;
+}
+
+// Joins row rl of `count` partial results (`at(i)`: the i-th, in the order of the list): the maximum, the total and
+// this lane's kD / 32 channels.
+template <int kD, bool kShared, class At>
+__device__ __forceinline__ void join_row(const At& at, int count, int part_rows, int rl, float& top, float& total,
+                                         float (&sum)[kD / 32]) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kV = kD / 32;
+  top = -INFINITY;
+  total = 0.0f;
+#pragma unroll
+  for (int v = 0; v < kV; ++v) sum[v] = 0.0f;
+  for (int i0 = 0; i0 < count; i0 += 32) {
+    float mi = -INFINITY, li = 0.0f;
+    if (i0 + lane < count) {
+      const float* q = at(i0 + lane) + part_rows * kD + rl;
+      mi = kShared ? q[0] : __ldcg(q);
+      li = kShared ? q[part_rows] : __ldcg(q + part_rows);
+    }
+    float up = mi;
+    for (int o = 16; o > 0; o >>= 1) up = fmaxf(up, __shfl_xor_sync(~0u, up, o));
+    up = fmaxf(up, top);
+    const float again = top == -INFINITY ? 0.0f : ex2(top - up);
+    const float f = mi == -INFINITY ? 0.0f : ex2(mi - up);
+    top = up;
+    total = total * again + warp_sum(f * li);
+#pragma unroll
+    for (int v = 0; v < kV; ++v) sum[v] *= again;
+    const int n = min(32, count - i0);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float fi = __shfl_sync(~0u, f, i);
+      const float* q = at(i0 + i) + rl * kD + lane * kV;
+      if constexpr (kV == 2) {
+        const float2 x = kShared ? *reinterpret_cast<const float2*>(q) : __ldcg(reinterpret_cast<const float2*>(q));
+        sum[0] = fmaf(fi, x.x, sum[0]), sum[1] = fmaf(fi, x.y, sum[1]);
+      } else {
+        const float4 x = kShared ? *reinterpret_cast<const float4*>(q) : __ldcg(reinterpret_cast<const float4*>(q));
+        sum[0] = fmaf(fi, x.x, sum[0]), sum[1] = fmaf(fi, x.y, sum[1]);
+        sum[2] = fmaf(fi, x.z, sum[2]), sum[3] = fmaf(fi, x.w, sum[3]);
+      }
+    }
+  }
+}
+
+// Writes a joined row: to the output, or to a partial result.
+template <int kD>
+__device__ __forceinline__ void put_row(const Kv8AttnParams& p, const Item& it, int rl, float* part, float top, float total,
+                                        const float (&sum)[kD / 32]) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kV = kD / 32;
+  if (part != nullptr) {
+    float* dst = part + rl * kD + lane * kV;
+    if constexpr (kV == 2) *reinterpret_cast<float2*>(dst) = make_float2(sum[0], sum[1]);
+    else *reinterpret_cast<float4*>(dst) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    if (lane == 0) part[p.part_rows * kD + rl] = top, part[p.part_rows * (kD + 1) + rl] = total;
+    return;
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  uint32_t w[kV / 2];
+#pragma unroll
+  for (int v = 0; v < kV / 2; ++v)
+    w[v] = p.bf16 ? float2_to_pair<WBK_DT_BF16>(sum[2 * v] * inv, sum[2 * v + 1] * inv)
+                  : float2_to_pair<WBK_DT_F16>(sum[2 * v] * inv, sum[2 * v + 1] * inv);
+  uint16_t* dst = out_row(p, it, it.rb * kRows + rl) + lane * kV;
+  if constexpr (kV == 2) *reinterpret_cast<uint32_t*>(dst) = w[0];
+  else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+}
+
+template <int kFmt, int kD>
+__global__ void __launch_bounds__(kThreads, kD == 64 ? 4 : 3)
 kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                 const Kv8AttnParams p) {
-  using Cfg = StepCfg<kD, kWR>;
-  using Smem = StepSmem<kD, kWR>;
-  constexpr int kStages = Cfg::kStages;
-  constexpr int kTG = kComputeWarps / kWR;   // warps that share a row group's tokens
-  constexpr int kKSteps = kD / 16;
-  constexpr int kNTiles = kD / 8;
+  constexpr int kKSteps = kD / 16;  // of a score product
+  constexpr int kMTiles = kD / 16;  // of an output product
+  constexpr int kTileBytes = 2 * kTile * kD;
   extern __shared__ uint8_t smem_raw[];
-  Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  StepSmem& s = *reinterpret_cast<StepSmem*>(rings + kWarps * p.stages * kTileBytes);
+  float* slots = reinterpret_cast<float*>(&s + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort_flag;
 
-  // this CTA's share [x0, x1) of the list
+  // this warp's share [x0, x1) of the list
   const int64_t total = total_tiles(p);
-  const int64_t active = max(min(static_cast<int64_t>(gridDim.x), total / kMinTiles), static_cast<int64_t>(1));
-  if (blockIdx.x >= active) return;
-  const int64_t x0 = blockIdx.x * total / active, x1 = (blockIdx.x + 1) * total / active;
-
+  const int64_t ctas = max(min(static_cast<int64_t>(gridDim.x), total * kTile / kMinShare), static_cast<int64_t>(1));
+  if (blockIdx.x >= ctas) return;
+  const int64_t warps = min(ctas * kWarps, total), me = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  const int64_t x0 = me * total / warps, x1 = (me + 1) * total / warps;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], kComputeWarps);
+    for (int i = 0; i < kWarps; ++i) {
+      for (int j = 0; j < kMaxStages; ++j) mbar_init(&s.full[i][j], 1);
+      s.tickets[i] = 0;
     }
     s.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
+  if (me >= warps) return;
+
   int tile = 0;
   Item it = locate(p, x0, tile);
+  uint8_t* ring = rings + warp * p.stages * kTileBytes;
+  Loader loader;
+  loader.start(p, it, tile, x0, x1);
+  for (int i = 0; i < p.stages && loader.x < x1; ++i)
+    loader.issue<kD>(p, &tmap_k, &tmap_v, ring + i * kTileBytes, s.factor[warp][i], &s.full[warp][i]);
 
-  if (warp == kComputeWarps) {
-    // ---------------------------------------------------------- producer
-    const int sub = p.c.block < kTile ? p.c.block_log2 : 6;          // log2 of tokens per TMA box
-    const int boxes = kTile >> sub;                                  // per tile
-    const int batch_tiles = p.c.block < kTile ? 32 / boxes : 32 << (p.c.block_log2 - 6);
-    uint32_t g = 0;
-    bool ok = true;
-    int64_t x = x0;
-    auto first_blk = [&](int t) { return (t * kTile) >> p.c.block_log2; };
-    PageLane cur = fetch_page(p, it, first_blk(tile) + lane);
-    while (x < x1 && ok) {
-      const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
-      Item nit = it;
-      if (x + (t1 - tile) < x1) next_item(p, nit);
-      for (int tb = tile; tb < t1 && ok;) {
-        const int blk0 = first_blk(tb);
-        const int te = min(t1, ((blk0 << p.c.block_log2) / kTile) + batch_tiles);  // tiles that cur covers
-        const PageLane nxt = te < t1 ? fetch_page(p, it, first_blk(te) + lane) : fetch_page(p, nit, lane);
-        for (int t = tb; t < te; ++t, ++g) {
-          const int st = static_cast<int>(g % kStages);
-          const uint32_t ph = (g / kStages) & 1u;
-          ok = __all_sync(~0u, mbar_wait_inl(&s.empty[st], ph ^ 1u, abort_flag, p.timeout_ns, KSITE_PRODUCER));
-          if (!ok) break;
-          const int pos = t * kTile + (lane & 3) * 16;  // of 16-token group lane & 3
-          const int from = ((pos >> p.c.block_log2) - blk0) & 31;
-          const int64_t page = __shfl_sync(~0u, cur.page, from);
-          const float ks = __shfl_sync(~0u, cur.ks, from), vs = __shfl_sync(~0u, cur.vs, from);
-          const bool there = page >= 0 && pos < it.len;
-          if (lane < kGroups)
-            s.factor[st][lane] = make_float4(ks * p.scale_log2, log2_scale(vs), 1.0f / vs, there ? 1.0f : 0.0f);
-          __syncwarp();
-          // the first 16-token group of each box stands for it
-          const bool load = lane < kGroups && there && (lane & ((1 << (sub - 4)) - 1)) == 0;
-          const uint32_t loads = __popc(__ballot_sync(~0u, load));
-          if (lane == 0) mbar_arrive_expect_tx(&s.full[st], loads * 2u * (static_cast<uint32_t>(kD) << sub));
-          __syncwarp();
-          if (load) {
-            const int y = (it.h << p.c.block_log2) + (pos & (p.c.block - 1));
-            tma_load_3d(&tmap_k, &s.full[st], s.k[st] + lane * 16 * kD, 0, y, static_cast<int>(page));
-            tma_load_3d(&tmap_v, &s.full[st], s.v[st] + lane * 16 * kD, 0, y, static_cast<int>(page));
-          }
+  const int gid = lane >> 2, c = lane & 3;
+  // Fragment addresses within a tile. Keys: 16 (or twice 16) bytes of token gid, channels c * kD / 4 .. Values: the
+  // tokens 2c and 2c + 1, channels gid * kD / 8 .. With head_dim 64 the value loads of a half-warp hit all banks
+  // once only if even and odd lanes of a quad read different halves of the 128-byte lines: odd c take
+  // the pair in the other order, and the selectors that interleave the pair's bytes swap it back.
+  const int koff = kD == 64 ? gid * 64 + ((c ^ (gid >> 1)) & 3) * 16 : gid * 128 + ((2 * c) ^ gid) * 16;
+  const int khop = kD == 64 ? 0 : (((2 * c + 1) ^ gid) - ((2 * c) ^ gid)) * 16;
+  const int pair = 2 * c + (kD == 64 ? c & 1 : 0);
+  const int voff0 = kTile * kD + (kD == 64 ? pair * 64 + ((gid >> 1) ^ c) * 16 + (gid & 1) * 8 : pair * 128 + (gid ^ pair) * 16);
+  const int voff1 = kTile * kD + (kD == 64 ? (pair ^ 1) * 64 + ((gid >> 1) ^ c) * 16 + (gid & 1) * 8
+                                           : (pair ^ 1) * 128 + (gid ^ pair ^ 1) * 16);
+  const uint32_t lo = kD == 64 && (c & 1) ? 0x1504u : 0x5140u, hi = kD == 64 && (c & 1) ? 0x3726u : 0x7362u;
+
+  int st = 0;
+  uint32_t phase = 0;
+  int64_t x = x0;
+  while (x < x1) {
+    const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
+    // ---- queries: row gid, channels c * kD / 4 ..
+    uint32_t qf[kD / 8];
+    float qfac = 1.0f;
+    {
+      const int r = it.rb * kRows + gid;
+#pragma unroll
+      for (int i = 0; i < kD / 8; ++i) qf[i] = 0u;
+      if (r < p.rows) {
+        const int gi = r / p.queries, i = r - gi * p.queries;
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + it.b * p.q_sb +
+                                                          (it.h * p.group + gi) * p.q_sh + i * p.q_ss + c * (kD / 4));
+#pragma unroll
+        for (int j = 0; j < kD / 32; ++j) {
+          const uint4 u = src[j];
+          qf[4 * j] = u.x, qf[4 * j + 1] = u.y, qf[4 * j + 2] = u.z, qf[4 * j + 3] = u.w;
         }
-        tb = te;
-        cur = nxt;
       }
-      x += t1 - tile;
-      tile = 0;
-      it = nit;
+      if (p.bf16) {
+        // bf16 -> fp16 times a power of two that puts the row's largest value into [2^14, 2^15): exact but for values
+        // 2^-28 of the largest and below; the power comes back as a factor of the scores
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kD / 8; ++i) {
+          const float2 f = pair_to_float2<WBK_DT_BF16>(qf[i]);
+          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
+        const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100), 127);
+        const float up = kv8_pow2(14 - e);
+        qfac = kv8_pow2(min(e - 14, 126));
+#pragma unroll
+        for (int i = 0; i < kD / 8; ++i) {
+          const float2 f = pair_to_float2<WBK_DT_BF16>(qf[i]);
+          qf[i] = float2_to_pair<WBK_DT_F16>(f.x * up, f.y * up);
+        }
+      }
     }
-    // Every copy lands before the CTA ends, also when a compute warp gave up waiting.
-    if (lane == 0) {
-      int dummy = 0;
-      for (uint32_t i = g > kStages ? g - kStages : 0; i < g; ++i)
-        mbar_wait_inl(&s.full[i % kStages], (i / kStages) & 1u, &dummy, kDrainNs, KSITE_DRAIN);
+    // ---- the columns of this lane's scores, rows 2c and 2c + 1: factor, and how many tokens they see
+    float qcol[2];
+    int vis[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      qcol[e] = __shfl_sync(~0u, qfac, (2 * c + e) * 4);
+      const int r = it.rb * kRows + 2 * c + e, i = r % p.queries;
+      // rows beyond the last hide nothing: their results are dropped
+      vis[e] = r >= p.rows ? INT_MAX : i >= it.n ? 0 : p.causal ? max(it.len - it.n + i + 1, 0) : it.len;
     }
-  } else {
-    // ----------------------------------------------------------- compute
-    const int wr = warp % kWR, tg = warp / kWR;  // row group, token group
-    const int gid = lane >> 2, c = lane & 3;
-    uint32_t g = 0;
-    bool ok = true;
-    int64_t x = x0;
-    while (x < x1) {
-      const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
-      // ---- this lane's rows (gid and gid + 8 of the row group), their queries and how much they see
-      uint32_t qf[kKSteps][4];
-      float qfac[2];
-      int vis[2];
+    const int clear = __reduce_min_sync(~0u, min(vis[0], vis[1]));  // tokens that no row hides
+
+    float o[kMTiles][4];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = it.rb * Cfg::kRows + wr * 16 + gid + half * 8;
-        vis[half] = INT_MAX;  // rows beyond the last hide nothing: their results are dropped
-        qfac[half] = 1.0f;
-        uint32_t w[kD / 8];
-#pragma unroll
-        for (int i = 0; i < kD / 8; ++i) w[i] = 0u;
-        if ((!kHalf || half == 0) && r < p.rows) {
-          const int gi = r / p.queries, i = r - gi * p.queries;
-          vis[half] = i >= it.n ? 0 : p.causal ? max(it.len - it.n + i + 1, 0) : it.len;
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + it.b * p.q_sb +
-                                                            (it.h * p.group + gi) * p.q_sh + i * p.q_ss + c * (kD / 4));
-#pragma unroll
-          for (int i4 = 0; i4 < kD / 32; ++i4) {
-            const uint4 u = src[i4];
-            w[4 * i4] = u.x, w[4 * i4 + 1] = u.y, w[4 * i4 + 2] = u.z, w[4 * i4 + 3] = u.w;
+    for (int j = 0; j < kMTiles; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+    for (int t = tile; t < t1; ++t) {
+      if (!__all_sync(~0u, mbar_wait_inl(&s.full[warp][st], phase, abort_flag, p.timeout_ns, KSITE_TILE))) {
+        // Give up: copies in flight land before the CTA ends (this tile's, and those of the stages after it).
+        int dummy = 0;
+        if (lane == 0) {
+          const int64_t left = loader.x - (x + (t - tile));
+          for (int64_t i = 0; i < left; ++i) {
+            mbar_wait_inl(&s.full[warp][st], phase, &dummy, kDrainNs, KSITE_DRAIN);
+            if (++st == p.stages) st = 0, phase ^= 1u;
           }
         }
-        if (p.bf16) {
-          // bf16 -> fp16 times a power of two that puts the row's largest value into [2^14, 2^15): exact but for
-          // values 2^-28 of the largest and below; the power comes back as a factor of the scores
-          float amax = 0.0f;
-#pragma unroll
-          for (int i = 0; i < kD / 8; ++i) {
-            const float2 f = pair_to_float2<WBK_DT_BF16>(w[i]);
-            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-          amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
-          amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
-          const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100), 127);
-          const float up = kv8_pow2(14 - e);
-          qfac[half] = kv8_pow2(min(e - 14, 126));
-#pragma unroll
-          for (int i = 0; i < kD / 8; ++i) {
-            const float2 f = pair_to_float2<WBK_DT_BF16>(w[i]);
-            w[i] = float2_to_pair<WBK_DT_F16>(f.x * up, f.y * up);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < kKSteps; ++k) qf[k][half] = w[2 * k], qf[k][half + 2] = w[2 * k + 1];
+        return;
       }
-      const int clear = __reduce_min_sync(~0u, min(vis[0], vis[1]));  // tokens that no row of this warp hides
-
-      float o[kNTiles][4];
+      const uint8_t* stage = ring + st * kTileBytes;
+      // ---- scores of 32 tokens: group gi holds tokens 16 gi + gid (sc 0, 1) and 16 gi + gid + 8 (sc 2, 3)
+      float sc[kGroups][4];
 #pragma unroll
-      for (int j = 0; j < kNTiles; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-
-      for (int t = tile; t < t1; ++t, ++g) {
-        const int st = static_cast<int>(g % kStages);
-        if (ok) ok = __all_sync(~0u, mbar_wait_inl(&s.full[st], (g / kStages) & 1u, abort_flag, p.timeout_ns, KSITE_COMPUTE));
-        if (ok) {
-#pragma unroll 1
-          for (int gi = tg; gi < kGroups; gi += kTG) {
-            const float4 fac = s.factor[st][gi];
-            if (fac.w == 0.0f) continue;
-            const uint8_t* kt = s.k[st];
-            const uint8_t* vt = s.v[st];
-            const int pos = t * kTile + gi * 16;
-            // ---- scores of 16 tokens: tokens gid (first n-tile) and gid + 8 (second)
-            float sc[2][4];
+      for (int gi = 0; gi < kGroups; ++gi) {
+        sc[gi][0] = sc[gi][1] = sc[gi][2] = sc[gi][3] = 0.0f;
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-              const int tok = gi * 16 + nt * 8 + gid;
-              sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
-              if constexpr (kD == 64) {
-                const uint4 u = lds16(kt + tok * 64 + ((c ^ ((tok >> 1) & 3)) << 4));
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        for (int h = 0; h < kD / 64; ++h) {
+          const uint8_t* at = stage + koff + gi * 16 * kD + (h == 0 ? 0 : khop);
+          const uint4 u = lds16(at), v = lds16(at + 8 * kD);
+          const uint32_t a[4] = {u.x, u.y, u.z, u.w}, b[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  mma16816(sc[nt], qf[k], half2_bits<kFmt>(w[k]), half2_bits<kFmt>(w[k] >> 16));
-              } else {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const uint4 u = lds16(kt + tok * 128 + (((2 * c + h) ^ (tok & 7)) << 4));
-                  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                  for (int k = 0; k < 4; ++k)
-                    mma16816(sc[nt], qf[4 * h + k], half2_bits<kFmt>(w[k]), half2_bits<kFmt>(w[k] >> 16));
-                }
-              }
-            }
-            // ---- x + log2 vs, masked; raise the maximum where a weight would pass 2^8
-            constexpr int kHalves = kHalf ? 1 : 2;
-            const bool edge = pos + 16 > clear;
-            float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int half = 0; half < kHalves; ++half) {
-              const float km = fac.x * qfac[half];
-#pragma unroll
-              for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  float v = fmaf(sc[nt][2 * half + e], km, fac.y);
-                  if (edge && pos + nt * 8 + 2 * c + e >= vis[half]) v = -INFINITY;
-                  sc[nt][2 * half + e] = v;
-                  top[half] = fmaxf(top[half], v);
-                }
-            }
-            if (__any_sync(~0u, top[0] > m[0] + kRaise || (!kHalf && top[1] > m[1] + kRaise))) {
-#pragma unroll
-              for (int half = 0; half < kHalves; ++half) {
-                top[half] = fmaxf(top[half], __shfl_xor_sync(~0u, top[half], 1));
-                top[half] = fmaxf(top[half], __shfl_xor_sync(~0u, top[half], 2));
-                const float up = fmaxf(m[half], top[half]);
-                const float alpha = up == -INFINITY ? 1.0f : ex2(m[half] - up);
-                m[half] = up;
-                l[half] *= alpha;
-#pragma unroll
-                for (int j = 0; j < kNTiles; ++j) o[j][2 * half] *= alpha, o[j][2 * half + 1] *= alpha;
-              }
-            }
-            // ---- weights, as the A operand of the second product
-            uint32_t pa[4];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              if (half < kHalves) {
-                const float ref = m[half] == -INFINITY ? 0.0f : m[half];
-                float sum = 0.0f;
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                  const float w0 = ex2(sc[nt][2 * half] - ref), w1 = ex2(sc[nt][2 * half + 1] - ref);
-                  const __half2 h = __floats2half2_rn(w0, w1);
-                  pa[2 * nt + half] = *reinterpret_cast<const uint32_t*>(&h);
-                  sum += w0 + w1;
-                }
-                l[half] = fmaf(sum, fac.z, l[half]);
-              } else {
-                pa[1] = pa[3] = 0u;
-              }
-            }
-            // ---- outputs: tokens 2c, 2c + 1 and 2c + 8, 2c + 9, channels gid * kD / 8 ..
-            uint32_t va[4][kD / 32];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              // for head_dim 64 odd lanes of a quad take the two tokens of a pair in the other order (see below)
-              const int e = kD == 64 ? (i & 1) ^ (c & 1) : i & 1;
-              const int tok = gi * 16 + (i >> 1) * 8 + 2 * c + e;
-              if constexpr (kD == 64) {
-                const uint2 u = lds8(vt + tok * 64 + (((gid >> 1) ^ ((tok >> 1) & 3)) << 4) + (gid & 1) * 8);
-                va[i][0] = u.x, va[i][1] = u.y;
-              } else {
-                const uint4 u = lds16(vt + tok * 128 + ((gid ^ (tok & 7)) << 4));
-                va[i][0] = u.x, va[i][1] = u.y, va[i][2] = u.z, va[i][3] = u.w;
-              }
-              if (edge && t * kTile + tok >= it.len) {  // whatever lies there, a weight of 0 has to give 0
-#pragma unroll
-                for (int w = 0; w < kD / 32; ++w) va[i][w] = 0u;
-              }
-            }
-            // bytes of a token pair side by side; with head_dim 64 the loads of a half-warp hit all banks once only
-            // if even and odd lanes of a quad read different halves of the 128-byte lines, so the selector swaps back
-            const uint32_t lo = kD == 64 && (c & 1) ? 0x1504u : 0x5140u, hi = kD == 64 && (c & 1) ? 0x3726u : 0x7362u;
-#pragma unroll
-            for (int w = 0; w < kD / 32; ++w) {
-              const uint32_t a01 = __byte_perm(va[0][w], va[1][w], lo), a23 = __byte_perm(va[0][w], va[1][w], hi);
-              const uint32_t b01 = __byte_perm(va[2][w], va[3][w], lo), b23 = __byte_perm(va[2][w], va[3][w], hi);
-              mma16816(o[4 * w], pa, half2_bits<kFmt>(a01), half2_bits<kFmt>(b01));
-              mma16816(o[4 * w + 1], pa, half2_bits<kFmt>(a01 >> 16), half2_bits<kFmt>(b01 >> 16));
-              mma16816(o[4 * w + 2], pa, half2_bits<kFmt>(a23), half2_bits<kFmt>(b23));
-              mma16816(o[4 * w + 3], pa, half2_bits<kFmt>(a23 >> 16), half2_bits<kFmt>(b23 >> 16));
-            }
+          for (int k = 0; k < 4; ++k) {
+            const uint2 fa = codes_to_half<kFmt>(a[k]), fb = codes_to_half<kFmt>(b[k]);
+            const uint32_t frag[4] = {fa.x, fb.x, fa.y, fb.y};
+            mma16816(sc[gi], frag, qf[8 * h + 2 * k], qf[8 * h + 2 * k + 1]);
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s.empty[st]);
         }
       }
-
-      // ---- join the warps that shared this row group's tokens, in order
+      // ---- x + log2 vs, masked; raise the maximum where a weight would pass 2^8
+      float inv[kGroups];  // 0: no tokens there
+      bool edge = (t + 1) * kTile > clear;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        l[half] += __shfl_xor_sync(~0u, l[half], 1);
-        l[half] += __shfl_xor_sync(~0u, l[half], 2);
-        if (kTG > 1 && c == 0) s.max[warp][gid + 8 * half] = m[half];
+      for (int gi = 0; gi < kGroups; ++gi) {
+        const float4 fac = s.factor[warp][st][gi];
+        inv[gi] = fac.z;
+        edge = edge || fac.z == 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[gi][e] = fmaf(sc[gi][e], fac.x * qcol[e & 1], fac.y);
       }
-      if constexpr (kTG > 1) {
-        compute_barrier();
-        float fac[2];
+      if (edge) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float top = -INFINITY;
+        for (int gi = 0; gi < kGroups; ++gi)
 #pragma unroll
-          for (int i = 0; i < kTG; ++i) top = fmaxf(top, s.max[wr + i * kWR][gid + 8 * half]);
-          fac[half] = m[half] == -INFINITY ? 0.0f : ex2(m[half] - top);
-          m[half] = top;
-          if (c == 0) s.total[warp][gid + 8 * half] = l[half] * fac[half];
-        }
-        for (int turn = 0; turn < kTG; ++turn) {
-          if (turn == tg) {
+          for (int e = 0; e < 4; ++e)
+            if (inv[gi] == 0.0f || t * kTile + gi * 16 + gid + (e >> 1) * 8 >= vis[e & 1]) sc[gi][e] = -INFINITY;
+      }
+      float top[2];
 #pragma unroll
-            for (int half = 0; half < (kHalf ? 1 : 2); ++half) {
-              float4* dst = reinterpret_cast<float4*>(&s.sum[(wr * 16 + gid + 8 * half) * kD + c * (kD / 4)]);
+      for (int e = 0; e < 2; ++e) top[e] = fmaxf(fmaxf(sc[0][e], sc[0][e + 2]), fmaxf(sc[1][e], sc[1][e + 2]));
+      if (__any_sync(~0u, top[0] > m[0] + kRaise || top[1] > m[1] + kRaise)) {
 #pragma unroll
-              for (int j = 0; j < kNTiles; j += 4) {  // column pair e of n-tile j is channel e * kD / 8 + j of the lane
+        for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  float4 v = make_float4(o[j][2 * half + e] * fac[half], o[j + 1][2 * half + e] * fac[half],
-                                         o[j + 2][2 * half + e] * fac[half], o[j + 3][2 * half + e] * fac[half]);
-                  float4& at = dst[(e * (kD / 8) + j) / 4];
-                  if (turn > 0) v.x += at.x, v.y += at.y, v.z += at.z, v.w += at.w;
-                  at = v;
-                  o[j][2 * half + e] = v.x, o[j + 1][2 * half + e] = v.y;
-                  o[j + 2][2 * half + e] = v.z, o[j + 3][2 * half + e] = v.w;
-                }
-              }
-            }
-          }
-          compute_barrier();
-        }
+          for (int d = 4; d < 32; d <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], d));
+          const float up = fmaxf(m[e], top[e]);
+          const float alpha = up == -INFINITY ? 1.0f : ex2(m[e] - up);
+          m[e] = up;
+          l[e] *= alpha;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          l[half] = 0.0f;
-#pragma unroll
-          for (int i = 0; i < kTG; ++i) l[half] += s.total[wr + i * kWR][gid + 8 * half];
+          for (int j = 0; j < kMTiles; ++j) o[j][e] *= alpha, o[j][e + 2] *= alpha;
         }
       }
-
-      // ---- the row groups' last warps hold the sums: write the output, or this CTA's part of it
-      const bool whole = tile == 0 && t1 == it.tiles;
-      const int slot = tile == 0 ? 1 : 0;
-      float* part = p.parts + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * Cfg::kPartFloats;
-      if (tg == kTG - 1) {
+      const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
 #pragma unroll
-        for (int half = 0; half < (kHalf ? 1 : 2); ++half) {
-          const int rl = wr * 16 + gid + 8 * half, r = it.rb * Cfg::kRows + rl;
-          if (r >= p.rows) continue;
-          if (whole) {
-            const int gi = r / p.queries, i = r - gi * p.queries;
-            const float inv = l[half] == 0.0f ? 0.0f : 1.0f / l[half];
-            uint16_t* dst = static_cast<uint16_t*>(p.out) + it.b * p.o_sb + (it.h * p.group + gi) * p.o_sh + i * p.o_ss +
-                            c * (kD / 4);
+      for (int gi = 0; gi < kGroups; ++gi) {
+        // ---- weights of 16 tokens, transposed: tokens 2c, 2c + 1 (pb0) and 8 further (pb1) of row gid
+        float w[4];
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < 4; ++e) w[e] = ex2(sc[gi][e] - ref[e & 1]);
+        l[0] = fmaf(w[0] + w[2], inv[gi], l[0]);
+        l[1] = fmaf(w[1] + w[3], inv[gi], l[1]);
+        const uint32_t pb0 = transpose8x8(float2_to_pair<WBK_DT_F16>(w[0], w[1]));
+        const uint32_t pb1 = transpose8x8(float2_to_pair<WBK_DT_F16>(w[2], w[3]));
+        // ---- outputs: tokens 2c, 2c + 1 and 8 further, channels gid * kD / 8 ..
+        uint32_t va[4][kD / 32];
 #pragma unroll
-              for (int j = 0; j < kNTiles; j += 8) {
-                uint32_t w[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const float a = o[j + 2 * k][2 * half + e] * inv, b = o[j + 2 * k + 1][2 * half + e] * inv;
-                  w[k] = p.bf16 ? float2_to_pair<WBK_DT_BF16>(a, b) : float2_to_pair<WBK_DT_F16>(a, b);
-                }
-                *reinterpret_cast<uint4*>(dst + e * (kD / 8) + j) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* at = stage + ((i & 1) ? voff1 : voff0) + (gi * 16 + (i >> 1) * 8) * kD;
+          if constexpr (kD == 64) {
+            const uint2 u = lds8(at);
+            va[i][0] = u.x, va[i][1] = u.y;
           } else {
-            float4* dst = reinterpret_cast<float4*>(part + rl * kD + c * (kD / 4));
+            const uint4 u = lds16(at);
+            va[i][0] = u.x, va[i][1] = u.y, va[i][2] = u.z, va[i][3] = u.w;
+          }
+        }
+        if (edge) {  // whatever lies at a place without a token, a weight of 0 has to give 0
 #pragma unroll
-            for (int j = 0; j < kNTiles; j += 4)
+          for (int i = 0; i < 4; ++i) {
+            const int tok = t * kTile + gi * 16 + (i >> 1) * 8 + 2 * c + (kD == 64 ? (i & 1) ^ (c & 1) : i & 1);
+            if (inv[gi] == 0.0f || tok >= it.len) {
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-                dst[(e * (kD / 8) + j) / 4] = make_float4(o[j][2 * half + e], o[j + 1][2 * half + e],
-                                                         o[j + 2][2 * half + e], o[j + 3][2 * half + e]);
-            if (c == 0) {
-              part[Cfg::kRows * kD + rl] = m[half];
-              part[Cfg::kRows * (kD + 1) + rl] = l[half];
+              for (int k = 0; k < kD / 32; ++k) va[i][k] = 0u;
             }
           }
         }
-      }
-      if (!whole) {
-        // the CTAs of this item: first .. last of the list's shares that reach into it
-        const int64_t begin = x - tile, end = begin + it.tiles;
-        const int first = static_cast<int>(((begin + 1) * active - 1) / total);
-        const int last = static_cast<int>((end * active - 1) / total);
-        __threadfence();
-        compute_barrier();
-        if (threadIdx.x == 0) {
-          const uint32_t before = atomicAdd(&p.tickets[first], 1u);
-          s.last = before == static_cast<uint32_t>(last - first);
-          if (s.last) p.tickets[first] = 0u;
-        }
-        compute_barrier();
-        if (s.last) {
-          __threadfence();
-          const int rows = min(Cfg::kRows, p.rows - it.rb * Cfg::kRows);
-          const int64_t stride = 2 * Cfg::kPartFloats;
-          // part of CTA i: its slot 0, but slot 1 for the first
-          const float* base = p.parts + static_cast<int64_t>(first) * stride;
-          const int parts = last - first + 1;
-          for (int idx = threadIdx.x; idx < rows * (kD / 4); idx += kComputeWarps * 32) {
-            const int rl = idx / (kD / 4), d4 = idx % (kD / 4);
-            float top = -INFINITY;
-            for (int i = 0; i < parts; ++i)
-              top = fmaxf(top, __ldcg(base + i * stride + (i == 0 ? Cfg::kPartFloats : 0) + Cfg::kRows * kD + rl));
-            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float tot = 0.0f;
-            for (int i = 0; i < parts; ++i) {
-              const float* q = base + i * stride + (i == 0 ? Cfg::kPartFloats : 0);
-              const float mi = __ldcg(q + Cfg::kRows * kD + rl);
-              const float f = mi == -INFINITY ? 0.0f : ex2(mi - top);
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(q + rl * kD) + d4);
-              tot = fmaf(f, __ldcg(q + Cfg::kRows * (kD + 1) + rl), tot);
-              sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y);
-              sum.z = fmaf(f, v.z, sum.z), sum.w = fmaf(f, v.w, sum.w);
-            }
-            const float inv = tot == 0.0f ? 0.0f : 1.0f / tot;
-            const int r = it.rb * Cfg::kRows + rl, gi = r / p.queries, i = r - gi * p.queries;
-            uint16_t* dst = static_cast<uint16_t*>(p.out) + it.b * p.o_sb + (it.h * p.group + gi) * p.o_sh + i * p.o_ss;
-            uint2 w;
-            if (p.bf16) {
-              w.x = float2_to_pair<WBK_DT_BF16>(sum.x * inv, sum.y * inv);
-              w.y = float2_to_pair<WBK_DT_BF16>(sum.z * inv, sum.w * inv);
-            } else {
-              w.x = float2_to_pair<WBK_DT_F16>(sum.x * inv, sum.y * inv);
-              w.y = float2_to_pair<WBK_DT_F16>(sum.z * inv, sum.w * inv);
-            }
-            *reinterpret_cast<uint2*>(dst + d4 * 4) = w;
-          }
+#pragma unroll
+        for (int k = 0; k < kD / 32; ++k) {  // bytes of a token pair side by side: channels 4k .. 4k + 3
+          const uint2 a01 = codes_to_half<kFmt>(__byte_perm(va[0][k], va[1][k], lo));
+          const uint2 b01 = codes_to_half<kFmt>(__byte_perm(va[2][k], va[3][k], lo));
+          const uint2 a23 = codes_to_half<kFmt>(__byte_perm(va[0][k], va[1][k], hi));
+          const uint2 b23 = codes_to_half<kFmt>(__byte_perm(va[2][k], va[3][k], hi));
+          const uint32_t f01[4] = {a01.x, a01.y, b01.x, b01.y}, f23[4] = {a23.x, a23.y, b23.x, b23.y};
+          mma16816(o[2 * k], f01, pb0, pb1);
+          mma16816(o[2 * k + 1], f23, pb0, pb1);
         }
       }
-      x += t1 - tile;
-      tile = 0;
-      if (x < x1) next_item(p, it);
+      __syncwarp();
+      if (loader.x < x1)
+        loader.issue<kD>(p, &tmap_k, &tmap_v, ring + st * kTileBytes, s.factor[warp][st], &s.full[warp][st]);
+      if (++st == p.stages) st = 0, phase ^= 1u;
     }
+
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(~0u, l[e], d);
+
+    // ---- the warps and CTAs that this item lies in
+    const int64_t begin = x - tile, end = begin + it.tiles;
+    const int64_t first = ((begin + 1) * warps - 1) / total, last = (end * warps - 1) / total;
+    const int cta = blockIdx.x, first_cta = static_cast<int>(first / kWarps), last_cta = static_cast<int>(last / kWarps);
+    const int w0 = first_cta == cta ? static_cast<int>(first % kWarps) : 0;
+    const int w1 = last_cta == cta ? static_cast<int>(last % kWarps) : kWarps - 1;
+    const bool alone = w0 == w1, here = first_cta == last_cta;
+    const int rows = min(kRows, p.rows - it.rb * kRows);
+    const int floats = part_floats(p.part_rows, kD);
+    float* part = here ? nullptr : p.parts + (static_cast<int64_t>(cta) * 2 + (first_cta == cta ? 1 : 0)) * floats;
+    auto slot_of = [&](int w) {  // a warp's partial result of this item in shared memory
+      return slots + (w == 0 ? 0 : w == kWarps - 1 ? kSlots - 1 : 2 * w - (w == w0 ? 0 : 1)) * floats;
+    };
+    float* mine = alone ? part : slot_of(warp);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int rl = 2 * c + e;
+      if (rl >= rows) continue;
+      if (mine == nullptr) {
+        const float invl = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
+        uint32_t w[kD / 16];
+#pragma unroll
+        for (int j = 0; j < kMTiles; ++j)
+          w[j] = p.bf16 ? float2_to_pair<WBK_DT_BF16>(o[j][e] * invl, o[j][e + 2] * invl)
+                        : float2_to_pair<WBK_DT_F16>(o[j][e] * invl, o[j][e + 2] * invl);
+        uint4* dst = reinterpret_cast<uint4*>(out_row(p, it, it.rb * kRows + rl) + gid * (kD / 8));
+#pragma unroll
+        for (int j = 0; j < kMTiles / 4; ++j) dst[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+      } else {
+        float4* dst = reinterpret_cast<float4*>(mine + rl * kD + gid * (kD / 8));
+#pragma unroll
+        for (int j = 0; j < kMTiles / 2; ++j)
+          dst[j] = make_float4(o[2 * j][e], o[2 * j][e + 2], o[2 * j + 1][e], o[2 * j + 1][e + 2]);
+        if (gid == 0) mine[p.part_rows * kD + rl] = m[e], mine[p.part_rows * (kD + 1) + rl] = l[e];
+      }
+    }
+    bool holder = alone;  // this warp has the CTA's result of the item
+    if (!alone) {
+      __threadfence_block();
+      __syncwarp();
+      uint32_t before = 0;
+      if (lane == 0) before = atomicAdd(&s.tickets[w0], 1u);
+      holder = __shfl_sync(~0u, before, 0) == static_cast<uint32_t>(w1 - w0);
+      if (holder) {
+        __threadfence_block();
+        for (int rl = 0; rl < rows; ++rl) {
+          float top, tot, sum[kD / 32];
+          join_row<kD, true>([&](int i) { return static_cast<const float*>(slot_of(w0 + i)); }, w1 - w0 + 1, p.part_rows, rl,
+                             top, tot, sum);
+          put_row<kD>(p, it, rl, part, top, tot, sum);
+        }
+      }
+    }
+    if (holder && !here) {
+      __threadfence();
+      __syncwarp();
+      uint32_t before = 0;
+      if (lane == 0) {
+        before = atomicAdd(&p.tickets[first_cta], 1u);
+        if (before == static_cast<uint32_t>(last_cta - first_cta)) p.tickets[first_cta] = 0u;
+      }
+      if (__shfl_sync(~0u, before, 0) == static_cast<uint32_t>(last_cta - first_cta)) {
+        __threadfence();
+        const float* base = p.parts + static_cast<int64_t>(first_cta) * 2 * floats;
+        for (int rl = 0; rl < rows; ++rl) {
+          float top, tot, sum[kD / 32];
+          join_row<kD, false>([&](int i) { return base + (i == 0 ? 1 : 2 * static_cast<int64_t>(i)) * floats; },
+                              last_cta - first_cta + 1, p.part_rows, rl, top, tot, sum);
+          put_row<kD>(p, it, rl, nullptr, top, tot, sum);
+        }
+      }
+    }
+    x += t1 - tile;
+    tile = 0;
+    if (x < x1) next_item(p, it);
   }
 }
 
@@ -639,19 +683,32 @@ int step_sms() {
   return n > 0 ? n : 148;
 }
 
-// Row groups (of 16) that share a CTA's tiles: as many as the rows need, up to 4.
-int row_groups(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+// How a launch divides an SM: CTAs on it and the stages of a warp's ring, from the
+// registers (4 CTAs with head_dim 64, 3 with 128) and the shared memory that
+// the partial results of `rows` rows leave. More warps before more stages, but two
+// stages at least: one tile is computed on while another is on its way.
+struct StepShape {
+  int ctas_per_sm, stages;
+  size_t smem;
+};
+StepShape step_shape(int64_t rows, int64_t d) {
+  const int part_rows = static_cast<int>(std::min<int64_t>(rows, kRows));
+  const size_t fixed = 1024 + sizeof(StepSmem) + static_cast<size_t>(kSlots) * part_floats(part_rows, static_cast<int>(d)) * 4;
+  const size_t set = static_cast<size_t>(kWarps) * 2 * kTile * d;
+  for (int ctas = d == 64 ? 4 : 3;; --ctas) {
+    const size_t room = 233472 / ctas - 1024;  // 228 KB per SM, 1 KB of it taken by each CTA
+    const int stages = room > fixed ? static_cast<int>(std::min<size_t>((room - fixed) / set, kMaxStages)) : 0;
+    if (stages >= 2 || ctas == 1) return {ctas, std::max(stages, 1), fixed + std::max(stages, 1) * set};
+  }
+}
 
 // Tickets first (one per CTA), then two partial results per CTA.
-int64_t step_ctas(int64_t head_dim) {
-  return static_cast<int64_t>(step_sms()) * (head_dim == 64 ? StepCfg<64, 1>::kCtasPerSm : StepCfg<128, 1>::kCtasPerSm);
-}
-int64_t ticket_bytes(int64_t head_dim) { return (step_ctas(head_dim) * 4 + 255) / 256 * 256; }
+int64_t step_ctas(const StepShape& s) { return static_cast<int64_t>(step_sms()) * s.ctas_per_sm; }
+int64_t ticket_bytes(int64_t ctas) { return (ctas * 4 + 255) / 256 * 256; }
 
-template <int kFmt, int kD, int kWR, bool kHalf>
-int launch_step(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(StepSmem<kD, kWR>) + 1024;
-  static_assert((smem + 1024) * StepCfg<kD, kWR>::kCtasPerSm <= 233472, "shared memory budget");
+template <int kFmt, int kD>
+int launch_step(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid, size_t smem,
+                cudaStream_t stream) {
   static std::mutex mu;
   static std::vector<char> configured;
   const int dev = current_device();
@@ -660,25 +717,14 @@ int launch_step(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParam
     std::lock_guard<std::mutex> lock(mu);
     if (static_cast<int>(configured.size()) <= dev) configured.resize(dev + 1, 0);
     if (!configured[dev]) {
-      if (int e = cuda_check(cudaFuncSetAttribute(kv8_step_kernel<kFmt, kD, kWR, kHalf>,
-                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
+      if (int e = cuda_check(cudaFuncSetAttribute(kv8_step_kernel<kFmt, kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448),
                              "kv8 attention smem attribute"))
         return e;
       configured[dev] = 1;
     }
   }
-  kv8_step_kernel<kFmt, kD, kWR, kHalf><<<grid, kStepThreads, smem, stream>>>(tk, tv, p);
+  kv8_step_kernel<kFmt, kD><<<grid, kThreads, smem, stream>>>(tk, tv, p);
   return cuda_check(cudaGetLastError(), "kv8 attention launch");
-}
-
-template <int kFmt, int kD>
-int dispatch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid, cudaStream_t stream) {
-  if (p.rows <= 8) return launch_step<kFmt, kD, 1, true>(tk, tv, p, grid, stream);
-  switch (row_groups(p.rows)) {
-    case 1: return launch_step<kFmt, kD, 1, false>(tk, tv, p, grid, stream);
-    case 2: return launch_step<kFmt, kD, 2, false>(tk, tv, p, grid, stream);
-    default: return launch_step<kFmt, kD, 4, false>(tk, tv, p, grid, stream);
-  }
 }
 
 }  // namespace
@@ -700,8 +746,9 @@ extern "C" {
 
 int64_t wbk_attention_kv8_ws_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t queries, int64_t head_dim) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || queries <= 0 || head_dim <= 0) return 0;
-  const int64_t rows = 16 * row_groups(heads / kv_heads * queries);
-  return ticket_bytes(head_dim) + step_ctas(head_dim) * 2 * rows * (head_dim + 2) * 4;
+  const int64_t rows = heads / kv_heads * queries;
+  const int64_t ctas = step_ctas(step_shape(rows, head_dim));
+  return ticket_bytes(ctas) + ctas * 2 * part_floats(static_cast<int>(std::min<int64_t>(rows, kRows)), static_cast<int>(head_dim)) * 4;
 }
 
 int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
@@ -751,26 +798,28 @@ int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_
   p.group = static_cast<int>(heads / kv_heads);
   p.queries = static_cast<int>(queries);
   p.rows = p.group * p.queries;
-  const int rb = 16 * row_groups(p.rows);
-  p.row_blocks = (p.rows + rb - 1) / rb;
+  p.row_blocks = (p.rows + kRows - 1) / kRows;
+  p.part_rows = std::min(p.rows, kRows);
+  const StepShape shape = step_shape(p.rows, head_dim);
+  p.stages = shape.stages;
   p.causal = causal;
   p.bf16 = dtype == WBK_DT_BF16;
   p.scale_log2 = scale * kLog2e;
   p.tickets = static_cast<uint32_t*>(workspace);
-  p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ticket_bytes(head_dim));
+  p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ticket_bytes(step_ctas(shape)));
   p.timeout_ns = wait_timeout_ns();
   CUtensorMap tk, tv;
   if (int e = make_tmap_pages(&tk, k_cache, pages, kv_heads, block, head_dim)) return e;
   if (int e = make_tmap_pages(&tv, v_cache, pages, kv_heads, block, head_dim)) return e;
   // the lengths are on the device: as many CTAs as the table could need, at most what the SMs hold
   const int64_t most = batch * kv_heads * p.row_blocks * ((max_blocks * block + kTile - 1) / kTile);
-  const int grid = static_cast<int>(std::min<int64_t>(step_ctas(head_dim), std::max<int64_t>(most / kMinTiles, 1)));
+  const int grid = static_cast<int>(std::min(step_ctas(shape), std::max<int64_t>(most * kTile / kMinShare, 1)));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (fmt == WBK_FMT_E4M3)
-    return head_dim == 64 ? dispatch_rows<WBK_FMT_E4M3, 64>(tk, tv, p, grid, st)
-                          : dispatch_rows<WBK_FMT_E4M3, 128>(tk, tv, p, grid, st);
-  return head_dim == 64 ? dispatch_rows<WBK_FMT_E5M2, 64>(tk, tv, p, grid, st)
-                        : dispatch_rows<WBK_FMT_E5M2, 128>(tk, tv, p, grid, st);
+    return head_dim == 64 ? launch_step<WBK_FMT_E4M3, 64>(tk, tv, p, grid, shape.smem, st)
+                          : launch_step<WBK_FMT_E4M3, 128>(tk, tv, p, grid, shape.smem, st);
+  return head_dim == 64 ? launch_step<WBK_FMT_E5M2, 64>(tk, tv, p, grid, shape.smem, st)
+                        : launch_step<WBK_FMT_E5M2, 128>(tk, tv, p, grid, shape.smem, st);
 }
 
 }  // extern "C"
