@@ -39,6 +39,7 @@ UNITS = {
     "wbk_attn.cu": [],
     "wbk_kv8.cu": [],
     "wbk_kv8_attn.cu": [],
+    "wbk_kv8_prompt.cu": [],
     "wbk_sample.cu": [],
 }
 HEADERS = [os.path.join(HERE, "wbk_common.cuh"), os.path.join(HERE, "wbk_sm100.cuh"),

@@ -27,8 +27,9 @@ int current_device();
 // Reads (and optionally clears) the device error word of the attention unit.
 int attn_read_device_error(uint32_t* v, bool clear);
 
-// The same for the unit of attention over the 8-bit cache.
+// The same for the units of attention over the 8-bit cache.
 int kv8_read_device_error(uint32_t* v, bool clear);
+int kv8_prompt_read_device_error(uint32_t* v, bool clear);
 
 // Wall-clock limit of the bounded device waits set by wbk_set_wait_timeout_ns
 // (0 = not set: the WBK_WAIT_TIMEOUT_MS / 4 s default applies).

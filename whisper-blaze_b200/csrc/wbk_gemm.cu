@@ -2351,13 +2351,14 @@ extern "C" {
 int wbk_device_error(uint32_t* code_out) {
   if (code_out == nullptr) return fail(WBK_ERR_INVALID_ARG, "wbk_device_error: null pointer");
   if (int e = cuda_check(cudaDeviceSynchronize(), "wbk_device_error synchronize")) return e;
-  uint32_t v = 0, va = 0, vk = 0;
+  uint32_t v = 0, va = 0, vk = 0, vp = 0;
   if (int e = cuda_check(cudaMemcpyFromSymbol(&v, g_device_error, sizeof(v)), "wbk_device_error read")) return e;
   const uint32_t zero = 0;
   if (int e = cuda_check(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero)), "wbk_device_error clear")) return e;
   if (int e = attn_read_device_error(&va, true)) return e;
   if (int e = kv8_read_device_error(&vk, true)) return e;
-  *code_out = v != 0 ? v : va != 0 ? va : vk;  // the GEMM unit's word first, then the attention units'
+  if (int e = kv8_prompt_read_device_error(&vp, true)) return e;
+  *code_out = v != 0 ? v : va != 0 ? va : vk != 0 ? vk : vp;  // the GEMM unit's word first, then the attention units'
   return WBK_OK;
 }
 

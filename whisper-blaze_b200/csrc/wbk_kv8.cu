@@ -49,6 +49,11 @@ Kv8Pages kv8_pages(int64_t pages, int64_t kv_heads, int64_t block, const int32_t
   return c;
 }
 
+int64_t kv8_ticket_bytes() {
+  const int sms = sm_count();
+  return (static_cast<int64_t>(sms > 0 ? sms : 148) * kKv8TicketsPerSm * 4 + 255) / 256 * 256;
+}
+
 namespace {
 
 // ------------------------------------------------------------------ append

@@ -10,6 +10,8 @@
 
 #include "wbk_common.cuh"
 
+struct CUtensorMap_st;
+
 namespace wbk {
 
 // Smallest scale exponent: a page of zeros (or of values too small to matter)
@@ -71,6 +73,25 @@ __device__ __forceinline__ __half2 kv8_half2(uint32_t codes) {
   return __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes & 0xFFFFu), kv8_interp<kFmt>()));
 }
 
+// Four codes -> two packed fp16 pairs (exact).
+template <int kFmt>
+__device__ __forceinline__ uint2 kv8_half4(uint32_t codes) {
+  uint2 r;
+  if constexpr (kFmt == WBK_FMT_E4M3)
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(r.x), "=r"(r.y) : "r"(codes));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e5m2x2 %0, l;\n\tcvt.rn.f16x2.e5m2x2 %1, h;\n\t}"
+        : "=r"(r.x), "=r"(r.y) : "r"(codes));
+  return r;
+}
+
+// log2 of a scale, exact for powers of two.
+__device__ __forceinline__ float kv8_log2(float s) {
+  const int e = static_cast<int>(__float_as_uint(s) >> 23) - 127;
+  return (__float_as_uint(s) & 0x7FFFFFu) == 0 ? static_cast<float>(e) : log2f(s);
+}
+
 // A packed pair of the 16-bit input type as fp32.
 template <int kDtype>
 __device__ __forceinline__ float2 pair_to_float2(uint32_t w) {
@@ -96,6 +117,33 @@ __device__ __forceinline__ int kv8_len(const int32_t* lens, int b, const Kv8Page
   const int64_t n = lens[b];
   return static_cast<int>(n < 0 ? 0 : n < cap ? n : cap);
 }
+
+// A call of attention over the cache, checked.
+struct Kv8Attention {
+  const void* q;
+  void* out;
+  int64_t q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;  // element strides: sequence, head, position
+  Kv8Pages c;
+  const void *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  const int32_t* lens;
+  const int32_t* q_lens;  // or NULL
+  int batch, group, queries, head_dim;  // group: query heads per KV head
+  int fmt, causal, bf16;
+  float scale_log2;  // scale * log2(e)
+};
+
+// A workspace begins with tickets, zero between calls, as many as the SMs can have CTAs or a CTA 32-row parts; partial
+// results follow. Both kernels of attention keep to this, so one workspace serves calls of either.
+constexpr int kKv8TicketsPerSm = 8;
+int64_t kv8_ticket_bytes();
+
+// Attention for many query rows per KV head (wbk_kv8_prompt.cu), its workspace and its device error word.
+int kv8_prompt_attention(const Kv8Attention& a, void* workspace, cudaStream_t stream);
+int64_t kv8_prompt_ws_bytes(int64_t head_dim);
+// A tensor map of pages (channel, head * block + token, page) with boxes of at most `tile` tokens of one page and head,
+// swizzled over the row length or not.
+int kv8_make_tmap(CUtensorMap_st* map, const void* base, const Kv8Attention& a, int tile, bool swizzle);
 
 // Host: the checks of cache geometry that the cache's entry points share.
 int kv8_check_pages(const char* what, const void* k_cache, const void* v_cache, const float* k_scale,

@@ -51,20 +51,11 @@ constexpr uint64_t kDrainNs = 100000000ull;  // limit of the waits for copies in
 
 enum : uint32_t { KSITE_TILE = 41, KSITE_DRAIN = 42 };
 
-struct Kv8AttnParams {
-  const void* q;
-  void* out;
-  int64_t q_sb, q_sh, q_ss, o_sb, o_sh, o_ss;
-  Kv8Pages c;
-  const float *k_scale, *v_scale;
-  const int32_t* lens;
-  const int32_t* q_lens;
-  int batch, group, queries, rows;  // rows = group * queries of one KV head
-  int row_blocks;                   // blocks of kRows rows
-  int part_rows;                    // rows of a partial result: min(rows, kRows)
-  int stages;                       // of a warp's ring
-  int causal, bf16;
-  float scale_log2;  // scale * log2(e)
+struct Kv8AttnParams : Kv8Attention {
+  int rows;        // group * queries of one KV head
+  int row_blocks;  // blocks of kRows rows
+  int part_rows;   // rows of a partial result: min(rows, kRows)
+  int stages;      // of a warp's ring
   uint32_t* tickets;
   float* parts;
   uint64_t timeout_ns;
@@ -92,19 +83,6 @@ __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Four codes -> two packed fp16 pairs (exact).
-template <int kFmt>
-__device__ __forceinline__ uint2 codes_to_half(uint32_t w) {
-  uint2 r;
-  if constexpr (kFmt == WBK_FMT_E4M3)
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-        : "=r"(r.x), "=r"(r.y) : "r"(w));
-  else
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e5m2x2 %0, l;\n\tcvt.rn.f16x2.e5m2x2 %1, h;\n\t}"
-        : "=r"(r.x), "=r"(r.y) : "r"(w));
-  return r;
 }
 
 __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
@@ -197,13 +175,6 @@ __device__ __forceinline__ PageLane fetch_page(const Kv8AttnParams& p, const Ite
   return r;
 }
 
-// log2, exact for powers of two.
-__device__ __forceinline__ float log2_scale(float s) {
-  const int e = static_cast<int>(__float_as_uint(s) >> 23) - 127;
-  const uint32_t frac = __float_as_uint(s) & 0x7FFFFFu;
-  return frac == 0 ? static_cast<float>(e) : log2f(s);
-}
-
 // A warp's loads: the place in its share that the next tile comes from, and the pages there.
 struct Loader {
   Item it;
@@ -247,7 +218,7 @@ struct Loader {
     const float ks = __shfl_sync(~0u, cur.ks, from), vs = __shfl_sync(~0u, cur.vs, from);
     const bool there = page >= 0 && pos < it.len;
     if (lane < kGroups)
-      factor[lane] = make_float4(ks * p.scale_log2, log2_scale(vs), there ? 1.0f / vs : 0.0f, 0.0f);
+      factor[lane] = make_float4(ks * p.scale_log2, kv8_log2(vs), there ? 1.0f / vs : 0.0f, 0.0f);
     // one box per page of the tile; the first 16-token group of it stands for it
     const int sub = min(p.c.block_log2, kTileLog2);
     const bool load = lane < kGroups && there && (lane & ((1 << (sub - 4)) - 1)) == 0;
@@ -486,7 +457,7 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
           const uint32_t a[4] = {u.x, u.y, u.z, u.w}, b[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint2 fa = codes_to_half<kFmt>(a[k]), fb = codes_to_half<kFmt>(b[k]);
+            const uint2 fa = kv8_half4<kFmt>(a[k]), fb = kv8_half4<kFmt>(b[k]);
             const uint32_t frag[4] = {fa.x, fb.x, fa.y, fb.y};
             mma16816(sc[gi], frag, qf[8 * h + 2 * k], qf[8 * h + 2 * k + 1]);
           }
@@ -562,10 +533,10 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
         }
 #pragma unroll
         for (int k = 0; k < kD / 32; ++k) {  // bytes of a token pair side by side: channels 4k .. 4k + 3
-          const uint2 a01 = codes_to_half<kFmt>(__byte_perm(va[0][k], va[1][k], lo));
-          const uint2 b01 = codes_to_half<kFmt>(__byte_perm(va[2][k], va[3][k], lo));
-          const uint2 a23 = codes_to_half<kFmt>(__byte_perm(va[0][k], va[1][k], hi));
-          const uint2 b23 = codes_to_half<kFmt>(__byte_perm(va[2][k], va[3][k], hi));
+          const uint2 a01 = kv8_half4<kFmt>(__byte_perm(va[0][k], va[1][k], lo));
+          const uint2 b01 = kv8_half4<kFmt>(__byte_perm(va[2][k], va[3][k], lo));
+          const uint2 a23 = kv8_half4<kFmt>(__byte_perm(va[0][k], va[1][k], hi));
+          const uint2 b23 = kv8_half4<kFmt>(__byte_perm(va[2][k], va[3][k], hi));
           const uint32_t f01[4] = {a01.x, a01.y, b01.x, b01.y}, f23[4] = {a23.x, a23.y, b23.x, b23.y};
           mma16816(o[2 * k], f01, pb0, pb1);
           mma16816(o[2 * k + 1], f23, pb0, pb1);
@@ -660,24 +631,6 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
   }
 }
 
-// Pages as a 3-D tensor (channel, head * block + token, page) of bytes; a box is one page's tokens of one head, at
-// most a tile of them, swizzled over its row length.
-int make_tmap_pages(CUtensorMap* map, const void* base, int64_t pages, int64_t kv_heads, int64_t block, int64_t d) {
-  auto encode = get_encode_fn();
-  if (encode == nullptr) return fail(WBK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(kv_heads * block),
-                              static_cast<cuuint64_t>(pages)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(kv_heads * block * d)};
-  const cuuint32_t box[3] = {static_cast<cuuint32_t>(d), static_cast<cuuint32_t>(std::min<int64_t>(block, kTile)), 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            d == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(WBK_ERR_CUDA, "cuTensorMapEncodeTiled (kv8 pages) failed (%d)", static_cast<int>(r));
-  return WBK_OK;
-}
-
 int step_sms() {
   const int n = sm_count();
   return n > 0 ? n : 148;
@@ -695,6 +648,7 @@ StepShape step_shape(int64_t rows, int64_t d) {
   const int part_rows = static_cast<int>(std::min<int64_t>(rows, kRows));
   const size_t fixed = 1024 + sizeof(StepSmem) + static_cast<size_t>(kSlots) * part_floats(part_rows, static_cast<int>(d)) * 4;
   const size_t set = static_cast<size_t>(kWarps) * 2 * kTile * d;
+  static_assert(4 <= kKv8TicketsPerSm, "workspace layout");
   for (int ctas = d == 64 ? 4 : 3;; --ctas) {
     const size_t room = 233472 / ctas - 1024;  // 228 KB per SM, 1 KB of it taken by each CTA
     const int stages = room > fixed ? static_cast<int>(std::min<size_t>((room - fixed) / set, kMaxStages)) : 0;
@@ -702,9 +656,11 @@ StepShape step_shape(int64_t rows, int64_t d) {
   }
 }
 
-// Tickets first (one per CTA), then two partial results per CTA.
+// Two partial results per CTA, behind a ticket per CTA.
 int64_t step_ctas(const StepShape& s) { return static_cast<int64_t>(step_sms()) * s.ctas_per_sm; }
-int64_t ticket_bytes(int64_t ctas) { return (ctas * 4 + 255) / 256 * 256; }
+
+// Many rows per KV head go to the tensor cores.
+bool prompt_kernel(int64_t group, int64_t queries) { return group <= 128 && group * queries > 16; }
 
 template <int kFmt, int kD>
 int launch_step(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int grid, size_t smem,
@@ -729,6 +685,22 @@ int launch_step(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParam
 
 }  // namespace
 
+int kv8_make_tmap(CUtensorMap* map, const void* base, const Kv8Attention& a, int tile, bool swizzle) {
+  auto encode = get_encode_fn();
+  if (encode == nullptr) return fail(WBK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  const cuuint64_t d = static_cast<cuuint64_t>(a.head_dim), page_rows = static_cast<cuuint64_t>(a.c.kv_heads) * a.c.block;
+  const cuuint64_t dims[3] = {d, page_rows, static_cast<cuuint64_t>(a.c.pages)};
+  const cuuint64_t strides[2] = {d, page_rows * d};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(d), static_cast<cuuint32_t>(std::min(a.c.block, tile)), 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            !swizzle ? CU_TENSOR_MAP_SWIZZLE_NONE : d == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(WBK_ERR_CUDA, "cuTensorMapEncodeTiled (kv8 pages) failed (%d)", static_cast<int>(r));
+  return WBK_OK;
+}
+
 int kv8_read_device_error(uint32_t* v, bool clear) {
   if (int e = cuda_check(cudaMemcpyFromSymbol(v, g_device_error, sizeof(*v)), "kv8 device error read")) return e;
   if (clear) {
@@ -748,7 +720,9 @@ int64_t wbk_attention_kv8_ws_bytes(int64_t batch, int64_t heads, int64_t kv_head
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || queries <= 0 || head_dim <= 0) return 0;
   const int64_t rows = heads / kv_heads * queries;
   const int64_t ctas = step_ctas(step_shape(rows, head_dim));
-  return ticket_bytes(ctas) + ctas * 2 * part_floats(static_cast<int>(std::min<int64_t>(rows, kRows)), static_cast<int>(head_dim)) * 4;
+  const int64_t step =
+      kv8_ticket_bytes() + ctas * 2 * part_floats(static_cast<int>(std::min<int64_t>(rows, kRows)), static_cast<int>(head_dim)) * 4;
+  return prompt_kernel(heads / kv_heads, queries) ? std::max(step, kv8_prompt_ws_bytes(head_dim)) : step;
 }
 
 int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
@@ -776,6 +750,7 @@ int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_
     return fail(WBK_ERR_INVALID_ARG, "wbk_attention_kv8: q_lens misaligned");
   if (!aligned(q, 16) || !aligned(out, 16))
     return fail(WBK_ERR_UNSUPPORTED, "wbk_attention_kv8: q and out must be 16-byte aligned");
+  if (!(scale >= 0.0f)) return fail(WBK_ERR_INVALID_ARG, "wbk_attention_kv8: scale %g is negative", static_cast<double>(scale));
   for (int i = 0; i < 6; ++i)
     if (!kv8_stride_ok(strides[i]))
       return fail(WBK_ERR_UNSUPPORTED, "wbk_attention_kv8: stride[%d] = %lld is not a multiple of 8 elements", i,
@@ -790,6 +765,8 @@ int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_
   p.q_sb = strides[0], p.q_sh = strides[1], p.q_ss = strides[2];
   p.o_sb = strides[3], p.o_sh = strides[4], p.o_ss = strides[5];
   p.c = kv8_pages(pages, kv_heads, block, block_table, max_blocks, table_stride);
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
   p.k_scale = k_scale;
   p.v_scale = v_scale;
   p.lens = seq_lens;
@@ -797,24 +774,30 @@ int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_
   p.batch = static_cast<int>(batch);
   p.group = static_cast<int>(heads / kv_heads);
   p.queries = static_cast<int>(queries);
+  p.head_dim = static_cast<int>(head_dim);
+  p.fmt = fmt;
+  p.causal = causal;
+  p.bf16 = dtype == WBK_DT_BF16;
+  p.scale_log2 = scale * kLog2e;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  // queries repeated by a stride of 0 cannot be described to TMA: the few-rows kernel loads them itself
+  const bool repeated = (batch > 1 && p.q_sb == 0) || (heads > 1 && p.q_sh == 0) || (queries > 1 && p.q_ss == 0);
+  if (prompt_kernel(p.group, queries) && !repeated) return kv8_prompt_attention(p, workspace, st);
+
   p.rows = p.group * p.queries;
   p.row_blocks = (p.rows + kRows - 1) / kRows;
   p.part_rows = std::min(p.rows, kRows);
   const StepShape shape = step_shape(p.rows, head_dim);
   p.stages = shape.stages;
-  p.causal = causal;
-  p.bf16 = dtype == WBK_DT_BF16;
-  p.scale_log2 = scale * kLog2e;
   p.tickets = static_cast<uint32_t*>(workspace);
-  p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ticket_bytes(step_ctas(shape)));
+  p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kv8_ticket_bytes());
   p.timeout_ns = wait_timeout_ns();
   CUtensorMap tk, tv;
-  if (int e = make_tmap_pages(&tk, k_cache, pages, kv_heads, block, head_dim)) return e;
-  if (int e = make_tmap_pages(&tv, v_cache, pages, kv_heads, block, head_dim)) return e;
+  if (int e = kv8_make_tmap(&tk, k_cache, p, kTile, true)) return e;
+  if (int e = kv8_make_tmap(&tv, v_cache, p, kTile, true)) return e;
   // the lengths are on the device: as many CTAs as the table could need, at most what the SMs hold
   const int64_t most = batch * kv_heads * p.row_blocks * ((max_blocks * block + kTile - 1) / kTile);
   const int grid = static_cast<int>(std::min(step_ctas(shape), std::max<int64_t>(most * kTile / kMinShare, 1)));
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (fmt == WBK_FMT_E4M3)
     return head_dim == 64 ? launch_step<WBK_FMT_E4M3, 64>(tk, tv, p, grid, shape.smem, st)
                           : launch_step<WBK_FMT_E4M3, 128>(tk, tv, p, grid, shape.smem, st);

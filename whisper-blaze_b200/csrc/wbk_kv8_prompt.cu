@@ -1,0 +1,891 @@
+// Attention over the 8-bit key/value cache for many query rows per KV head (a
+// prompt, or a chunk of one) on the tcgen05 tensor cores.
+//
+// What bounds it: 4 * head_dim operations per query row and visible token on the
+// tensor cores, and 128 * 128 exponentials per tile of scores; the codes are read
+// from L2 as a rule.
+//
+//   * Codes cannot meet fp16 queries in one tcgen05.mma, so each 128-token tile of
+//     codes is converted once per CTA, by a warpgroup of its own, into fp16
+//     (keys: the queries' type, exact for both) in the swizzled layout that
+//     the products read, and serves two tiles of 128 query rows: 1/16 of an
+//     instruction per product of the tensor cores.
+//   * Rows of a tile are (position, query head of the group), position first, so
+//     the query heads that share a KV head share its tiles, and a causal tile ends
+//     where its last position does.
+//   * The work is the list of 128-token tiles of all (sequence, block of
+//     positions, KV head) items; every CTA (one per SM) takes an equal, contiguous
+//     share of it, so causal triangles, ragged lengths and few long items fill the
+//     SMs alike. An item that lies in several CTAs is joined by the last of them,
+//     per 32 rows, in the order of the list.
+//   * Warps 0-3 and 4-7: softmax of one query tile each, a row per thread; 8: TMA
+//     producer; 9: tcgen05 issuer; 12-15: converters (10, 11 hand their registers
+//     over). With head_dim 64 scores and weights have their own TMEM columns; with
+//     128 the weights replace their scores, and the next scores of a tile wait for
+//     its output product (commit and wait: the order of products with different
+//     accumulators is not guaranteed).
+//
+// The softmax is that of the few-rows kernel: running maximum of
+// log2(e) * scale * q.k + log2(value scale), raised when it is passed by 2^8.
+//
+// Every mbarrier wait is bounded; one that runs out records WBK_ERR_DEVICE_TIMEOUT,
+// raises the CTA's abort flag and every role leaves its loop; copies and products
+// in flight are waited for (with a limit) before TMEM is freed. No warp waits
+// at a block-wide barrier in between.
+#include <algorithm>
+#include <mutex>
+#include <vector>
+
+#include "wbk_kv8.cuh"
+#include "wbk_sm100.cuh"
+
+namespace wbk {
+namespace {
+
+constexpr int kTile = 128;  // tokens per tile, and rows of a query tile
+constexpr int kTileLog2 = 7;
+constexpr int kGroups = kTile / 16;
+constexpr int kThreads = 512;
+constexpr int kConvThreads = 128;
+constexpr int kStages = 2;       // converted tiles of keys, and of values
+constexpr int kFactors = 8;      // slots of per-tile factors: more tiles than the ring lets the producer be ahead
+constexpr int kBlockBytes = kTile * 128;  // 64 channels of a 16-bit tile
+constexpr uint32_t kTmemCols = 512;
+constexpr float kRaise = 8.0f;   // log2 units
+constexpr int kTickets = 8;      // per CTA: one for each 32 rows
+static_assert(kTickets <= kKv8TicketsPerSm, "workspace layout");
+// Register split (setmaxnreg) of the launch's 512 x 128: softmax 2 x 128 threads, control and converters 128 each.
+constexpr int kLaunchRegs = 128;
+constexpr int kSoftmaxRegs = 176;
+constexpr int kControlRegs = 72;
+constexpr int kConvRegs = 88;
+static_assert(256 * kSoftmaxRegs + 128 * kControlRegs + 128 * kConvRegs <= kThreads * kLaunchRegs, "register split");
+
+enum : uint32_t {
+  PSITE_PRODUCER = 51,
+  PSITE_CONVERT = 52,
+  PSITE_MMA = 53,
+  PSITE_SOFTMAX = 54,
+  PSITE_DRAIN = 55,
+};
+
+template <int kD>
+struct Cfg {
+  static constexpr bool kAlias = kD == 128;           // weights in their scores' columns
+  static constexpr int kRawUnits = kD == 64 ? 4 : 2;  // tiles of codes: keys and values in turn
+  static constexpr int kRawBytes = kTile * kD;
+  static constexpr int kBlocks = kD / 64;
+  static constexpr int kTileBytes = kBlocks * kBlockBytes;
+  static constexpr uint32_t s_col(int t) { return static_cast<uint32_t>(t * 128); }
+  static constexpr uint32_t p_col(int t) { return kAlias ? s_col(t) : static_cast<uint32_t>(256 + t * 64); }
+  static constexpr uint32_t o_col(int t) { return kAlias ? static_cast<uint32_t>(256 + t * 128) : static_cast<uint32_t>(384 + t * 64); }
+};
+
+template <int kD>
+struct PromptSmem {
+  uint8_t q[2][Cfg<kD>::kTileBytes];  // 1024-byte aligned
+  uint8_t k[kStages][Cfg<kD>::kTileBytes];
+  uint8_t v[kStages][Cfg<kD>::kTileBytes];
+  uint8_t raw[Cfg<kD>::kRawUnits][Cfg<kD>::kRawBytes];
+  float4 factor[kFactors][kGroups];  // of 16 tokens: key factor, log2 of the value scale, its inverse (0: not there)
+  int limit[kFactors];               // tokens of the tile that the sequence has
+  uint32_t holes[kFactors];          // groups below the limit whose page is outside the pool
+  uint64_t q_full[2], q_empty[2], raw_full[Cfg<kD>::kRawUnits], raw_empty[Cfg<kD>::kRawUnits];
+  uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], factor_full[kFactors];
+  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2], drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct PromptParams {
+  Kv8Attention a;
+  int tile_pos;     // query positions per 128-row tile: 128 / group
+  int tiles_q;      // query tiles per item, 1 or 2
+  int pos_blocks;   // items per sequence and KV head
+  uint32_t idesc_s, idesc_o;
+  uint32_t* tickets;
+  float* parts;
+  uint64_t timeout_ns;
+};
+
+// Partial result of an item: sums as [head_dim / 4][256 rows] float4, maxima [256], totals [256].
+__host__ __device__ constexpr int64_t part_floats(int d) { return 256 * static_cast<int64_t>(d) + 512; }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ void tma_load_5d(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int y, int z, int u,
+                                            int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(u), "r"(w)
+      : "memory");
+}
+
+// D[tmem] (+)= A[smem] . B[smem] and A[tmem] . B[smem], 16-bit operands.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  const uint32_t z = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  const uint32_t z = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Descriptor of the value tile as the B operand (N = channels contiguous): 128-byte rows of 64 channels per token,
+// 8-token swizzle atoms 1024 bytes apart, 64-channel blocks kBlockBytes apart.
+__device__ __forceinline__ uint64_t value_desc(const void* p) {
+  const uint32_t addr = smem_u32(p);
+  uint64_t d = static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(kBlockBytes >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+// A wait of a whole warp with one result for all lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns,
+                                          uint32_t site) {
+  return __all_sync(~0u, mbar_wait_inl(bar, parity, abort_flag, timeout_ns, site));
+}
+
+// One item of the work list: query positions pos0 .. of sequence b, KV head h.
+struct Item {
+  int b, pb, h;
+  int len, n;  // tokens that its last row sees, real query positions
+  int tiles;   // at least 1
+};
+
+__device__ __forceinline__ int tiles_of(const PromptParams& p, int unit, int& len, int& n) {
+  const int b = unit / p.pos_blocks, pb = unit - b * p.pos_blocks;
+  const int per = p.tile_pos * p.tiles_q;
+  len = kv8_len(p.a.lens, b, p.a.c);
+  n = p.a.q_lens != nullptr ? min(max(p.a.q_lens[b], 0), p.a.queries) : p.a.queries;
+  if (pb * per >= n) len = 0;
+  else if (p.a.causal) len = max(len - n + min(n, (pb + 1) * per), 0);
+  return max((len + kTile - 1) >> kTileLog2, 1);
+}
+
+__device__ __forceinline__ int64_t total_tiles(const PromptParams& p) {
+  int64_t sum = 0;
+  int len, n;
+  for (int u = threadIdx.x & 31; u < p.a.batch * p.pos_blocks; u += 32) sum += tiles_of(p, u, len, n);
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  return sum * p.a.c.kv_heads;
+}
+
+// The item and tile at place x of the list, by a converged warp.
+__device__ __forceinline__ Item locate(const PromptParams& p, int64_t x, int& tile) {
+  const int lane = threadIdx.x & 31, units = p.a.batch * p.pos_blocks;
+  const int64_t heads = p.a.c.kv_heads;
+  Item it{};
+  for (int u0 = 0;; u0 += 32) {
+    int len = 0, n = 0;
+    const int t = u0 + lane < units ? tiles_of(p, u0 + lane, len, n) : 0;
+    int64_t upto = t;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) upto += y;
+    }
+    const uint32_t past = __ballot_sync(~0u, upto * heads > x);
+    if (past == 0 && u0 + 32 < units) {
+      x -= __shfl_sync(~0u, upto, 31) * heads;
+      continue;
+    }
+    const int src = past != 0 ? __ffs(past) - 1 : 31;
+    x -= __shfl_sync(~0u, upto - t, src) * heads;
+    it.b = (u0 + src) / p.pos_blocks;
+    it.pb = (u0 + src) - it.b * p.pos_blocks;
+    it.len = __shfl_sync(~0u, len, src);
+    it.n = __shfl_sync(~0u, n, src);
+    it.tiles = __shfl_sync(~0u, t, src);
+    it.h = static_cast<int>(x / it.tiles);
+    tile = static_cast<int>(x - static_cast<int64_t>(it.h) * it.tiles);
+    return it;
+  }
+}
+
+__device__ __forceinline__ void next_item(const PromptParams& p, Item& it) {
+  if (++it.h < p.a.c.kv_heads) return;
+  it.h = 0;
+  const int unit = it.b * p.pos_blocks + it.pb + 1;
+  it.b = unit / p.pos_blocks;
+  it.pb = unit - it.b * p.pos_blocks;
+  if (it.b < p.a.batch) it.tiles = tiles_of(p, unit, it.len, it.n);
+}
+
+// A lane's page of 32 consecutive pages, with its scales.
+struct PageLane {
+  int64_t page;
+  float ks, vs;
+};
+__device__ __forceinline__ PageLane fetch_page(const PromptParams& p, const Item& it, int blk) {
+  PageLane r{-1, 0.0f, 1.0f};
+  if ((static_cast<int64_t>(blk) << p.a.c.block_log2) < it.len) r.page = kv8_page(p.a.c, it.b, blk);
+  if (r.page >= 0) {
+    const int64_t ph = r.page * p.a.c.kv_heads + it.h;
+    r.ks = p.a.k_scale[ph];
+    r.vs = p.a.v_scale[ph];
+  }
+  return r;
+}
+
+// 16 codes -> 16 values of the 16-bit type, in order.
+template <int kFmt, bool kBf16>
+__device__ __forceinline__ void convert16(const uint4& u, uint4& a, uint4& b) {
+  uint32_t w[8];
+  const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint2 h = kv8_half4<kFmt>(in[i]);
+    w[2 * i] = h.x;
+    w[2 * i + 1] = h.y;
+  }
+  if constexpr (kBf16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      w[i] = float2_to_pair<WBK_DT_BF16>(f.x, f.y);  // exact: at most 4 significant bits
+    }
+  }
+  a = make_uint4(w[0], w[1], w[2], w[3]);
+  b = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+// One tile of codes [128][kD] -> the 16-bit swizzled tile. kClear: tokens that are not there become 0.
+template <int kFmt, int kD, bool kBf16, bool kClear>
+__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, const float4* factor, int limit) {
+  const int tid = threadIdx.x & (kConvThreads - 1);
+  constexpr int kPer = kD / 16;  // 16-byte pieces per token, and per thread
+#pragma unroll 4
+  for (int i = 0; i < kPer; ++i) {
+    const int id = tid + i * kConvThreads, token = id / kPer, piece = id % kPer;
+    uint4 u = *reinterpret_cast<const uint4*>(raw + id * 16);
+    if (kClear && (token >= limit || factor[token >> 4].z == 0.0f)) u = make_uint4(0u, 0u, 0u, 0u);
+    uint4 a, b;
+    convert16<kFmt, kBf16>(u, a, b);
+    // 8 lanes store to 8 different 16-byte columns: those of the second 64 channels start with the odd one
+    const int block = piece >> 2, j = (piece & 3) * 2, sw = token & 7;
+    uint8_t* row = dst + block * kBlockBytes + token * 128;
+    const bool odd = block != 0;
+    *reinterpret_cast<uint4*>(row + (((j + odd) ^ sw) << 4)) = odd ? b : a;
+    *reinterpret_cast<uint4*>(row + (((j + !odd) ^ sw) << 4)) = odd ? a : b;
+  }
+}
+
+template <int kFmt, int kD, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1)
+kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                  const __grid_constant__ CUtensorMap tmap_v, const PromptParams p) {
+  using C = Cfg<kD>;
+  extern __shared__ uint8_t smem_raw[];
+  PromptSmem<kD>& s = *reinterpret_cast<PromptSmem<kD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                         ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &s.abort_flag;
+  const int nq = p.tiles_q;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s.q_full[t], 1);
+      mbar_init(&s.q_empty[t], 1);
+      mbar_init(&s.s_full[t], 1);
+      mbar_init(&s.s_free[t], kTile);
+      mbar_init(&s.p_full[t], kTile);
+      mbar_init(&s.pv_done[t], 1);
+      mbar_init(&s.o_free[t], kTile);
+    }
+    for (int i = 0; i < C::kRawUnits; ++i) {
+      mbar_init(&s.raw_full[i], 1);
+      mbar_init(&s.raw_empty[i], kConvThreads);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s.k_full[i], kConvThreads);
+      mbar_init(&s.k_empty[i], 1);
+      mbar_init(&s.v_full[i], kConvThreads);
+      mbar_init(&s.v_empty[i], 1);
+    }
+    for (int i = 0; i < kFactors; ++i) mbar_init(&s.factor_full[i], 1);
+    mbar_init(&s.drain, 1);
+    s.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_tmap(&tmap_q);
+    prefetch_tmap(&tmap_k);
+    prefetch_tmap(&tmap_v);
+  }
+  if (warp == 9) {
+    tmem_alloc(&s.tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+
+  // this CTA's share [x0, x1) of the list
+  const int64_t total = total_tiles(p);
+  const int64_t active = max(min(static_cast<int64_t>(gridDim.x), total / 2), static_cast<int64_t>(1));
+  const int64_t x0 = blockIdx.x < active ? blockIdx.x * total / active : 0;
+  const int64_t x1 = blockIdx.x < active ? (blockIdx.x + 1) * total / active : 0;
+  int tile = 0;
+  Item it{};
+  if (x0 < x1) it = locate(p, x0, tile);
+  int64_t x = x0;
+
+  if (warp >= 8 && warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+    if (warp == 8) {
+      // -------------------------------------------------------- producer
+      const int sub = min(p.a.c.block_log2, kTileLog2);  // log2 of tokens per TMA box
+      const int cover = 32 << p.a.c.block_log2;          // tokens that 32 pages hold
+      uint32_t unit = 0, g = 0, q_loads = 0;
+      bool ok = true;
+      while (x < x1 && ok) {
+        const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
+        int blk0 = 0, te = tile;
+        PageLane pages{-1, 0.0f, 1.0f};
+        for (int t = tile; t < t1 && ok; ++t, ++g) {
+          if (t == te) {
+            blk0 = (t * kTile) >> p.a.c.block_log2;
+            pages = fetch_page(p, it, blk0 + lane);
+            te = ((blk0 << p.a.c.block_log2) + cover) >> kTileLog2;
+          }
+          // ---- the tile's factors, before its codes
+          const int slot = static_cast<int>(g % kFactors);
+          const int pos = t * kTile + (lane & (kGroups - 1)) * 16;
+          const int from = ((pos >> p.a.c.block_log2) - blk0) & 31;
+          const int64_t page = __shfl_sync(~0u, pages.page, from);
+          const float ks = __shfl_sync(~0u, pages.ks, from), vs = __shfl_sync(~0u, pages.vs, from);
+          const bool there = page >= 0 && pos < it.len;
+          // the factor stays above 0, so that a masked -inf stays -inf
+          if (lane < kGroups)
+            s.factor[slot][lane] = make_float4(fmaxf(ks * p.a.scale_log2, 1.17549435e-38f), kv8_log2(vs), there ? 1.0f / vs : 0.0f, 0.0f);
+          const uint32_t holes = __ballot_sync(~0u, lane < kGroups && pos < it.len && !there);
+          if (lane == 0) {
+            s.limit[slot] = it.len - t * kTile;
+            s.holes[slot] = holes;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.factor_full[slot]);
+          // ---- keys, then values: one box per page, which its first group stands for
+          const bool load = lane < kGroups && there && (lane & ((1 << (sub - 4)) - 1)) == 0;
+          const uint32_t bytes = __popc(__ballot_sync(~0u, load)) * (static_cast<uint32_t>(kD) << sub);
+          const int y = (it.h << p.a.c.block_log2) + (pos & (p.a.c.block - 1));
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv, ++unit) {
+            const int u = static_cast<int>(unit % C::kRawUnits);
+            if (ok) ok = warp_wait(&s.raw_empty[u], ((unit / C::kRawUnits) & 1u) ^ 1u, abort_flag, p.timeout_ns, PSITE_PRODUCER);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[u], bytes);
+            __syncwarp();
+            if (load) tma_load_3d(kv == 0 ? &tmap_k : &tmap_v, &s.raw_full[u], s.raw[u] + lane * 16 * kD, 0, y, static_cast<int>(page));
+          }
+          if (!ok) break;
+          // ---- queries, behind the item's first codes
+          if (t == tile) {
+            for (int qt = 0; qt < nq && ok; ++qt) {
+              ok = warp_wait(&s.q_empty[qt], (q_loads & 1u) ^ 1u, abort_flag, p.timeout_ns, PSITE_PRODUCER);
+              if (!ok) break;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&s.q_full[qt], static_cast<uint32_t>(p.tile_pos * p.a.group * kD * 2));
+                for (int i = 0; i < C::kBlocks; ++i)
+                  tma_load_5d(&tmap_q, &s.q_full[qt], s.q[qt] + i * kBlockBytes, i * 64, 0, (it.pb * nq + qt) * p.tile_pos, it.h, it.b);
+              }
+              __syncwarp();
+            }
+            ++q_loads;
+          }
+        }
+        x += t1 - tile;
+        tile = 0;
+        if (x < x1) next_item(p, it);
+      }
+      // The CTA ends only when what was issued has landed and been used: every unit and query tile given back.
+      if (lane == 0) {
+        int dummy = 0;
+        const uint64_t limit = ok ? p.timeout_ns : 100000000ull;
+        for (uint32_t i = unit > C::kRawUnits ? unit - C::kRawUnits : 0; i < unit; ++i)
+          mbar_wait_inl(&s.raw_full[i % C::kRawUnits], (i / C::kRawUnits) & 1u, &dummy, limit, PSITE_DRAIN);
+        if (q_loads > 0)
+          for (int qt = 0; qt < nq; ++qt) mbar_wait_inl(&s.q_full[qt], (q_loads - 1) & 1u, &dummy, limit, PSITE_DRAIN);
+        if (ok) {  // and no commit to these barriers is still on its way
+          if (q_loads > 0)
+            for (int qt = 0; qt < nq; ++qt) mbar_wait_inl(&s.q_empty[qt], (q_loads - 1) & 1u, abort_flag, limit, PSITE_DRAIN);
+          for (uint32_t i = g > kStages ? g - kStages : 0; i < g; ++i) {
+            mbar_wait_inl(&s.k_empty[i % kStages], (i / kStages) & 1u, abort_flag, limit, PSITE_DRAIN);
+            mbar_wait_inl(&s.v_empty[i % kStages], (i / kStages) & 1u, abort_flag, limit, PSITE_DRAIN);
+          }
+        }
+      }
+    } else if (warp == 9 && lane == 0) {
+      // ------------------------------------------------------ MMA issuer
+      uint32_t g = 0, ui = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok) ok = mbar_wait_inl(bar, parity, abort_flag, p.timeout_ns, PSITE_MMA);
+        return ok;
+      };
+      auto issue_s = [&](int t, uint32_t gj) {
+        const int st = static_cast<int>(gj % kStages);
+#pragma unroll
+        for (int i = 0; i < C::kBlocks; ++i) {
+          const uint64_t qd = make_sw128_desc(s.q[t] + i * kBlockBytes), kd = make_sw128_desc(s.k[st] + i * kBlockBytes);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ss(tmem + C::s_col(t), qd + kk * 2, kd + kk * 2, p.idesc_s, i > 0 || kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s.s_full[t]);
+      };
+      auto issue_pv = [&](int t, uint32_t gj, bool first) {
+        const uint64_t vd = value_desc(s.v[gj % kStages]);
+#pragma unroll
+        for (int kk = 0; kk < kTile / 16; ++kk)
+          mma_ts(tmem + C::o_col(t), tmem + C::p_col(t) + kk * 8, vd + kk * (2048 >> 4), p.idesc_o, first && kk == 0 ? 0u : 1u);
+        umma_commit(&s.pv_done[t]);
+      };
+      while (x < x1 && ok) {
+        const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
+        const int n = t1 - tile;
+        for (int t = 0; t < nq; ++t) wait(&s.q_full[t], ui & 1u);
+        wait(&s.k_full[g % kStages], (g / kStages) & 1u);
+        for (int t = 0; t < nq; ++t) {
+          if (!C::kAlias) wait(&s.s_free[t], (g & 1u) ^ 1u);
+          else if (g > 0) wait(&s.pv_done[t], (g - 1) & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(t, g);
+        }
+        if (!ok) break;
+        umma_commit(&s.k_empty[g % kStages]);
+        if (n == 1)
+          for (int t = 0; t < nq; ++t) umma_commit(&s.q_empty[t]);
+        for (int j = 0; j < n && ok; ++j) {
+          const uint32_t gj = g + static_cast<uint32_t>(j), gn = gj + 1;
+          auto next_scores = [&](int t) {
+            if (C::kAlias) wait(&s.pv_done[t], gj & 1u);
+            else wait(&s.s_free[t], gj & 1u);
+            if (!ok) return;
+            tc_fence_after();
+            issue_s(t, gn);
+          };
+          if (!C::kAlias && j + 1 < n) {
+            wait(&s.k_full[gn % kStages], (gn / kStages) & 1u);
+            for (int t = 0; t < nq && ok; ++t) next_scores(t);
+          }
+          wait(&s.v_full[gj % kStages], (gj / kStages) & 1u);
+          for (int t = 0; t < nq && ok; ++t) {
+            wait(&s.p_full[t], gj & 1u);
+            if (j == 0) wait(&s.o_free[t], (ui & 1u) ^ 1u);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(t, gj, j == 0);
+            if (C::kAlias && j + 1 < n) {
+              if (t == 0) wait(&s.k_full[gn % kStages], (gn / kStages) & 1u);
+              next_scores(t);
+            }
+          }
+          if (!ok) break;
+          umma_commit(&s.v_empty[gj % kStages]);
+          if (j + 1 < n) {
+            umma_commit(&s.k_empty[gn % kStages]);
+            if (j + 2 == n)  // the item's last scores are issued
+              for (int t = 0; t < nq; ++t) umma_commit(&s.q_empty[t]);
+          }
+        }
+        g += static_cast<uint32_t>(n);
+        ++ui;
+        x += n;
+        tile = 0;
+        if (x < x1) {
+          // next_item, by one thread (tiles_of uses no warp operations)
+          next_item(p, it);
+        }
+      }
+      // TMEM and the barriers are in use until every product issued has finished.
+      umma_commit(&s.drain);
+      int dummy = 0;
+      mbar_wait_inl(&s.drain, 0, &dummy, ok ? p.timeout_ns : 100000000ull, PSITE_DRAIN);
+    }
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
+    // ---------------------------------------------------------- converters
+    uint32_t unit = 0;
+    bool ok = true;
+    const int64_t mine = x1 - x0;
+    for (int64_t i = 0; i < mine && ok; ++i) {
+      const uint32_t g = static_cast<uint32_t>(i);
+      const int st = static_cast<int>(g % kStages), slot = static_cast<int>(g % kFactors);
+      const uint32_t empty = ((g / kStages) & 1u) ^ 1u;
+      ok = warp_wait(&s.factor_full[slot], (g / kFactors) & 1u, abort_flag, p.timeout_ns, PSITE_CONVERT);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv, ++unit) {
+        const int u = static_cast<int>(unit % C::kRawUnits);
+        if (ok) ok = warp_wait(&s.raw_full[u], (unit / C::kRawUnits) & 1u, abort_flag, p.timeout_ns, PSITE_CONVERT);
+        if (ok) ok = warp_wait(kv == 0 ? &s.k_empty[st] : &s.v_empty[st], empty, abort_flag, p.timeout_ns, PSITE_CONVERT);
+        if (!ok) break;
+        if (kv == 0) convert_tile<kFmt, kD, kBf16, false>(s.raw[u], s.k[st], s.factor[slot], 0);
+        else convert_tile<kFmt, kD, false, true>(s.raw[u], s.v[st], s.factor[slot], s.limit[slot]);
+        fence_async_smem();
+        mbar_arrive(&s.raw_empty[u]);
+        mbar_arrive(kv == 0 ? &s.k_full[st] : &s.v_full[st]);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // ------------------------------------------------------------- softmax
+    const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    uint32_t g = 0;
+    bool ok = t < nq;
+    while (x < x1 && ok) {
+      const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
+      const int i = (it.pb * nq + t) * p.tile_pos + r / p.a.group, gi = r % p.a.group;  // query position and head
+      const bool real = r < p.tile_pos * p.a.group && i < p.a.queries;
+      const int seq = kv8_len(p.a.lens, it.b, p.a.c);
+      const int vis = i >= it.n ? 0 : p.a.causal ? max(seq - it.n + i + 1, 0) : seq;
+      float m = -INFINITY, l = 0.0f;
+      for (int tt = tile; tt < t1; ++tt, ++g) {
+        const int slot = static_cast<int>(g % kFactors);
+        if (!warp_wait(&s.factor_full[slot], (g / kFactors) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX) ||
+            !warp_wait(&s.s_full[t], g & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t sr[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(lane_addr + C::s_col(t) + c * 32, sr + 32 * c);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_wait(sr + 32 * c);
+        tc_fence_before();
+        if (!C::kAlias) mbar_arrive(&s.s_free[t]);
+        float* v = reinterpret_cast<float*>(sr);
+        const int lim = vis - tt * kTile;
+        if (__any_sync(~0u, lim < kTile)) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c >= lim) v[c] = -INFINITY;
+        }
+        const uint32_t holes = s.holes[slot];
+        if (holes != 0) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (holes >> (c >> 4) & 1u) v[c] = -INFINITY;
+        }
+        // ---- the row's largest x + log2 vs: factors are positive, so that of a group is that of its largest score
+        float mx = -INFINITY;
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          const float4 f = s.factor[slot][gr];
+          const float* y = v + 16 * gr;
+          const float a = max3(y[0], y[1], y[2]), b = max3(y[3], y[4], y[5]), c = max3(y[6], y[7], y[8]);
+          const float d = max3(y[9], y[10], y[11]), e = max3(y[12], y[13], y[14]);
+          mx = fmaxf(mx, fmaf(fmaxf(max3(a, b, c), max3(d, e, y[15])), f.x, f.y));
+        }
+        float alpha = 1.0f;
+        if (mx > m + kRaise) {
+          alpha = ex2(m - mx);
+          m = mx;
+        }
+        l *= alpha;
+        const bool rescale = tt > tile && __any_sync(~0u, alpha != 1.0f);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        if (tt > tile) {
+          // the weights' columns and the sums are free once the previous output product is done
+          if (!warp_wait(&s.pv_done[t], (g - 1) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pw[16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 f = s.factor[slot][2 * c + h];
+            const float off = f.y - ref;
+            float rs0 = 0.0f, rs1 = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float* y = v + 32 * c + 16 * h + 2 * k;
+              const float w0 = ex2(fmaf(y[0], f.x, off)), w1 = ex2(fmaf(y[1], f.x, off));
+              pw[8 * h + k] = pack_half2(w0, w1);
+              rs0 += w0;  // not of the fp16 weights: those of a page of small value scale may be 0
+              rs1 += w1;
+            }
+            l = fmaf(rs0 + rs1, f.z, l);
+          }
+          tmem_st_x16(lane_addr + C::p_col(t) + c * 16, pw);
+        }
+        if (rescale) {
+#pragma unroll 1
+          for (int c = 0; c < kD / 32; ++c) {
+            uint32_t orr[32];
+            const uint32_t oa = lane_addr + C::o_col(t) + c * 32;
+            tmem_ld_32x32b_x32(oa, orr);
+            tmem_ld_wait(orr);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) orr[k] = __float_as_uint(__uint_as_float(orr[k]) * alpha);
+            tmem_st_x32(oa, orr);
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&s.p_full[t]);
+      }
+      if (!ok) break;
+      // ---- the item's rows: output, or this CTA's part of it
+      if (!warp_wait(&s.pv_done[t], (g - 1) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) break;
+      tc_fence_after();
+      const bool whole = tile == 0 && t1 == it.tiles;
+      const int row = t * kTile + r;
+      uint16_t* dst = static_cast<uint16_t*>(p.a.out) + it.b * p.a.o_sb + (static_cast<int64_t>(it.h) * p.a.group + gi) * p.a.o_sh +
+                      i * p.a.o_ss;
+      float* part = p.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (tile == 0 ? 1 : 0)) * part_floats(kD);
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+      for (int c = 0; c < kD / 32; ++c) {
+        uint32_t orr[32];
+        tmem_ld_32x32b_x32(lane_addr + C::o_col(t) + c * 32, orr);
+        tmem_ld_wait(orr);
+        if (c == kD / 32 - 1) {  // read to the end: the next item's first product may overwrite it
+          tc_fence_before();
+          mbar_arrive(&s.o_free[t]);
+        }
+        const float* o = reinterpret_cast<const float*>(orr);
+        if (!whole) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            reinterpret_cast<float4*>(part)[(c * 8 + k) * 256 + row] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        } else if (real) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = float2_to_pair<kBf16 ? WBK_DT_BF16 : WBK_DT_F16>(o[8 * k + 2 * e] * inv, o[8 * k + 2 * e + 1] * inv);
+            reinterpret_cast<uint4*>(dst + c * 32)[k] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (!whole) {
+        part[256 * kD + row] = m;
+        part[256 * kD + 256 + row] = l;
+        // the CTAs that this item lies in; the last of them to finish these 32 rows joins them
+        const int64_t begin = x - tile, end = begin + it.tiles;
+        const int first = static_cast<int>(((begin + 1) * active - 1) / total), last = static_cast<int>((end * active - 1) / total);
+        __threadfence();
+        __syncwarp();
+        uint32_t before = 0;
+        if (lane == 0) {
+          uint32_t* ticket = &p.tickets[first * kTickets + warp];
+          before = atomicAdd(ticket, 1u);
+          if (before == static_cast<uint32_t>(last - first)) *ticket = 0u;
+        }
+        if (__shfl_sync(~0u, before, 0) == static_cast<uint32_t>(last - first)) {
+          __threadfence();
+          const float* base = p.parts + static_cast<int64_t>(first) * 2 * part_floats(kD);
+          const int count = last - first + 1;
+          auto at = [&](int k) { return base + (k == 0 ? 1 : 2 * static_cast<int64_t>(k)) * part_floats(kD); };
+          float top = -INFINITY, tot = 0.0f;
+          for (int k = 0; k < count; ++k) top = fmaxf(top, __ldcg(at(k) + 256 * kD + row));
+          for (int k = 0; k < count; ++k) {
+            const float mk = __ldcg(at(k) + 256 * kD + row);
+            tot = fmaf(mk == -INFINITY ? 0.0f : ex2(mk - top), __ldcg(at(k) + 256 * kD + 256 + row), tot);
+          }
+          const float invt = tot == 0.0f ? 0.0f : 1.0f / tot;
+#pragma unroll 1
+          for (int c = 0; c < kD / 32; ++c) {
+            float o[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = 0.0f;
+            for (int k = 0; k < count; ++k) {
+              const float mk = __ldcg(at(k) + 256 * kD + row), f = mk == -INFINITY ? 0.0f : ex2(mk - top);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(at(k)) + (c * 8 + e) * 256 + row);
+                o[4 * e] = fmaf(f, y.x, o[4 * e]), o[4 * e + 1] = fmaf(f, y.y, o[4 * e + 1]);
+                o[4 * e + 2] = fmaf(f, y.z, o[4 * e + 2]), o[4 * e + 3] = fmaf(f, y.w, o[4 * e + 3]);
+              }
+            }
+            if (real) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  w[e] = float2_to_pair<kBf16 ? WBK_DT_BF16 : WBK_DT_F16>(o[8 * k + 2 * e] * invt, o[8 * k + 2 * e + 1] * invt);
+                reinterpret_cast<uint4*>(dst + c * 32)[k] = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
+          }
+        }
+      }
+      x += t1 - tile;
+      tile = 0;
+      if (x < x1) next_item(p, it);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Queries as a 5-D tensor (channel, head of the group, position, KV head, sequence); a box is 64 channels of one tile's
+// rows, swizzled.
+int make_tmap_queries(CUtensorMap* map, const Kv8Attention& a, int tile_pos) {
+  auto encode = get_encode_fn();
+  if (encode == nullptr) return fail(WBK_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  const auto stride = [&](int64_t s, int64_t size) { return static_cast<cuuint64_t>(size > 1 ? s * 2 : 16); };
+  const int64_t heads = a.c.kv_heads;
+  const cuuint64_t dims[5] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.group),
+                              static_cast<cuuint64_t>(a.queries), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(a.batch)};
+  const cuuint64_t strides[4] = {stride(a.q_sh, a.group), stride(a.q_ss, a.queries), stride(a.q_sh * a.group, heads),
+                                 stride(a.q_sb, a.batch)};
+  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(tile_pos), 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = encode(map, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                            const_cast<void*>(a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(WBK_ERR_CUDA, "cuTensorMapEncodeTiled (queries) failed (%d)", static_cast<int>(r));
+  return WBK_OK;
+}
+
+// tcgen05 instruction descriptor, kind::f16: D fp32 (bit 4), A and B fp16 (0) or bf16 (1) at bits 7 and 10, B
+// major-ness at bit 16 (1 = N contiguous), N >> 3 at bit 17, M >> 4 at bit 24.
+constexpr uint32_t instruction(int n, bool bf16, bool b_n_major) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_n_major ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+
+int prompt_sms() {
+  const int n = sm_count();
+  return n > 0 ? n : 148;
+}
+
+template <int kFmt, int kD, bool kBf16>
+int launch_prompt(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PromptParams& p, int grid,
+                  cudaStream_t stream) {
+  constexpr size_t smem = sizeof(PromptSmem<kD>) + 1024;
+  static_assert(smem <= 232448, "shared memory budget");
+  static std::mutex mu;
+  static std::vector<char> configured;
+  const int dev = current_device();
+  if (dev < 0) return fail(WBK_ERR_CUDA, "no current CUDA device");
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (static_cast<int>(configured.size()) <= dev) configured.resize(dev + 1, 0);
+    if (!configured[dev]) {
+      cudaFuncAttributes fa;
+      if (int e = cuda_check(cudaFuncGetAttributes(&fa, kv8_prompt_kernel<kFmt, kD, kBf16>), "kv8 prompt function attributes"))
+        return e;
+      if (fa.numRegs < kLaunchRegs)  // the setmaxnreg split would wait for registers that do not exist
+        return fail(WBK_ERR_UNSUPPORTED, "kv8 prompt kernel built with %d registers per thread, needs %d", fa.numRegs, kLaunchRegs);
+      if (int e = cuda_check(cudaFuncSetAttribute(kv8_prompt_kernel<kFmt, kD, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                  static_cast<int>(smem)),
+                             "kv8 prompt smem attribute"))
+        return e;
+      configured[dev] = 1;
+    }
+  }
+  kv8_prompt_kernel<kFmt, kD, kBf16><<<grid, kThreads, smem, stream>>>(tq, tk, tv, p);
+  return cuda_check(cudaGetLastError(), "kv8 prompt launch");
+}
+
+template <int kFmt, int kD>
+int dispatch_type(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PromptParams& p, int grid,
+                  cudaStream_t stream) {
+  return p.a.bf16 ? launch_prompt<kFmt, kD, true>(tq, tk, tv, p, grid, stream)
+                  : launch_prompt<kFmt, kD, false>(tq, tk, tv, p, grid, stream);
+}
+
+}  // namespace
+
+int64_t kv8_prompt_ws_bytes(int64_t head_dim) {
+  return kv8_ticket_bytes() + static_cast<int64_t>(prompt_sms()) * 2 * part_floats(static_cast<int>(head_dim)) * 4;
+}
+
+int kv8_prompt_attention(const Kv8Attention& a, void* workspace, cudaStream_t stream) {
+  PromptParams p{};
+  p.a = a;
+  p.tile_pos = kTile / a.group;
+  p.tiles_q = a.queries > p.tile_pos ? 2 : 1;
+  const int64_t per = static_cast<int64_t>(p.tile_pos) * p.tiles_q;
+  p.pos_blocks = static_cast<int>((a.queries + per - 1) / per);
+  p.idesc_s = instruction(kTile, a.bf16, false);
+  p.idesc_o = instruction(a.head_dim, false, true);
+  p.tickets = static_cast<uint32_t*>(workspace);
+  p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kv8_ticket_bytes());
+  p.timeout_ns = wait_timeout_ns();
+  CUtensorMap tq, tk, tv;
+  if (int e = make_tmap_queries(&tq, a, p.tile_pos)) return e;
+  if (int e = kv8_make_tmap(&tk, a.k_cache, a, kTile, false)) return e;
+  if (int e = kv8_make_tmap(&tv, a.v_cache, a, kTile, false)) return e;
+  const int64_t most = static_cast<int64_t>(a.batch) * p.pos_blocks * a.c.kv_heads *
+                       ((static_cast<int64_t>(a.c.max_blocks) * a.c.block + kTile - 1) / kTile);
+  const int grid = static_cast<int>(std::min<int64_t>(prompt_sms(), std::max<int64_t>(most / 2, 1)));
+  if (a.fmt == WBK_FMT_E4M3)
+    return a.head_dim == 64 ? dispatch_type<WBK_FMT_E4M3, 64>(tq, tk, tv, p, grid, stream)
+                            : dispatch_type<WBK_FMT_E4M3, 128>(tq, tk, tv, p, grid, stream);
+  return a.head_dim == 64 ? dispatch_type<WBK_FMT_E5M2, 64>(tq, tk, tv, p, grid, stream)
+                          : dispatch_type<WBK_FMT_E5M2, 128>(tq, tk, tv, p, grid, stream);
+}
+
+int kv8_prompt_read_device_error(uint32_t* v, bool clear) {
+  if (int e = cuda_check(cudaMemcpyFromSymbol(v, g_device_error, sizeof(*v)), "kv8 prompt device error read")) return e;
+  if (clear) {
+    const uint32_t zero = 0;
+    if (int e = cuda_check(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero)), "kv8 prompt device error clear")) return e;
+  }
+  return WBK_OK;
+}
+
+}  // namespace wbk
