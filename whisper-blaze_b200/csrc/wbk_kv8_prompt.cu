@@ -153,6 +153,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       : "memory");
 }
 
+// The first 16 of r.
 __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -189,6 +190,12 @@ __device__ __forceinline__ uint64_t value_desc(const void* p) {
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns,
                                           uint32_t site) {
   return __all_sync(~0u, mbar_wait_inl(bar, parity, abort_flag, timeout_ns, site));
+}
+
+// One arrival for a warp, after what all its lanes did.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 // One item of the work list: query positions pos0 .. of sequence b, KV head h.
@@ -299,7 +306,7 @@ template <int kFmt, int kD, bool kBf16, bool kClear>
 __device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, const float4* factor, int limit) {
   const int tid = threadIdx.x & (kConvThreads - 1);
   constexpr int kPer = kD / 16;  // 16-byte pieces per token, and per thread
-#pragma unroll 4
+#pragma unroll 2
   for (int i = 0; i < kPer; ++i) {
     const int id = tid + i * kConvThreads, token = id / kPer, piece = id % kPer;
     uint4 u = *reinterpret_cast<const uint4*>(raw + id * 16);
@@ -313,6 +320,49 @@ __device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, c
     *reinterpret_cast<uint4*>(row + (((j + odd) ^ sw) << 4)) = odd ? b : a;
     *reinterpret_cast<uint4*>(row + (((j + !odd) ^ sw) << 4)) = odd ? a : b;
   }
+}
+
+// Scores of 32 columns that are not to count: at or after `lim`, or in one of the two groups that `holes` names.
+__device__ __forceinline__ void hide(uint32_t (&y)[32], int lim, uint32_t holes) {
+#pragma unroll
+  for (int k = 0; k < 32; ++k)
+    if (k >= lim || (holes >> (k >> 4) & 1u)) y[k] = 0xFF800000u;  // -inf
+}
+// The largest x + log2 vs of 32 columns.
+__device__ __forceinline__ float largest(uint32_t (&y)[32], const float4* factor, int lim, uint32_t holes, bool edge) {
+  if (edge) hide(y, lim, holes);
+  float mx = -INFINITY;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float* v = reinterpret_cast<const float*>(y) + 16 * h;
+    const float a = max3(v[0], v[1], v[2]), b = max3(v[3], v[4], v[5]), c = max3(v[6], v[7], v[8]);
+    const float d = max3(v[9], v[10], v[11]), e = max3(v[12], v[13], v[14]);
+    const float4 f = factor[h];
+    mx = fmaxf(mx, fmaf(fmaxf(max3(a, b, c), max3(d, e, v[15])), f.x, f.y));
+  }
+  return mx;
+}
+// The weights of 32 columns relative to 2^ref, as fp16 pairs in y[0 .. 15]; returns their sum over the value scales, of
+// the fp32 weights (as fp16 those of a page of small value scale may be 0).
+__device__ __forceinline__ float weights(uint32_t (&y)[32], const float4* factor, int lim, uint32_t holes, bool edge,
+                                         float ref) {
+  if (edge) hide(y, lim, holes);
+  float sum = 0.0f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float4 f = factor[h];
+    const float2 mul = make_float2(f.x, f.x), off = make_float2(f.y - ref, f.y - ref);
+    float2 rs = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float2 x = f2_fma(make_float2(__uint_as_float(y[16 * h + 2 * k]), __uint_as_float(y[16 * h + 2 * k + 1])), mul, off);
+      const float2 w = make_float2(ex2(x.x), ex2(x.y));
+      y[8 * h + k] = pack_half2(w.x, w.y);
+      rs = f2_add(rs, w);
+    }
+    sum = fmaf(rs.x + rs.y, f.z, sum);
+  }
+  return sum;
 }
 
 template <int kFmt, int kD, bool kBf16>
@@ -332,19 +382,19 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       mbar_init(&s.q_full[t], 1);
       mbar_init(&s.q_empty[t], 1);
       mbar_init(&s.s_full[t], 1);
-      mbar_init(&s.s_free[t], kTile);
-      mbar_init(&s.p_full[t], kTile);
+      mbar_init(&s.s_free[t], 4);  // one arrival per warp
+      mbar_init(&s.p_full[t], 4);
       mbar_init(&s.pv_done[t], 1);
-      mbar_init(&s.o_free[t], kTile);
+      mbar_init(&s.o_free[t], 4);
     }
     for (int i = 0; i < C::kRawUnits; ++i) {
       mbar_init(&s.raw_full[i], 1);
-      mbar_init(&s.raw_empty[i], kConvThreads);
+      mbar_init(&s.raw_empty[i], kConvThreads / 32);
     }
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&s.k_full[i], kConvThreads);
+      mbar_init(&s.k_full[i], kConvThreads / 32);
       mbar_init(&s.k_empty[i], 1);
-      mbar_init(&s.v_full[i], kConvThreads);
+      mbar_init(&s.v_full[i], kConvThreads / 32);
       mbar_init(&s.v_empty[i], 1);
     }
     for (int i = 0; i < kFactors; ++i) mbar_init(&s.factor_full[i], 1);
@@ -568,8 +618,11 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         if (kv == 0) convert_tile<kFmt, kD, kBf16, false>(s.raw[u], s.k[st], s.factor[slot], 0);
         else convert_tile<kFmt, kD, false, true>(s.raw[u], s.v[st], s.factor[slot], s.limit[slot]);
         fence_async_smem();
-        mbar_arrive(&s.raw_empty[u]);
-        mbar_arrive(kv == 0 ? &s.k_full[st] : &s.v_full[st]);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s.raw_empty[u]);
+          mbar_arrive(kv == 0 ? &s.k_full[st] : &s.v_full[st]);
+        }
       }
     }
   } else {
@@ -594,35 +647,25 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           break;
         }
         tc_fence_after();
-        uint32_t sr[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(lane_addr + C::s_col(t) + c * 32, sr + 32 * c);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_wait(sr + 32 * c);
-        tc_fence_before();
-        if (!C::kAlias) mbar_arrive(&s.s_free[t]);
-        float* v = reinterpret_cast<float*>(sr);
-        const int lim = vis - tt * kTile;
-        if (__any_sync(~0u, lim < kTile)) {
-#pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c >= lim) v[c] = -INFINITY;
-        }
+        const uint32_t sa = lane_addr + C::s_col(t), pa = lane_addr + C::p_col(t);
         const uint32_t holes = s.holes[slot];
-        if (holes != 0) {
-#pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (holes >> (c >> 4) & 1u) v[c] = -INFINITY;
-        }
+        const int lim = vis - tt * kTile;
+        const bool edge = holes != 0 || __any_sync(~0u, lim < kTile);
+        const float4* fac = s.factor[slot];
+        // Both passes over the scores read them from TMEM, 32 columns at a time, the next 32 on their way meanwhile: as
+        // straight-line code over 128 registers they ran at 4 clocks an instruction, starved of instructions.
+        uint32_t ya[32], yb[32];
         // ---- the row's largest x + log2 vs: factors are positive, so that of a group is that of its largest score
         float mx = -INFINITY;
-#pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) {
-          const float4 f = s.factor[slot][gr];
-          const float* y = v + 16 * gr;
-          const float a = max3(y[0], y[1], y[2]), b = max3(y[3], y[4], y[5]), c = max3(y[6], y[7], y[8]);
-          const float d = max3(y[9], y[10], y[11]), e = max3(y[12], y[13], y[14]);
-          mx = fmaxf(mx, fmaf(fmaxf(max3(a, b, c), max3(d, e, y[15])), f.x, f.y));
+        tmem_ld_32x32b_x32(sa, ya);
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          tmem_ld_wait(ya);
+          tmem_ld_32x32b_x32(sa + (c + 1) * 32, yb);
+          mx = fmaxf(mx, largest(ya, fac + 2 * c, lim - 32 * c, holes >> (2 * c), edge));
+          tmem_ld_wait(yb);
+          tmem_ld_32x32b_x32(sa + ((c + 2) & 3) * 32, ya);  // in the end the first again, for the second pass
+          mx = fmaxf(mx, largest(yb, fac + 2 * c + 2, lim - 32 * c - 32, holes >> (2 * c + 2), edge));
         }
         float alpha = 1.0f;
         if (mx > m + kRaise) {
@@ -640,25 +683,21 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           }
           tc_fence_after();
         }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pw[16];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float4 f = s.factor[slot][2 * c + h];
-            const float off = f.y - ref;
-            float rs0 = 0.0f, rs1 = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float* y = v + 32 * c + 16 * h + 2 * k;
-              const float w0 = ex2(fmaf(y[0], f.x, off)), w1 = ex2(fmaf(y[1], f.x, off));
-              pw[8 * h + k] = pack_half2(w0, w1);
-              rs0 += w0;  // not of the fp16 weights: those of a page of small value scale may be 0
-              rs1 += w1;
-            }
-            l = fmaf(rs0 + rs1, f.z, l);
-          }
-          tmem_st_x16(lane_addr + C::p_col(t) + c * 16, pw);
+        // ---- weights; where they replace their scores, 16 columns end before the next 32 begin
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          tmem_ld_wait(ya);
+          tmem_ld_32x32b_x32(sa + (c + 1) * 32, yb);
+          l += weights(ya, fac + 2 * c, lim - 32 * c, holes >> (2 * c), edge, ref);
+          tmem_st_x16(pa + c * 16, ya);
+          tmem_ld_wait(yb);
+          if (c == 0) tmem_ld_32x32b_x32(sa + 64, ya);
+          l += weights(yb, fac + 2 * c + 2, lim - 32 * c - 32, holes >> (2 * c + 2), edge, ref);
+          tmem_st_x16(pa + c * 16 + 16, yb);
+        }
+        if (!C::kAlias) {
+          tc_fence_before();
+          warp_arrive(&s.s_free[t]);
         }
         if (rescale) {
 #pragma unroll 1
@@ -674,7 +713,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         }
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&s.p_full[t]);
+        warp_arrive(&s.p_full[t]);
       }
       if (!ok) break;
       // ---- the item's rows: output, or this CTA's part of it
@@ -693,7 +732,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         tmem_ld_wait(orr);
         if (c == kD / 32 - 1) {  // read to the end: the next item's first product may overwrite it
           tc_fence_before();
-          mbar_arrive(&s.o_free[t]);
+          warp_arrive(&s.o_free[t]);
         }
         const float* o = reinterpret_cast<const float*>(orr);
         if (!whole) {
