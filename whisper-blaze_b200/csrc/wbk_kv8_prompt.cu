@@ -19,8 +19,7 @@
 //     SMs alike. An item that lies in several CTAs is joined by the last of them,
 //     per 32 rows, in the order of the list.
 //   * Warps 0-3 and 4-7: softmax of one query tile each, a row per thread; 8: TMA
-//     producer; 9: tcgen05 issuer; 12-15: converters (10, 11 hand their registers
-//     over). With head_dim 64 scores and weights have their own TMEM columns; with
+//     producer; 9: tcgen05 issuer; 10-13: converters. With head_dim 64 scores and weights have their own TMEM columns; with
 //     128 the weights replace their scores, and the next scores of a tile wait for
 //     its output product (commit and wait: the order of products with different
 //     accumulators is not guaranteed).
@@ -45,7 +44,7 @@ namespace {
 constexpr int kTile = 128;  // tokens per tile, and rows of a query tile
 constexpr int kTileLog2 = 7;
 constexpr int kGroups = kTile / 16;
-constexpr int kThreads = 512;
+constexpr int kThreads = 448;
 constexpr int kConvThreads = 128;
 constexpr int kStages = 2;       // converted tiles of keys, and of values
 constexpr int kFactors = 8;      // slots of per-tile factors: more tiles than the ring lets the producer be ahead
@@ -54,13 +53,6 @@ constexpr uint32_t kTmemCols = 512;
 constexpr float kRaise = 8.0f;   // log2 units
 constexpr int kTickets = 8;      // per CTA: one for each 32 rows
 static_assert(kTickets <= kKv8TicketsPerSm, "workspace layout");
-// Register split (setmaxnreg) of the launch's 512 x 128: softmax 2 x 128 threads, control and converters 128 each.
-constexpr int kLaunchRegs = 128;
-constexpr int kSoftmaxRegs = 176;
-constexpr int kControlRegs = 72;
-constexpr int kConvRegs = 88;
-static_assert(256 * kSoftmaxRegs + 128 * kControlRegs + 128 * kConvRegs <= kThreads * kLaunchRegs, "register split");
-
 enum : uint32_t {
   PSITE_PRODUCER = 51,
   PSITE_CONVERT = 52,
@@ -135,23 +127,32 @@ __device__ __forceinline__ void tma_load_5d(const CUtensorMap* map, uint64_t* ba
       : "memory");
 }
 
-// D[tmem] (+)= A[smem] . B[smem] and A[tmem] . B[smem], 16-bit operands.
+// D[tmem] (+)= A[smem] . B[smem] and A[tmem] . B[smem], 16-bit operands. Issued by one
+// elected lane of a converged warp from values that the compiler knows to be the same in
+// all its lanes: issued by a lone thread, each product costs about 148 clocks of moves
+// into uniform registers, whatever its size; so issued, 128 x 128 x 16 takes its 64.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  const uint32_t z = 0;
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  const uint32_t z = 0;
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// A value that is the same in all lanes, in a form that the compiler knows it to be.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(~0u, x, 0); }
 
 // The first 16 of r.
 __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
@@ -304,7 +305,7 @@ __device__ __forceinline__ void convert16(const uint4& u, uint4& a, uint4& b) {
 // One tile of codes [128][kD] -> the 16-bit swizzled tile. kClear: tokens that are not there become 0.
 template <int kFmt, int kD, bool kBf16, bool kClear>
 __device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, const float4* factor, int limit) {
-  const int tid = threadIdx.x & (kConvThreads - 1);
+  const int tid = static_cast<int>(threadIdx.x) - 10 * 32;
   constexpr int kPer = kD / 16;  // 16-byte pieces per token, and per thread
 #pragma unroll 2
   for (int i = 0; i < kPer; ++i) {
@@ -424,8 +425,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   if (x0 < x1) it = locate(p, x0, tile);
   int64_t x = x0;
 
-  if (warp >= 8 && warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+  if (warp == 8 || warp == 9) {
     if (warp == 8) {
       // -------------------------------------------------------- producer
       const int sub = min(p.a.c.block_log2, kTileLog2);  // log2 of tokens per TMA box
@@ -509,31 +509,46 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           }
         }
       }
-    } else if (warp == 9 && lane == 0) {
+    } else {
       // ------------------------------------------------------ MMA issuer
       uint32_t g = 0, ui = 0;
       bool ok = true;
+      const uint32_t tm = static_cast<uint32_t>(uniform(static_cast<int>(tmem)));
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok) ok = mbar_wait_inl(bar, parity, abort_flag, p.timeout_ns, PSITE_MMA);
+        if (ok) ok = warp_wait(bar, parity, abort_flag, p.timeout_ns, PSITE_MMA);
         return ok;
       };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) umma_commit(bar);
+        __syncwarp();
+      };
       auto issue_s = [&](int t, uint32_t gj) {
-        const int st = static_cast<int>(gj % kStages);
+        const int st = uniform(static_cast<int>(gj % kStages)), qt = uniform(t);
+        if (elect_one()) {
+          const uint32_t d = tm + static_cast<uint32_t>(qt) * 128u;
 #pragma unroll
-        for (int i = 0; i < C::kBlocks; ++i) {
-          const uint64_t qd = make_sw128_desc(s.q[t] + i * kBlockBytes), kd = make_sw128_desc(s.k[st] + i * kBlockBytes);
+          for (int i = 0; i < C::kBlocks; ++i) {
+            const uint64_t qd = make_sw128_desc(s.q[qt] + i * kBlockBytes), kd = make_sw128_desc(s.k[st] + i * kBlockBytes);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_ss(tmem + C::s_col(t), qd + kk * 2, kd + kk * 2, p.idesc_s, i > 0 || kk > 0 ? 1u : 0u);
+            for (int kk = 0; kk < 4; ++kk) mma_ss(d, qd + kk * 2, kd + kk * 2, p.idesc_s, i > 0 || kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&s.s_full[qt]);
         }
-        umma_commit(&s.s_full[t]);
+        __syncwarp();
       };
       auto issue_pv = [&](int t, uint32_t gj, bool first) {
-        const uint64_t vd = value_desc(s.v[gj % kStages]);
+        const int st = uniform(static_cast<int>(gj % kStages)), qt = uniform(t);
+        const uint32_t onto = static_cast<uint32_t>(uniform(first ? 0 : 1));
+        if (elect_one()) {
+          const uint64_t vd = value_desc(s.v[st]);
+          const uint32_t d = tm + C::o_col(0) + static_cast<uint32_t>(qt) * (C::o_col(1) - C::o_col(0));
+          const uint32_t a = tm + C::p_col(0) + static_cast<uint32_t>(qt) * (C::p_col(1) - C::p_col(0));
 #pragma unroll
-        for (int kk = 0; kk < kTile / 16; ++kk)
-          mma_ts(tmem + C::o_col(t), tmem + C::p_col(t) + kk * 8, vd + kk * (2048 >> 4), p.idesc_o, first && kk == 0 ? 0u : 1u);
-        umma_commit(&s.pv_done[t]);
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            mma_ts(d, a + kk * 8, vd + kk * (2048 >> 4), p.idesc_o, kk == 0 ? onto : 1u);
+          umma_commit(&s.pv_done[qt]);
+        }
+        __syncwarp();
       };
       while (x < x1 && ok) {
         const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
@@ -548,9 +563,9 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           issue_s(t, g);
         }
         if (!ok) break;
-        umma_commit(&s.k_empty[g % kStages]);
+        commit(&s.k_empty[g % kStages]);
         if (n == 1)
-          for (int t = 0; t < nq; ++t) umma_commit(&s.q_empty[t]);
+          for (int t = 0; t < nq; ++t) commit(&s.q_empty[t]);
         for (int j = 0; j < n && ok; ++j) {
           const uint32_t gj = g + static_cast<uint32_t>(j), gn = gj + 1;
           auto next_scores = [&](int t) {
@@ -577,29 +592,25 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             }
           }
           if (!ok) break;
-          umma_commit(&s.v_empty[gj % kStages]);
+          commit(&s.v_empty[gj % kStages]);
           if (j + 1 < n) {
-            umma_commit(&s.k_empty[gn % kStages]);
+            commit(&s.k_empty[gn % kStages]);
             if (j + 2 == n)  // the item's last scores are issued
-              for (int t = 0; t < nq; ++t) umma_commit(&s.q_empty[t]);
+              for (int t = 0; t < nq; ++t) commit(&s.q_empty[t]);
           }
         }
         g += static_cast<uint32_t>(n);
         ++ui;
         x += n;
         tile = 0;
-        if (x < x1) {
-          // next_item, by one thread (tiles_of uses no warp operations)
-          next_item(p, it);
-        }
+        if (x < x1) next_item(p, it);
       }
       // TMEM and the barriers are in use until every product issued has finished.
-      umma_commit(&s.drain);
+      commit(&s.drain);
       int dummy = 0;
       mbar_wait_inl(&s.drain, 0, &dummy, ok ? p.timeout_ns : 100000000ull, PSITE_DRAIN);
     }
-  } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
+  } else if (warp >= 10) {
     // ---------------------------------------------------------- converters
     uint32_t unit = 0;
     bool ok = true;
@@ -626,7 +637,6 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------- softmax
     const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -863,11 +873,6 @@ int launch_prompt(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMa
     std::lock_guard<std::mutex> lock(mu);
     if (static_cast<int>(configured.size()) <= dev) configured.resize(dev + 1, 0);
     if (!configured[dev]) {
-      cudaFuncAttributes fa;
-      if (int e = cuda_check(cudaFuncGetAttributes(&fa, kv8_prompt_kernel<kFmt, kD, kBf16>), "kv8 prompt function attributes"))
-        return e;
-      if (fa.numRegs < kLaunchRegs)  // the setmaxnreg split would wait for registers that do not exist
-        return fail(WBK_ERR_UNSUPPORTED, "kv8 prompt kernel built with %d registers per thread, needs %d", fa.numRegs, kLaunchRegs);
       if (int e = cuda_check(cudaFuncSetAttribute(kv8_prompt_kernel<kFmt, kD, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                   static_cast<int>(smem)),
                              "kv8 prompt smem attribute"))
