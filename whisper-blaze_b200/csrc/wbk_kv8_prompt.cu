@@ -19,10 +19,12 @@
 //     SMs alike. An item that lies in several CTAs is joined by the last of them,
 //     per 32 rows, in the order of the list.
 //   * Warps 0-3 and 4-7: softmax of one query tile each, a row per thread; 8: TMA
-//     producer; 9: tcgen05 issuer; 10-13: converters. With head_dim 64 scores and weights have their own TMEM columns; with
-//     128 the weights replace their scores, and the next scores of a tile wait for
-//     its output product (commit and wait: the order of products with different
-//     accumulators is not guaranteed).
+//     producer; 9 and 14: tcgen05 issuers, one per query tile; 10-13: converters.
+//   * Scores are computed for 64 tokens at a time, in two sets of TMEM columns per
+//     query tile, and the weights replace their scores there. While a softmax warpgroup
+//     works on one half of a tile, the tensor cores finish the other half's product and
+//     then bring its next scores (the order of products with different accumulators is
+//     not guaranteed, so the issuer waits for the first).
 //
 // The softmax is that of the few-rows kernel: running maximum of
 // log2(e) * scale * q.k + log2(value scale), raised when it is passed by 2^8.
@@ -44,8 +46,10 @@ namespace {
 constexpr int kTile = 128;  // tokens per tile, and rows of a query tile
 constexpr int kTileLog2 = 7;
 constexpr int kGroups = kTile / 16;
-constexpr int kThreads = 448;
+constexpr int kHalf = kTile / 2;      // tokens of one score product
+constexpr int kThreads = 480;
 constexpr int kConvThreads = 128;
+constexpr int kConvWarp = 10;  // the first of them
 constexpr int kStages = 2;       // converted tiles of keys, and of values
 constexpr int kFactors = 8;      // slots of per-tile factors: more tiles than the ring lets the producer be ahead
 constexpr int kBlockBytes = kTile * 128;  // 64 channels of a 16-bit tile
@@ -63,15 +67,14 @@ enum : uint32_t {
 
 template <int kD>
 struct Cfg {
-  static constexpr bool kAlias = kD == 128;           // weights in their scores' columns
   static constexpr int kRawUnits = kD == 64 ? 4 : 2;  // tiles of codes: keys and values in turn
   static constexpr int kRawBytes = kTile * kD;
   static constexpr int kBlocks = kD / 64;
   static constexpr int kTileBytes = kBlocks * kBlockBytes;
-  static constexpr uint32_t s_col(int t) { return static_cast<uint32_t>(t * 128); }
-  static constexpr uint32_t p_col(int t) { return kAlias ? s_col(t) : static_cast<uint32_t>(256 + t * 64); }
-  static constexpr uint32_t o_col(int t) { return kAlias ? static_cast<uint32_t>(256 + t * 128) : static_cast<uint32_t>(384 + t * 64); }
 };
+// TMEM columns: scores, then weights, of half h of query tile t; sums of query tile t.
+__device__ __forceinline__ uint32_t s_col(int t, int h) { return static_cast<uint32_t>(t * 128 + h * 64); }
+__device__ __forceinline__ uint32_t o_col(int t) { return static_cast<uint32_t>(256 + t * 128); }
 
 template <int kD>
 struct PromptSmem {
@@ -84,7 +87,7 @@ struct PromptSmem {
   uint32_t holes[kFactors];          // groups below the limit whose page is outside the pool
   uint64_t q_full[2], q_empty[2], raw_full[Cfg<kD>::kRawUnits], raw_empty[Cfg<kD>::kRawUnits];
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], factor_full[kFactors];
-  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2], drain;
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], o_free[2], drain[2];  // [query tile][half]
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -193,12 +196,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(~0u, mbar_wait_inl(bar, parity, abort_flag, timeout_ns, site));
 }
 
-// One arrival for a warp, after what all its lanes did.
-__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-}
-
 // One item of the work list: query positions pos0 .. of sequence b, KV head h.
 struct Item {
   int b, pb, h;
@@ -302,24 +299,42 @@ __device__ __forceinline__ void convert16(const uint4& u, uint4& a, uint4& b) {
   b = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
-// One tile of codes [128][kD] -> the 16-bit swizzled tile. kClear: tokens that are not there become 0.
-template <int kFmt, int kD, bool kBf16, bool kClear>
-__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, const float4* factor, int limit) {
-  const int tid = static_cast<int>(threadIdx.x) - 10 * 32;
-  constexpr int kPer = kD / 16;  // 16-byte pieces per token, and per thread
-#pragma unroll 2
+// One arrival for a warp, after what all its lanes did.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// One tile of codes [128][kD] -> the 16-bit swizzled tile; `raw_empty` is given back as soon as the codes are read.
+// `clear`: tokens at or after `limit`, or in groups that are not there, become 0.
+template <int kFmt, int kD, bool kBf16>
+__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* dst, uint64_t* raw_empty, bool clear,
+                                             const float4* factor, int limit) {
+  const int tid = static_cast<int>(threadIdx.x) - kConvWarp * 32;
+  constexpr int kPer = kD / 16;                     // 16-byte pieces per token, and per thread
+  constexpr int kStep = kConvThreads / kPer;        // tokens from one piece of a thread to its next
+  const int token = tid / kPer, piece = tid % kPer;
+  uint4 u[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) u[i] = *reinterpret_cast<const uint4*>(raw + (tid + i * kConvThreads) * 16);
+  if (clear) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (token + i * kStep >= limit || factor[(token + i * kStep) >> 4].z == 0.0f) u[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  warp_arrive(raw_empty);
+  // 8 lanes store to 8 different 16-byte columns: those of the second 64 channels start with the odd one
+  const int j = (piece & 3) * 2, sw = token & 7;  // kStep is a multiple of 8
+  const bool odd = piece >= 4;
+  uint8_t* row = dst + (piece >> 2) * kBlockBytes + token * 128;
+  uint8_t* one = row + (((j + odd) ^ sw) << 4);
+  uint8_t* two = row + (((j + !odd) ^ sw) << 4);
+#pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int id = tid + i * kConvThreads, token = id / kPer, piece = id % kPer;
-    uint4 u = *reinterpret_cast<const uint4*>(raw + id * 16);
-    if (kClear && (token >= limit || factor[token >> 4].z == 0.0f)) u = make_uint4(0u, 0u, 0u, 0u);
     uint4 a, b;
-    convert16<kFmt, kBf16>(u, a, b);
-    // 8 lanes store to 8 different 16-byte columns: those of the second 64 channels start with the odd one
-    const int block = piece >> 2, j = (piece & 3) * 2, sw = token & 7;
-    uint8_t* row = dst + block * kBlockBytes + token * 128;
-    const bool odd = block != 0;
-    *reinterpret_cast<uint4*>(row + (((j + odd) ^ sw) << 4)) = odd ? b : a;
-    *reinterpret_cast<uint4*>(row + (((j + !odd) ^ sw) << 4)) = odd ? a : b;
+    convert16<kFmt, kBf16>(u[i], a, b);
+    *reinterpret_cast<uint4*>(one + i * kStep * 128) = odd ? b : a;
+    *reinterpret_cast<uint4*>(two + i * kStep * 128) = odd ? a : b;
   }
 }
 
@@ -330,8 +345,7 @@ __device__ __forceinline__ void hide(uint32_t (&y)[32], int lim, uint32_t holes)
     if (k >= lim || (holes >> (k >> 4) & 1u)) y[k] = 0xFF800000u;  // -inf
 }
 // The largest x + log2 vs of 32 columns.
-__device__ __forceinline__ float largest(uint32_t (&y)[32], const float4* factor, int lim, uint32_t holes, bool edge) {
-  if (edge) hide(y, lim, holes);
+__device__ __forceinline__ float largest(const uint32_t (&y)[32], const float4* factor) {
   float mx = -INFINITY;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -345,9 +359,7 @@ __device__ __forceinline__ float largest(uint32_t (&y)[32], const float4* factor
 }
 // The weights of 32 columns relative to 2^ref, as fp16 pairs in y[0 .. 15]; returns their sum over the value scales, of
 // the fp32 weights (as fp16 those of a page of small value scale may be 0).
-__device__ __forceinline__ float weights(uint32_t (&y)[32], const float4* factor, int lim, uint32_t holes, bool edge,
-                                         float ref) {
-  if (edge) hide(y, lim, holes);
+__device__ __forceinline__ float weights(uint32_t (&y)[32], const float4* factor, float ref) {
   float sum = 0.0f;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -382,11 +394,13 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s.q_full[t], 1);
       mbar_init(&s.q_empty[t], 1);
-      mbar_init(&s.s_full[t], 1);
-      mbar_init(&s.s_free[t], 4);  // one arrival per warp
-      mbar_init(&s.p_full[t], 4);
-      mbar_init(&s.pv_done[t], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&s.s_full[t][h], 1);
+        mbar_init(&s.p_full[t][h], 4);  // one arrival per warp
+        mbar_init(&s.pv_done[t][h], 1);
+      }
       mbar_init(&s.o_free[t], 4);
+      mbar_init(&s.drain[t], 1);
     }
     for (int i = 0; i < C::kRawUnits; ++i) {
       mbar_init(&s.raw_full[i], 1);
@@ -394,12 +408,11 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.k_full[i], kConvThreads / 32);
-      mbar_init(&s.k_empty[i], 1);
+      mbar_init(&s.k_empty[i], static_cast<uint32_t>(nq));  // one per issuer
       mbar_init(&s.v_full[i], kConvThreads / 32);
-      mbar_init(&s.v_empty[i], 1);
+      mbar_init(&s.v_empty[i], static_cast<uint32_t>(nq));
     }
     for (int i = 0; i < kFactors; ++i) mbar_init(&s.factor_full[i], 1);
-    mbar_init(&s.drain, 1);
     s.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_tmap(&tmap_q);
@@ -425,7 +438,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   if (x0 < x1) it = locate(p, x0, tile);
   int64_t x = x0;
 
-  if (warp == 8 || warp == 9) {
+  if (warp == 8 || warp == 9 || warp == 14) {
     if (warp == 8) {
       // -------------------------------------------------------- producer
       const int sub = min(p.a.c.block_log2, kTileLog2);  // log2 of tokens per TMA box
@@ -510,9 +523,10 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         }
       }
     } else {
-      // ------------------------------------------------------ MMA issuer
+      // ------------------------------------- MMA issuers: warp 9 query tile 0, warp 14 query tile 1
+      const int t = warp == 9 ? 0 : 1;
       uint32_t g = 0, ui = 0;
-      bool ok = true;
+      bool ok = t < nq;
       const uint32_t tm = static_cast<uint32_t>(uniform(static_cast<int>(tmem)));
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (ok) ok = warp_wait(bar, parity, abort_flag, p.timeout_ns, PSITE_MMA);
@@ -522,81 +536,72 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         if (elect_one()) umma_commit(bar);
         __syncwarp();
       };
-      auto issue_s = [&](int t, uint32_t gj) {
-        const int st = uniform(static_cast<int>(gj % kStages)), qt = uniform(t);
+      const int qt = uniform(t);
+      auto issue_s = [&](int h, uint32_t gj) {
+        const int st = uniform(static_cast<int>(gj % kStages)), qh = uniform(h);
         if (elect_one()) {
-          const uint32_t d = tm + static_cast<uint32_t>(qt) * 128u;
+          const uint32_t d = tm + s_col(qt, qh);
 #pragma unroll
           for (int i = 0; i < C::kBlocks; ++i) {
-            const uint64_t qd = make_sw128_desc(s.q[qt] + i * kBlockBytes), kd = make_sw128_desc(s.k[st] + i * kBlockBytes);
+            const uint64_t qd = make_sw128_desc(s.q[qt] + i * kBlockBytes);
+            const uint64_t kd = make_sw128_desc(s.k[st] + i * kBlockBytes + qh * (kHalf * 128));
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) mma_ss(d, qd + kk * 2, kd + kk * 2, p.idesc_s, i > 0 || kk > 0 ? 1u : 0u);
           }
-          umma_commit(&s.s_full[qt]);
+          umma_commit(&s.s_full[qt][qh]);
         }
         __syncwarp();
       };
-      auto issue_pv = [&](int t, uint32_t gj, bool first) {
-        const int st = uniform(static_cast<int>(gj % kStages)), qt = uniform(t);
+      auto issue_pv = [&](int h, uint32_t gj, bool first) {
+        const int st = uniform(static_cast<int>(gj % kStages)), qh = uniform(h);
         const uint32_t onto = static_cast<uint32_t>(uniform(first ? 0 : 1));
         if (elect_one()) {
-          const uint64_t vd = value_desc(s.v[st]);
-          const uint32_t d = tm + C::o_col(0) + static_cast<uint32_t>(qt) * (C::o_col(1) - C::o_col(0));
-          const uint32_t a = tm + C::p_col(0) + static_cast<uint32_t>(qt) * (C::p_col(1) - C::p_col(0));
+          const uint64_t vd = value_desc(s.v[st] + qh * (kHalf * 128));
+          const uint32_t d = tm + o_col(qt), a = tm + s_col(qt, qh);
 #pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk)
+          for (int kk = 0; kk < kHalf / 16; ++kk)
             mma_ts(d, a + kk * 8, vd + kk * (2048 >> 4), p.idesc_o, kk == 0 ? onto : 1u);
-          umma_commit(&s.pv_done[qt]);
+          umma_commit(&s.pv_done[qt][qh]);
         }
         __syncwarp();
       };
       while (x < x1 && ok) {
         const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
         const int n = t1 - tile;
-        for (int t = 0; t < nq; ++t) wait(&s.q_full[t], ui & 1u);
+        wait(&s.q_full[t], ui & 1u);
         wait(&s.k_full[g % kStages], (g / kStages) & 1u);
-        for (int t = 0; t < nq; ++t) {
-          if (!C::kAlias) wait(&s.s_free[t], (g & 1u) ^ 1u);
-          else if (g > 0) wait(&s.pv_done[t], (g - 1) & 1u);
+        for (int h = 0; h < 2; ++h) {
+          if (g > 0) wait(&s.pv_done[t][h], (g - 1) & 1u);
           if (!ok) break;
           tc_fence_after();
-          issue_s(t, g);
+          issue_s(h, g);
         }
         if (!ok) break;
         commit(&s.k_empty[g % kStages]);
-        if (n == 1)
-          for (int t = 0; t < nq; ++t) commit(&s.q_empty[t]);
+        if (n == 1) commit(&s.q_empty[t]);
         for (int j = 0; j < n && ok; ++j) {
           const uint32_t gj = g + static_cast<uint32_t>(j), gn = gj + 1;
-          auto next_scores = [&](int t) {
-            if (C::kAlias) wait(&s.pv_done[t], gj & 1u);
-            else wait(&s.s_free[t], gj & 1u);
-            if (!ok) return;
-            tc_fence_after();
-            issue_s(t, gn);
-          };
-          if (!C::kAlias && j + 1 < n) {
-            wait(&s.k_full[gn % kStages], (gn / kStages) & 1u);
-            for (int t = 0; t < nq && ok; ++t) next_scores(t);
-          }
           wait(&s.v_full[gj % kStages], (gj / kStages) & 1u);
-          for (int t = 0; t < nq && ok; ++t) {
-            wait(&s.p_full[t], gj & 1u);
-            if (j == 0) wait(&s.o_free[t], (ui & 1u) ^ 1u);
+          for (int h = 0; h < 2; ++h) {
+            wait(&s.p_full[t][h], gj & 1u);
+            if (j == 0 && h == 0) wait(&s.o_free[t], (ui & 1u) ^ 1u);
             if (!ok) break;
             tc_fence_after();
-            issue_pv(t, gj, j == 0);
-            if (C::kAlias && j + 1 < n) {
-              if (t == 0) wait(&s.k_full[gn % kStages], (gn / kStages) & 1u);
-              next_scores(t);
+            issue_pv(h, gj, j == 0 && h == 0);
+            if (j + 1 < n) {
+              // the half's next scores replace the weights that this product reads
+              if (h == 0) wait(&s.k_full[gn % kStages], (gn / kStages) & 1u);
+              wait(&s.pv_done[t][h], gj & 1u);
+              if (!ok) break;
+              tc_fence_after();
+              issue_s(h, gn);
             }
           }
           if (!ok) break;
           commit(&s.v_empty[gj % kStages]);
           if (j + 1 < n) {
             commit(&s.k_empty[gn % kStages]);
-            if (j + 2 == n)  // the item's last scores are issued
-              for (int t = 0; t < nq; ++t) commit(&s.q_empty[t]);
+            if (j + 2 == n) commit(&s.q_empty[t]);  // the item's last scores are issued
           }
         }
         g += static_cast<uint32_t>(n);
@@ -606,9 +611,9 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         if (x < x1) next_item(p, it);
       }
       // TMEM and the barriers are in use until every product issued has finished.
-      commit(&s.drain);
+      commit(&s.drain[t]);
       int dummy = 0;
-      mbar_wait_inl(&s.drain, 0, &dummy, ok ? p.timeout_ns : 100000000ull, PSITE_DRAIN);
+      mbar_wait_inl(&s.drain[t], 0, &dummy, ok ? p.timeout_ns : 100000000ull, PSITE_DRAIN);
     }
   } else if (warp >= 10) {
     // ---------------------------------------------------------- converters
@@ -626,14 +631,11 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         if (ok) ok = warp_wait(&s.raw_full[u], (unit / C::kRawUnits) & 1u, abort_flag, p.timeout_ns, PSITE_CONVERT);
         if (ok) ok = warp_wait(kv == 0 ? &s.k_empty[st] : &s.v_empty[st], empty, abort_flag, p.timeout_ns, PSITE_CONVERT);
         if (!ok) break;
-        if (kv == 0) convert_tile<kFmt, kD, kBf16, false>(s.raw[u], s.k[st], s.factor[slot], 0);
-        else convert_tile<kFmt, kD, false, true>(s.raw[u], s.v[st], s.factor[slot], s.limit[slot]);
+        if (kv == 0) convert_tile<kFmt, kD, kBf16>(s.raw[u], s.k[st], &s.raw_empty[u], false, nullptr, 0);
+        else convert_tile<kFmt, kD, false>(s.raw[u], s.v[st], &s.raw_empty[u], s.limit[slot] < kTile || s.holes[slot] != 0,
+                                           s.factor[slot], s.limit[slot]);
         fence_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&s.raw_empty[u]);
-          mbar_arrive(kv == 0 ? &s.k_full[st] : &s.v_full[st]);
-        }
+        warp_arrive(kv == 0 ? &s.k_full[st] : &s.v_full[st]);
       }
     }
   } else {
@@ -649,85 +651,67 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const int seq = kv8_len(p.a.lens, it.b, p.a.c);
       const int vis = i >= it.n ? 0 : p.a.causal ? max(seq - it.n + i + 1, 0) : seq;
       float m = -INFINITY, l = 0.0f;
-      for (int tt = tile; tt < t1; ++tt, ++g) {
-        const int slot = static_cast<int>(g % kFactors);
-        if (!warp_wait(&s.factor_full[slot], (g / kFactors) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX) ||
-            !warp_wait(&s.s_full[t], g & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) {
+      for (int hh = 2 * tile; hh < 2 * t1; ++hh) {  // 64 tokens at a time
+        const int h = hh & 1, slot = static_cast<int>(g % kFactors);
+        if ((h == 0 && !warp_wait(&s.factor_full[slot], (g / kFactors) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) ||
+            !warp_wait(&s.s_full[t][h], g & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t sa = lane_addr + C::s_col(t), pa = lane_addr + C::p_col(t);
-        const uint32_t holes = s.holes[slot];
-        const int lim = vis - tt * kTile;
-        const bool edge = holes != 0 || __any_sync(~0u, lim < kTile);
-        const float4* fac = s.factor[slot];
-        // Both passes over the scores read them from TMEM, 32 columns at a time, the next 32 on their way meanwhile: as
-        // straight-line code over 128 registers they ran at 4 clocks an instruction, starved of instructions.
+        const uint32_t sa = lane_addr + s_col(t, h);
         uint32_t ya[32], yb[32];
-        // ---- the row's largest x + log2 vs: factors are positive, so that of a group is that of its largest score
-        float mx = -INFINITY;
         tmem_ld_32x32b_x32(sa, ya);
-#pragma unroll 1
-        for (int c = 0; c < 4; c += 2) {
-          tmem_ld_wait(ya);
-          tmem_ld_32x32b_x32(sa + (c + 1) * 32, yb);
-          mx = fmaxf(mx, largest(ya, fac + 2 * c, lim - 32 * c, holes >> (2 * c), edge));
-          tmem_ld_wait(yb);
-          tmem_ld_32x32b_x32(sa + ((c + 2) & 3) * 32, ya);  // in the end the first again, for the second pass
-          mx = fmaxf(mx, largest(yb, fac + 2 * c + 2, lim - 32 * c - 32, holes >> (2 * c + 2), edge));
+        tmem_ld_32x32b_x32(sa + 32, yb);
+        const uint32_t holes = s.holes[slot] >> (4 * h);
+        const int lim = vis - hh * kHalf;
+        const bool edge = holes != 0 || __any_sync(~0u, lim < kHalf);
+        const float4* fac = s.factor[slot] + 4 * h;
+        tmem_ld_wait(ya);
+        tmem_ld_wait(yb);
+        if (edge) {
+          hide(ya, lim, holes);
+          hide(yb, lim - 32, holes >> 2);
         }
+        // ---- the row's largest x + log2 vs: factors are positive, so that of a group is that of its largest score
+        const float mx = fmaxf(largest(ya, fac), largest(yb, fac + 2));
         float alpha = 1.0f;
         if (mx > m + kRaise) {
           alpha = ex2(m - mx);
           m = mx;
         }
         l *= alpha;
-        const bool rescale = tt > tile && __any_sync(~0u, alpha != 1.0f);
         const float ref = m == -INFINITY ? 0.0f : m;
-        if (tt > tile) {
-          // the weights' columns and the sums are free once the previous output product is done
-          if (!warp_wait(&s.pv_done[t], (g - 1) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) {
+        // ---- weights, in place of their scores
+        l += weights(ya, fac, ref);
+        tmem_st_x16(sa, ya);
+        l += weights(yb, fac + 2, ref);
+        tmem_st_x16(sa + 16, yb);
+        if (hh > 2 * tile && __any_sync(~0u, alpha != 1.0f)) {
+          // the sums are free once the previous half's product is done
+          if (!warp_wait(&s.pv_done[t][h ^ 1], (h == 1 ? g : g - 1) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) {
             ok = false;
             break;
           }
           tc_fence_after();
-        }
-        // ---- weights; where they replace their scores, 16 columns end before the next 32 begin
-#pragma unroll 1
-        for (int c = 0; c < 4; c += 2) {
-          tmem_ld_wait(ya);
-          tmem_ld_32x32b_x32(sa + (c + 1) * 32, yb);
-          l += weights(ya, fac + 2 * c, lim - 32 * c, holes >> (2 * c), edge, ref);
-          tmem_st_x16(pa + c * 16, ya);
-          tmem_ld_wait(yb);
-          if (c == 0) tmem_ld_32x32b_x32(sa + 64, ya);
-          l += weights(yb, fac + 2 * c + 2, lim - 32 * c - 32, holes >> (2 * c + 2), edge, ref);
-          tmem_st_x16(pa + c * 16 + 16, yb);
-        }
-        if (!C::kAlias) {
-          tc_fence_before();
-          warp_arrive(&s.s_free[t]);
-        }
-        if (rescale) {
 #pragma unroll 1
           for (int c = 0; c < kD / 32; ++c) {
-            uint32_t orr[32];
-            const uint32_t oa = lane_addr + C::o_col(t) + c * 32;
-            tmem_ld_32x32b_x32(oa, orr);
-            tmem_ld_wait(orr);
+            const uint32_t oa = lane_addr + o_col(t) + c * 32;
+            tmem_ld_32x32b_x32(oa, yb);
+            tmem_ld_wait(yb);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) orr[k] = __float_as_uint(__uint_as_float(orr[k]) * alpha);
-            tmem_st_x32(oa, orr);
+            for (int k = 0; k < 32; ++k) yb[k] = __float_as_uint(__uint_as_float(yb[k]) * alpha);
+            tmem_st_x32(oa, yb);
           }
         }
         tmem_st_wait();
         tc_fence_before();
-        warp_arrive(&s.p_full[t]);
+        warp_arrive(&s.p_full[t][h]);
+        if (h == 1) ++g;
       }
       if (!ok) break;
       // ---- the item's rows: output, or this CTA's part of it
-      if (!warp_wait(&s.pv_done[t], (g - 1) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) break;
+      if (!warp_wait(&s.pv_done[t][1], (g - 1) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) break;
       tc_fence_after();
       const bool whole = tile == 0 && t1 == it.tiles;
       const int row = t * kTile + r;
@@ -738,7 +722,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll 1
       for (int c = 0; c < kD / 32; ++c) {
         uint32_t orr[32];
-        tmem_ld_32x32b_x32(lane_addr + C::o_col(t) + c * 32, orr);
+        tmem_ld_32x32b_x32(lane_addr + o_col(t) + c * 32, orr);
         tmem_ld_wait(orr);
         if (c == kD / 32 - 1) {  // read to the end: the next item's first product may overwrite it
           tc_fence_before();
@@ -904,7 +888,7 @@ int kv8_prompt_attention(const Kv8Attention& a, void* workspace, cudaStream_t st
   p.tiles_q = a.queries > p.tile_pos ? 2 : 1;
   const int64_t per = static_cast<int64_t>(p.tile_pos) * p.tiles_q;
   p.pos_blocks = static_cast<int>((a.queries + per - 1) / per);
-  p.idesc_s = instruction(kTile, a.bf16, false);
+  p.idesc_s = instruction(kHalf, a.bf16, false);
   p.idesc_o = instruction(a.head_dim, false, true);
   p.tickets = static_cast<uint32_t*>(workspace);
   p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kv8_ticket_bytes());
