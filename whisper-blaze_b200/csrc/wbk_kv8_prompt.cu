@@ -193,7 +193,7 @@ __device__ __forceinline__ uint64_t value_desc(const void* p) {
 // A wait of a whole warp with one result for all lanes.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns,
                                           uint32_t site) {
-  return __all_sync(~0u, mbar_wait_inl(bar, parity, abort_flag, timeout_ns, site));
+  return __all_sync(~0u, mbar_wait(bar, parity, abort_flag, timeout_ns, site));
 }
 
 // One item of the work list: query positions pos0 .. of sequence b, KV head h.
@@ -476,7 +476,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           const bool load = lane < kGroups && there && (lane & ((1 << (sub - 4)) - 1)) == 0;
           const uint32_t bytes = __popc(__ballot_sync(~0u, load)) * (static_cast<uint32_t>(kD) << sub);
           const int y = (it.h << p.a.c.block_log2) + (pos & (p.a.c.block - 1));
-#pragma unroll
+#pragma unroll 1
           for (int kv = 0; kv < 2; ++kv, ++unit) {
             const int u = static_cast<int>(unit % C::kRawUnits);
             if (ok) ok = warp_wait(&s.raw_empty[u], ((unit / C::kRawUnits) & 1u) ^ 1u, abort_flag, p.timeout_ns, PSITE_PRODUCER);
@@ -510,15 +510,15 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         int dummy = 0;
         const uint64_t limit = ok ? p.timeout_ns : 100000000ull;
         for (uint32_t i = unit > C::kRawUnits ? unit - C::kRawUnits : 0; i < unit; ++i)
-          mbar_wait_inl(&s.raw_full[i % C::kRawUnits], (i / C::kRawUnits) & 1u, &dummy, limit, PSITE_DRAIN);
+          mbar_wait(&s.raw_full[i % C::kRawUnits], (i / C::kRawUnits) & 1u, &dummy, limit, PSITE_DRAIN);
         if (q_loads > 0)
-          for (int qt = 0; qt < nq; ++qt) mbar_wait_inl(&s.q_full[qt], (q_loads - 1) & 1u, &dummy, limit, PSITE_DRAIN);
+          for (int qt = 0; qt < nq; ++qt) mbar_wait(&s.q_full[qt], (q_loads - 1) & 1u, &dummy, limit, PSITE_DRAIN);
         if (ok) {  // and no commit to these barriers is still on its way
           if (q_loads > 0)
-            for (int qt = 0; qt < nq; ++qt) mbar_wait_inl(&s.q_empty[qt], (q_loads - 1) & 1u, abort_flag, limit, PSITE_DRAIN);
+            for (int qt = 0; qt < nq; ++qt) mbar_wait(&s.q_empty[qt], (q_loads - 1) & 1u, abort_flag, limit, PSITE_DRAIN);
           for (uint32_t i = g > kStages ? g - kStages : 0; i < g; ++i) {
-            mbar_wait_inl(&s.k_empty[i % kStages], (i / kStages) & 1u, abort_flag, limit, PSITE_DRAIN);
-            mbar_wait_inl(&s.v_empty[i % kStages], (i / kStages) & 1u, abort_flag, limit, PSITE_DRAIN);
+            mbar_wait(&s.k_empty[i % kStages], (i / kStages) & 1u, abort_flag, limit, PSITE_DRAIN);
+            mbar_wait(&s.v_empty[i % kStages], (i / kStages) & 1u, abort_flag, limit, PSITE_DRAIN);
           }
         }
       }
@@ -569,36 +569,31 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
         const int n = t1 - tile;
         wait(&s.q_full[t], ui & 1u);
-        wait(&s.k_full[g % kStages], (g / kStages) & 1u);
-        for (int h = 0; h < 2; ++h) {
-          if (g > 0) wait(&s.pv_done[t][h], (g - 1) & 1u);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(h, g);
-        }
-        if (!ok) break;
-        commit(&s.k_empty[g % kStages]);
-        if (n == 1) commit(&s.q_empty[t]);
-        for (int j = 0; j < n && ok; ++j) {
+        // Half by half: the output product of tile j, then the scores of tile j + 1, which replace the weights that it
+        // read. Tile -1 has no product: the item's first scores follow the item before.
+#pragma unroll 1
+        for (int j = -1; j < n && ok; ++j) {
           const uint32_t gj = g + static_cast<uint32_t>(j), gn = gj + 1;
-          wait(&s.v_full[gj % kStages], (gj / kStages) & 1u);
+          if (j >= 0) wait(&s.v_full[gj % kStages], (gj / kStages) & 1u);
+#pragma unroll 1
           for (int h = 0; h < 2; ++h) {
-            wait(&s.p_full[t][h], gj & 1u);
-            if (j == 0 && h == 0) wait(&s.o_free[t], (ui & 1u) ^ 1u);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(h, gj, j == 0 && h == 0);
+            if (j >= 0) {
+              wait(&s.p_full[t][h], gj & 1u);
+              if (j == 0 && h == 0) wait(&s.o_free[t], (ui & 1u) ^ 1u);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(h, gj, j == 0 && h == 0);
+            }
             if (j + 1 < n) {
-              // the half's next scores replace the weights that this product reads
               if (h == 0) wait(&s.k_full[gn % kStages], (gn / kStages) & 1u);
-              wait(&s.pv_done[t][h], gj & 1u);
+              if (gn > 0) wait(&s.pv_done[t][h], gj & 1u);
               if (!ok) break;
               tc_fence_after();
               issue_s(h, gn);
             }
           }
           if (!ok) break;
-          commit(&s.v_empty[gj % kStages]);
+          if (j >= 0) commit(&s.v_empty[gj % kStages]);
           if (j + 1 < n) {
             commit(&s.k_empty[gn % kStages]);
             if (j + 2 == n) commit(&s.q_empty[t]);  // the item's last scores are issued
@@ -613,7 +608,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       // TMEM and the barriers are in use until every product issued has finished.
       commit(&s.drain[t]);
       int dummy = 0;
-      mbar_wait_inl(&s.drain[t], 0, &dummy, ok ? p.timeout_ns : 100000000ull, PSITE_DRAIN);
+      mbar_wait(&s.drain[t], 0, &dummy, ok ? p.timeout_ns : 100000000ull, PSITE_DRAIN);
     }
   } else if (warp >= 10) {
     // ---------------------------------------------------------- converters
@@ -625,15 +620,16 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const int st = static_cast<int>(g % kStages), slot = static_cast<int>(g % kFactors);
       const uint32_t empty = ((g / kStages) & 1u) ^ 1u;
       ok = warp_wait(&s.factor_full[slot], (g / kFactors) & 1u, abort_flag, p.timeout_ns, PSITE_CONVERT);
-#pragma unroll
+#pragma unroll 1
       for (int kv = 0; kv < 2; ++kv, ++unit) {
         const int u = static_cast<int>(unit % C::kRawUnits);
         if (ok) ok = warp_wait(&s.raw_full[u], (unit / C::kRawUnits) & 1u, abort_flag, p.timeout_ns, PSITE_CONVERT);
         if (ok) ok = warp_wait(kv == 0 ? &s.k_empty[st] : &s.v_empty[st], empty, abort_flag, p.timeout_ns, PSITE_CONVERT);
         if (!ok) break;
-        if (kv == 0) convert_tile<kFmt, kD, kBf16>(s.raw[u], s.k[st], &s.raw_empty[u], false, nullptr, 0);
-        else convert_tile<kFmt, kD, false>(s.raw[u], s.v[st], &s.raw_empty[u], s.limit[slot] < kTile || s.holes[slot] != 0,
-                                           s.factor[slot], s.limit[slot]);
+        const bool clear = kv == 1 && (s.limit[slot] < kTile || s.holes[slot] != 0);
+        uint8_t* to = kv == 0 ? s.k[st] : s.v[st];
+        if (kBf16 && kv == 0) convert_tile<kFmt, kD, kBf16>(s.raw[u], to, &s.raw_empty[u], false, s.factor[slot], 0);
+        else convert_tile<kFmt, kD, false>(s.raw[u], to, &s.raw_empty[u], clear, s.factor[slot], s.limit[slot]);
         fence_async_smem();
         warp_arrive(kv == 0 ? &s.k_full[st] : &s.v_full[st]);
       }
