@@ -10,7 +10,8 @@
 //     batches and one long sequence fill the SMs alike. Warps share nothing but the
 //     items that lie in several of them: such an item is joined first by the last warp
 //     of a CTA to finish, through shared memory, then by the last of its CTAs, through
-//     global memory, always in the order of the list.
+//     global memory, always in the order of the list. Short items are not split
+//     between CTAs.
 //   * Each warp keeps a ring of tiles in flight with TMA (swizzled, so that the
 //     fragment loads below have no bank conflicts) and looks pages and scales up 32
 //     at a time and one batch ahead.
@@ -27,6 +28,7 @@
 // sum (w_j / vs). So w_j, rounded to fp16, is relative to the largest product of
 // weight and value scale, and pages of small scale lose nothing.
 #include <algorithm>
+#include <climits>
 #include <mutex>
 #include <vector>
 
@@ -44,7 +46,8 @@ constexpr int kGroups = kTile / 16;
 constexpr int kRows = 8;           // query rows per item
 constexpr int kSlots = 6;          // partial results that the warps of a CTA can have for one another
 constexpr int kMaxStages = 4;
-constexpr int kMinShare = 256;     // tokens of a CTA's share, where the SMs are not full: two tiles per warp
+constexpr int kMinShare = 8;
+constexpr int kWhole = 16;         // tiles of an item that is not split between CTAs
 constexpr float kRaise = 8.0f;     // log2 units
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint64_t kDrainNs = 100000000ull;  // limit of the waits for copies in flight after a wait gave up
@@ -95,6 +98,13 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
+// Tiles of a CTA's share, at least, where the SMs are not full: two per warp, and more for long items. An item of L
+// tiles in P parts takes about a * L / P + b * P, with a the time of a tile in a CTA and b that of joining a part
+// (0.18 and 0.45 us), least at a share of L / P = sqrt(L * b / a).
+__device__ __forceinline__ int least_share(int total, int items) {
+  return max(kMinShare, static_cast<int>(1.6f * sqrtf(static_cast<float>(total) / items)));
+}
+
 // One item of the work list: KV head h of sequence b, rows kRows * rb onwards.
 struct Item {
   int b, h, rb;
@@ -109,45 +119,67 @@ __device__ __forceinline__ int tiles_of(const Kv8AttnParams& p, int b, int& len,
   return max((len + kTile - 1) >> kTileLog2, 1);
 }
 
-// Tiles of the whole list, by a converged warp.
-__device__ __forceinline__ int64_t total_tiles(const Kv8AttnParams& p) {
-  int64_t sum = 0;
-  int len, n;
+// Tiles of the whole list, by a converged warp. (The host keeps the list below 2^31 tiles.)
+__device__ __forceinline__ int total_tiles(const Kv8AttnParams& p) {
+  int sum = 0, len, n;
   for (int b = threadIdx.x & 31; b < p.batch; b += 32) sum += tiles_of(p, b, len, n);
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  return sum * p.c.kv_heads * p.row_blocks;
+  return __reduce_add_sync(~0u, sum) * p.c.kv_heads * p.row_blocks;
 }
 
 // The item and tile at place x of the list, by a converged warp.
-__device__ __forceinline__ Item locate(const Kv8AttnParams& p, int64_t x, int& tile) {
-  const int lane = threadIdx.x & 31;
-  const int64_t per = static_cast<int64_t>(p.c.kv_heads) * p.row_blocks;
+__device__ __forceinline__ Item locate(const Kv8AttnParams& p, int x, int& tile) {
+  const int lane = threadIdx.x & 31, per = p.c.kv_heads * p.row_blocks;
   Item it{};
   for (int b0 = 0;; b0 += 32) {
     int len = 0, n = 0;
     const int t = b0 + lane < p.batch ? tiles_of(p, b0 + lane, len, n) : 0;
-    int64_t upto = t;
+    int upto = t * per;
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(~0u, upto, o);
+      const int y = __shfl_up_sync(~0u, upto, o);
       if (lane >= o) upto += y;
     }
-    const uint32_t past = __ballot_sync(~0u, upto * per > x);
+    const uint32_t past = __ballot_sync(~0u, upto > x);
     if (past == 0 && b0 + 32 < p.batch) {
-      x -= __shfl_sync(~0u, upto, 31) * per;
+      x -= __shfl_sync(~0u, upto, 31);
       continue;
     }
     const int src = past != 0 ? __ffs(past) - 1 : 31;
-    x -= __shfl_sync(~0u, upto - t, src) * per;
+    x -= __shfl_sync(~0u, upto - t * per, src);
     it.b = b0 + src;
     it.len = __shfl_sync(~0u, len, src);
     it.n = __shfl_sync(~0u, n, src);
     it.tiles = __shfl_sync(~0u, t, src);
-    const int hr = static_cast<int>(x / it.tiles);
-    tile = static_cast<int>(x - static_cast<int64_t>(hr) * it.tiles);
+    const int hr = x / it.tiles;
+    tile = x - hr * it.tiles;
     it.h = hr / p.row_blocks;
     it.rb = hr - it.h * p.row_blocks;
     return it;
   }
+}
+
+// `total` places dealt to n owners in contiguous shares, the first `r` of them one longer.
+struct Split {
+  int q, r;
+  __device__ __forceinline__ Split(int total, int n) : q(total / n), r(total - total / n * n) {}
+  __device__ __forceinline__ int start(int k) const { return k * q + min(k, r); }
+  __device__ __forceinline__ int owner(int x) const {
+    const int longer = r * (q + 1);
+    return x < longer ? x / (q + 1) : r + (x - longer) / q;
+  }
+};
+
+// Whether CTAs may split an item of so many tiles. Joining the parts takes a CTA about 4 us, whatever their size, and
+// not splitting leaves the shares uneven by half an item: 0.37 us for two tiles where all SMs read at HBM's rate.
+__device__ __forceinline__ bool splits(int tiles, int share) { return tiles > min(share, kWhole); }
+
+// Where CTA k's share begins: at the nearer end of an item that is not to be split.
+__device__ __forceinline__ int share_start(const Kv8AttnParams& p, const Split& split, int k, int ctas, int total) {
+  if (k == 0 || k == ctas) return k == 0 ? 0 : total;
+  int tile;
+  const int x = split.start(k);
+  const Item it = locate(p, x, tile);
+  if (splits(it.tiles, split.q)) return x;
+  return 2 * tile < it.tiles ? x - tile : x - tile + it.tiles;
 }
 
 __device__ __forceinline__ void next_item(const Kv8AttnParams& p, Item& it) {
@@ -180,16 +212,21 @@ struct Loader {
   Item it;
   int tile, t1;       // next tile of the item, end of this warp's tiles of it
   int blk0, te;       // cur covers the tiles up to te; its first page
-  int64_t x, x1;      // place in the list, end of the share
-  PageLane cur, nxt;  // this and the next batch of 32 pages
+  int x, x1;          // place in the list, end of the share
+  PageLane cur, nxt;  // this batch of 32 pages and, if `ahead`, the next
+  bool ahead;
 
   __device__ __forceinline__ int first_blk(const Kv8AttnParams& p, int t) const { return (t * kTile) >> p.c.block_log2; }
   __device__ __forceinline__ void take(const Kv8AttnParams& p, const PageLane& pages) {
-    const int lane = threadIdx.x & 31;
     cur = pages;
+    ahead = false;
     blk0 = first_blk(p, tile);
-    const int covered = ((blk0 + 32) << p.c.block_log2) >> kTileLog2;
-    te = min(t1, covered);
+    te = min(t1, ((blk0 + 32) << p.c.block_log2) >> kTileLog2);
+  }
+  __device__ __forceinline__ void look_ahead(const Kv8AttnParams& p) {
+    const int lane = threadIdx.x & 31;
+    if (ahead) return;
+    ahead = true;
     if (te < t1) {
       nxt = fetch_page(p, it, first_blk(p, te) + lane);
     } else if (x + (t1 - tile) < x1) {
@@ -198,12 +235,12 @@ struct Loader {
       nxt = fetch_page(p, n, lane);
     }
   }
-  __device__ __forceinline__ void start(const Kv8AttnParams& p, const Item& first, int t, int64_t begin, int64_t end) {
+  __device__ __forceinline__ void start(const Kv8AttnParams& p, const Item& first, int t, int begin, int end) {
     it = first;
     tile = t;
     x = begin;
     x1 = end;
-    t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
+    t1 = min(it.tiles, tile + (x1 - x));
     nxt = PageLane{-1, 0.0f, 1.0f};
     take(p, fetch_page(p, it, first_blk(p, tile) + (threadIdx.x & 31)));
   }
@@ -232,15 +269,14 @@ struct Loader {
     }
     ++tile;
     ++x;
-    if (x < x1) {
+    if (x < x1 && tile == te) {
+      look_ahead(p);
       if (tile == t1) {
         next_item(p, it);
         tile = 0;
-        t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), x1 - x));
-        take(p, nxt);
-      } else if (tile == te) {
-        take(p, nxt);
+        t1 = min(it.tiles, x1 - x);
       }
+      take(p, nxt);
     }
   }
 };
@@ -251,72 +287,81 @@ __device__ __forceinline__ uint16_t* out_row(const Kv8AttnParams& p, const Item&
   return static_cast<uint16_t*>(p.out) + it.b * p.o_sb + (it.h * p.group + gi) * p.o_sh + i * p.o_ss;
 }
 
-// Joins row rl of `count` partial results (`at(i)`: the i-th, in the order of the list): the maximum, the total and
-// this lane's kD / 32 channels.
+// Joins `count` partial results (`at(i)`: the i-th, in the order of the list) and writes the rows: to the output, or,
+// where `part` is given, to a partial result.
 template <int kD, bool kShared, class At>
-__device__ __forceinline__ void join_row(const At& at, int count, int part_rows, int rl, float& top, float& total,
-                                         float (&sum)[kD / 32]) {
-  const int lane = threadIdx.x & 31;
-  constexpr int kV = kD / 32;
-  top = -INFINITY;
-  total = 0.0f;
-#pragma unroll
-  for (int v = 0; v < kV; ++v) sum[v] = 0.0f;
-  for (int i0 = 0; i0 < count; i0 += 32) {
-    float mi = -INFINITY, li = 0.0f;
-    if (i0 + lane < count) {
-      const float* q = at(i0 + lane) + part_rows * kD + rl;
-      mi = kShared ? q[0] : __ldcg(q);
-      li = kShared ? q[part_rows] : __ldcg(q + part_rows);
+__device__ __forceinline__ void join(const Kv8AttnParams& p, const Item& it, const At& at, int count, int rows, float* part) {
+  constexpr int kV = kD / 32;                  // channels per lane
+  constexpr int kAtOnce = kShared ? kWarps : 8;  // parts in flight
+  const int lane = threadIdx.x & 31, r = lane & (kRows - 1), q = lane / kRows;
+  const auto load = [](const float* x) { return kShared ? *x : __ldcg(x); };
+  // maxima and totals: lane (r, q) looks at row r of every 4th part
+  float top = -INFINITY, total = 0.0f;
+  if (r < rows) {
+#pragma unroll 4
+    for (int i = q; i < count; i += 4) top = fmaxf(top, load(at(i) + p.part_rows * kD + r));
+  }
+  top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+  top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+  const float ref = top == -INFINITY ? 0.0f : top;  // a part that saw nothing has -inf, and factor 0
+  if (r < rows) {
+#pragma unroll 4
+    for (int i = q; i < count; i += 4) {
+      const float* src = at(i) + p.part_rows * kD + r;
+      total = fmaf(ex2(load(src) - ref), load(src + p.part_rows), total);
     }
-    float up = mi;
-    for (int o = 16; o > 0; o >>= 1) up = fmaxf(up, __shfl_xor_sync(~0u, up, o));
-    up = fmaxf(up, top);
-    const float again = top == -INFINITY ? 0.0f : ex2(top - up);
-    const float f = mi == -INFINITY ? 0.0f : ex2(mi - up);
-    top = up;
-    total = total * again + warp_sum(f * li);
+  }
+  total += __shfl_xor_sync(~0u, total, 8);
+  total += __shfl_xor_sync(~0u, total, 16);
+  if (part != nullptr && lane < rows) {
+    part[p.part_rows * kD + lane] = top;
+    part[p.part_rows * (kD + 1) + lane] = total;
+  }
+#pragma unroll 1
+  for (int rl = 0; rl < rows; ++rl) {
+    float sum[kV];
 #pragma unroll
-    for (int v = 0; v < kV; ++v) sum[v] *= again;
-    const int n = min(32, count - i0);
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const float fi = __shfl_sync(~0u, f, i);
-      const float* q = at(i0 + i) + rl * kD + lane * kV;
-      if constexpr (kV == 2) {
-        const float2 x = kShared ? *reinterpret_cast<const float2*>(q) : __ldcg(reinterpret_cast<const float2*>(q));
-        sum[0] = fmaf(fi, x.x, sum[0]), sum[1] = fmaf(fi, x.y, sum[1]);
-      } else {
-        const float4 x = kShared ? *reinterpret_cast<const float4*>(q) : __ldcg(reinterpret_cast<const float4*>(q));
-        sum[0] = fmaf(fi, x.x, sum[0]), sum[1] = fmaf(fi, x.y, sum[1]);
-        sum[2] = fmaf(fi, x.z, sum[2]), sum[3] = fmaf(fi, x.w, sum[3]);
+    for (int v = 0; v < kV; ++v) sum[v] = 0.0f;
+    const float peak = __shfl_sync(~0u, ref, rl), li = __shfl_sync(~0u, total, rl);
+#pragma unroll 1
+    for (int i0 = 0; i0 < count; i0 += kAtOnce) {
+      float x[kAtOnce][kV];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float* y = at(min(i0 + k, count - 1)) + rl * kD + lane * kV;
+        if constexpr (kV == 2) {
+          const float2 z = kShared ? *reinterpret_cast<const float2*>(y) : __ldcg(reinterpret_cast<const float2*>(y));
+          x[k][0] = z.x, x[k][1] = z.y;
+        } else {
+          const float4 z = kShared ? *reinterpret_cast<const float4*>(y) : __ldcg(reinterpret_cast<const float4*>(y));
+          x[k][0] = z.x, x[k][1] = z.y, x[k][2] = z.z, x[k][3] = z.w;
+        }
+      }
+      float f = 0.0f;  // of part i0 + lane
+      if (lane < kAtOnce && i0 + lane < count) f = ex2(load(at(i0 + lane) + p.part_rows * kD + rl) - peak);
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float fk = __shfl_sync(~0u, f, k);  // 0 past the last part
+#pragma unroll
+        for (int v = 0; v < kV; ++v) sum[v] = fmaf(fk, x[k][v], sum[v]);
       }
     }
-  }
-}
-
-// Writes a joined row: to the output, or to a partial result.
-template <int kD>
-__device__ __forceinline__ void put_row(const Kv8AttnParams& p, const Item& it, int rl, float* part, float top, float total,
-                                        const float (&sum)[kD / 32]) {
-  const int lane = threadIdx.x & 31;
-  constexpr int kV = kD / 32;
-  if (part != nullptr) {
-    float* dst = part + rl * kD + lane * kV;
-    if constexpr (kV == 2) *reinterpret_cast<float2*>(dst) = make_float2(sum[0], sum[1]);
-    else *reinterpret_cast<float4*>(dst) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-    if (lane == 0) part[p.part_rows * kD + rl] = top, part[p.part_rows * (kD + 1) + rl] = total;
-    return;
-  }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  uint32_t w[kV / 2];
+    if (part != nullptr) {
+      float* dst = part + rl * kD + lane * kV;
+      if constexpr (kV == 2) *reinterpret_cast<float2*>(dst) = make_float2(sum[0], sum[1]);
+      else *reinterpret_cast<float4*>(dst) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+      continue;
+    }
+    const float inv = li == 0.0f ? 0.0f : 1.0f / li;
+    uint32_t w[kV / 2];
 #pragma unroll
-  for (int v = 0; v < kV / 2; ++v)
-    w[v] = p.bf16 ? float2_to_pair<WBK_DT_BF16>(sum[2 * v] * inv, sum[2 * v + 1] * inv)
-                  : float2_to_pair<WBK_DT_F16>(sum[2 * v] * inv, sum[2 * v + 1] * inv);
-  uint16_t* dst = out_row(p, it, it.rb * kRows + rl) + lane * kV;
-  if constexpr (kV == 2) *reinterpret_cast<uint32_t*>(dst) = w[0];
-  else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    for (int v = 0; v < kV / 2; ++v)
+      w[v] = p.bf16 ? float2_to_pair<WBK_DT_BF16>(sum[2 * v] * inv, sum[2 * v + 1] * inv)
+                    : float2_to_pair<WBK_DT_F16>(sum[2 * v] * inv, sum[2 * v + 1] * inv);
+    uint16_t* dst = out_row(p, it, it.rb * kRows + rl) + lane * kV;
+    if constexpr (kV == 2) *reinterpret_cast<uint32_t*>(dst) = w[0];
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  }
 }
 
 template <int kFmt, int kD>
@@ -333,12 +378,15 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort_flag;
 
-  // this warp's share [x0, x1) of the list
-  const int64_t total = total_tiles(p);
-  const int64_t ctas = max(min(static_cast<int64_t>(gridDim.x), total * kTile / kMinShare), static_cast<int64_t>(1));
+  // this CTA's share [c0, c1) of the list, and of it this warp's, [x0, x1)
+  const int total = total_tiles(p), items = p.batch * p.c.kv_heads * p.row_blocks;
+  const int ctas = min(static_cast<int>(gridDim.x), max(items, total / least_share(total, items)));
   if (blockIdx.x >= ctas) return;
-  const int64_t warps = min(ctas * kWarps, total), me = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
-  const int64_t x0 = me * total / warps, x1 = (me + 1) * total / warps;
+  const Split split(total, ctas);
+  const int c0 = share_start(p, split, blockIdx.x, ctas, total), c1 = share_start(p, split, blockIdx.x + 1, ctas, total);
+  if (c0 == c1) return;
+  const int warps = min(kWarps, c1 - c0);
+  const Split own(c1 - c0, warps);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kWarps; ++i) {
       for (int j = 0; j < kMaxStages; ++j) mbar_init(&s.full[i][j], 1);
@@ -348,7 +396,8 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  if (me >= warps) return;
+  if (warp >= warps) return;
+  const int x0 = c0 + own.start(warp), x1 = c0 + own.start(warp + 1);
 
   int tile = 0;
   Item it = locate(p, x0, tile);
@@ -357,6 +406,7 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
   loader.start(p, it, tile, x0, x1);
   for (int i = 0; i < p.stages && loader.x < x1; ++i)
     loader.issue<kD>(p, &tmap_k, &tmap_v, ring + i * kTileBytes, s.factor[warp][i], &s.full[warp][i]);
+  if (loader.x < x1) loader.look_ahead(p);
 
   const int gid = lane >> 2, c = lane & 3;
   // Fragment addresses within a tile. Keys: 16 (or twice 16) bytes of token gid, channels c * kD / 4 .. Values: the
@@ -373,9 +423,9 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
 
   int st = 0;
   uint32_t phase = 0;
-  int64_t x = x0;
+  int x = x0;
   while (x < x1) {
-    const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
+    const int t1 = min(it.tiles, tile + (x1 - x));
     // ---- queries: row gid, channels c * kD / 4 ..
     uint32_t qf[kD / 8];
     float qfac = 1.0f;
@@ -436,8 +486,8 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
         // Give up: copies in flight land before the CTA ends (this tile's, and those of the stages after it).
         int dummy = 0;
         if (lane == 0) {
-          const int64_t left = loader.x - (x + (t - tile));
-          for (int64_t i = 0; i < left; ++i) {
+          const int left = loader.x - (x + (t - tile));
+          for (int i = 0; i < left; ++i) {
             mbar_wait_inl(&s.full[warp][st], phase, &dummy, kDrainNs, KSITE_DRAIN);
             if (++st == p.stages) st = 0, phase ^= 1u;
           }
@@ -543,8 +593,10 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
         }
       }
       __syncwarp();
-      if (loader.x < x1)
+      if (loader.x < x1) {
         loader.issue<kD>(p, &tmap_k, &tmap_v, ring + st * kTileBytes, s.factor[warp][st], &s.full[warp][st]);
+        if (loader.x < x1) loader.look_ahead(p);
+      }
       if (++st == p.stages) st = 0, phase ^= 1u;
     }
 
@@ -554,11 +606,10 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
       for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(~0u, l[e], d);
 
     // ---- the warps and CTAs that this item lies in
-    const int64_t begin = x - tile, end = begin + it.tiles;
-    const int64_t first = ((begin + 1) * warps - 1) / total, last = (end * warps - 1) / total;
-    const int cta = blockIdx.x, first_cta = static_cast<int>(first / kWarps), last_cta = static_cast<int>(last / kWarps);
-    const int w0 = first_cta == cta ? static_cast<int>(first % kWarps) : 0;
-    const int w1 = last_cta == cta ? static_cast<int>(last % kWarps) : kWarps - 1;
+    const int begin = x - tile, end = begin + it.tiles, cta = blockIdx.x;
+    const int w0 = own.owner(max(begin, c0) - c0), w1 = own.owner(min(end, c1) - 1 - c0);
+    const bool split_up = splits(it.tiles, split.q);
+    const int first_cta = split_up ? split.owner(begin) : cta, last_cta = split_up ? split.owner(end - 1) : cta;
     const bool alone = w0 == w1, here = first_cta == last_cta;
     const int rows = min(kRows, p.rows - it.rb * kRows);
     const int floats = part_floats(p.part_rows, kD);
@@ -598,12 +649,7 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
       holder = __shfl_sync(~0u, before, 0) == static_cast<uint32_t>(w1 - w0);
       if (holder) {
         __threadfence_block();
-        for (int rl = 0; rl < rows; ++rl) {
-          float top, tot, sum[kD / 32];
-          join_row<kD, true>([&](int i) { return static_cast<const float*>(slot_of(w0 + i)); }, w1 - w0 + 1, p.part_rows, rl,
-                             top, tot, sum);
-          put_row<kD>(p, it, rl, part, top, tot, sum);
-        }
+        join<kD, true>(p, it, [&](int i) { return static_cast<const float*>(slot_of(w0 + i)); }, w1 - w0 + 1, rows, part);
       }
     }
     if (holder && !here) {
@@ -617,12 +663,8 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
       if (__shfl_sync(~0u, before, 0) == static_cast<uint32_t>(last_cta - first_cta)) {
         __threadfence();
         const float* base = p.parts + static_cast<int64_t>(first_cta) * 2 * floats;
-        for (int rl = 0; rl < rows; ++rl) {
-          float top, tot, sum[kD / 32];
-          join_row<kD, false>([&](int i) { return base + (i == 0 ? 1 : 2 * static_cast<int64_t>(i)) * floats; },
-                              last_cta - first_cta + 1, p.part_rows, rl, top, tot, sum);
-          put_row<kD>(p, it, rl, nullptr, top, tot, sum);
-        }
+        join<kD, false>(p, it, [&](int i) { return base + (i == 0 ? 1 : 2 * static_cast<int64_t>(i)) * floats; },
+                        last_cta - first_cta + 1, rows, nullptr);
       }
     }
     x += t1 - tile;
@@ -796,8 +838,9 @@ int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_
   if (int e = kv8_make_tmap(&tk, k_cache, p, kTile, true)) return e;
   if (int e = kv8_make_tmap(&tv, v_cache, p, kTile, true)) return e;
   // the lengths are on the device: as many CTAs as the table could need, at most what the SMs hold
-  const int64_t most = batch * kv_heads * p.row_blocks * ((max_blocks * block + kTile - 1) / kTile);
-  const int grid = static_cast<int>(std::min(step_ctas(shape), std::max<int64_t>(most * kTile / kMinShare, 1)));
+  const int64_t items = batch * kv_heads * p.row_blocks, most = items * ((max_blocks * block + kTile - 1) / kTile);
+  if (most > INT_MAX) return fail(WBK_ERR_UNSUPPORTED, "wbk_attention_kv8: more than 2^31 tiles of 32 tokens in one call");
+  const int grid = static_cast<int>(std::min(step_ctas(shape), std::max<int64_t>(most / kMinShare, items)));
   if (fmt == WBK_FMT_E4M3)
     return head_dim == 64 ? launch_step<WBK_FMT_E4M3, 64>(tk, tv, p, grid, shape.smem, st)
                           : launch_step<WBK_FMT_E4M3, 128>(tk, tv, p, grid, shape.smem, st);
