@@ -191,18 +191,20 @@ __device__ __forceinline__ void next_item(const Kv8AttnParams& p, Item& it) {
   if (it.b < p.batch) it.tiles = tiles_of(p, it.b, it.len, it.n);
 }
 
-// A lane's page of a batch of 32 consecutive pages of an item, with its scales.
+// A lane's page of a batch of 32 consecutive pages of an item, and what its scales are to the softmax.
 struct PageLane {
-  int64_t page;
-  float ks, vs;
+  int page;               // -1: not there
+  float key, log2v, inv;  // factor of the scores, log2 of the value scale, its inverse
 };
 __device__ __forceinline__ PageLane fetch_page(const Kv8AttnParams& p, const Item& it, int blk) {
-  PageLane r{-1, 0.0f, 1.0f};
-  if ((static_cast<int64_t>(blk) << p.c.block_log2) < it.len) r.page = kv8_page(p.c, it.b, blk);
+  PageLane r{-1, 0.0f, 0.0f, 0.0f};
+  if ((static_cast<int64_t>(blk) << p.c.block_log2) < it.len) r.page = static_cast<int>(kv8_page(p.c, it.b, blk));
   if (r.page >= 0) {
-    const int64_t ph = r.page * p.c.kv_heads + it.h;
-    r.ks = p.k_scale[ph];
-    r.vs = p.v_scale[ph];
+    const int64_t ph = static_cast<int64_t>(r.page) * p.c.kv_heads + it.h;
+    const float vs = p.v_scale[ph];
+    r.key = p.k_scale[ph] * p.scale_log2;
+    r.log2v = kv8_log2(vs);
+    r.inv = 1.0f / vs;
   }
   return r;
 }
@@ -241,7 +243,7 @@ struct Loader {
     x = begin;
     x1 = end;
     t1 = min(it.tiles, tile + (x1 - x));
-    nxt = PageLane{-1, 0.0f, 1.0f};
+    nxt = PageLane{-1, 0.0f, 0.0f, 0.0f};
     take(p, fetch_page(p, it, first_blk(p, tile) + (threadIdx.x & 31)));
   }
   // Loads the next tile into a stage of the ring.
@@ -251,11 +253,11 @@ struct Loader {
     const int lane = threadIdx.x & 31;
     const int pos = tile * kTile + (lane & (kGroups - 1)) * 16;  // of a 16-token group
     const int from = ((pos >> p.c.block_log2) - blk0) & 31;
-    const int64_t page = __shfl_sync(~0u, cur.page, from);
-    const float ks = __shfl_sync(~0u, cur.ks, from), vs = __shfl_sync(~0u, cur.vs, from);
+    const int page = __shfl_sync(~0u, cur.page, from);
+    const float key = __shfl_sync(~0u, cur.key, from), log2v = __shfl_sync(~0u, cur.log2v, from);
+    const float inv = __shfl_sync(~0u, cur.inv, from);
     const bool there = page >= 0 && pos < it.len;
-    if (lane < kGroups)
-      factor[lane] = make_float4(ks * p.scale_log2, kv8_log2(vs), there ? 1.0f / vs : 0.0f, 0.0f);
+    if (lane < kGroups) factor[lane] = make_float4(key, log2v, there ? inv : 0.0f, 0.0f);
     // one box per page of the tile; the first 16-token group of it stands for it
     const int sub = min(p.c.block_log2, kTileLog2);
     const bool load = lane < kGroups && there && (lane & ((1 << (sub - 4)) - 1)) == 0;
@@ -264,8 +266,8 @@ struct Loader {
     __syncwarp();
     if (load) {
       const int y = (it.h << p.c.block_log2) + (pos & (p.c.block - 1));
-      tma_load_3d(tk, full, stage + lane * 16 * kD, 0, y, static_cast<int>(page));
-      tma_load_3d(tv, full, stage + (kTile + lane * 16) * kD, 0, y, static_cast<int>(page));
+      tma_load_3d(tk, full, stage + lane * 16 * kD, 0, y, page);
+      tma_load_3d(tv, full, stage + (kTile + lane * 16) * kD, 0, y, page);
     }
     ++tile;
     ++x;
@@ -482,13 +484,13 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
     for (int t = tile; t < t1; ++t) {
-      if (!__all_sync(~0u, mbar_wait_inl(&s.full[warp][st], phase, abort_flag, p.timeout_ns, KSITE_TILE))) {
+      if (!__all_sync(~0u, mbar_wait(&s.full[warp][st], phase, abort_flag, p.timeout_ns, KSITE_TILE))) {
         // Give up: copies in flight land before the CTA ends (this tile's, and those of the stages after it).
         int dummy = 0;
         if (lane == 0) {
           const int left = loader.x - (x + (t - tile));
           for (int i = 0; i < left; ++i) {
-            mbar_wait_inl(&s.full[warp][st], phase, &dummy, kDrainNs, KSITE_DRAIN);
+            mbar_wait(&s.full[warp][st], phase, &dummy, kDrainNs, KSITE_DRAIN);
             if (++st == p.stages) st = 0, phase ^= 1u;
           }
         }
