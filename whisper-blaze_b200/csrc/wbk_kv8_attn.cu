@@ -191,20 +191,25 @@ __device__ __forceinline__ void next_item(const Kv8AttnParams& p, Item& it) {
   if (it.b < p.batch) it.tiles = tiles_of(p, it.b, it.len, it.n);
 }
 
-// A lane's page of a batch of 32 consecutive pages of an item, and what its scales are to the softmax.
+// A lane's page of a batch of 32 consecutive pages of an item, with its scales; `factors` turns these into what they
+// are to the softmax. Apart, so that the page's codes can be asked for before its scales have come.
 struct PageLane {
-  int page;               // -1: not there
-  float key, log2v, inv;  // factor of the scores, log2 of the value scale, its inverse
+  int page;           // -1: not there
+  float ks, vs;       // scales
+  float log2v, inv;   // after factors(): log2 of the value scale, its inverse; ks is the factor of the scores
+  __device__ __forceinline__ void factors(const Kv8AttnParams& p) {
+    ks *= p.scale_log2;
+    log2v = kv8_log2(vs);
+    inv = 1.0f / vs;
+  }
 };
 __device__ __forceinline__ PageLane fetch_page(const Kv8AttnParams& p, const Item& it, int blk) {
-  PageLane r{-1, 0.0f, 0.0f, 0.0f};
+  PageLane r{-1, 0.0f, 1.0f, 0.0f, 0.0f};
   if ((static_cast<int64_t>(blk) << p.c.block_log2) < it.len) r.page = static_cast<int>(kv8_page(p.c, it.b, blk));
   if (r.page >= 0) {
     const int64_t ph = static_cast<int64_t>(r.page) * p.c.kv_heads + it.h;
-    const float vs = p.v_scale[ph];
-    r.key = p.k_scale[ph] * p.scale_log2;
-    r.log2v = kv8_log2(vs);
-    r.inv = 1.0f / vs;
+    r.ks = p.k_scale[ph];
+    r.vs = p.v_scale[ph];
   }
   return r;
 }
@@ -243,21 +248,24 @@ struct Loader {
     x = begin;
     x1 = end;
     t1 = min(it.tiles, tile + (x1 - x));
-    nxt = PageLane{-1, 0.0f, 0.0f, 0.0f};
+    nxt = PageLane{-1, 0.0f, 1.0f, 0.0f, 0.0f};
     take(p, fetch_page(p, it, first_blk(p, tile) + (threadIdx.x & 31)));
   }
-  // Loads the next tile into a stage of the ring.
+  // The 16-token group of this lane (of kGroups) in a tile of the item: its first position, the lane of cur that has its
+  // page, and whether it is there.
+  __device__ __forceinline__ bool group_of(const Kv8AttnParams& p, int t, int& pos, int& page, int& from) const {
+    pos = t * kTile + (threadIdx.x & (kGroups - 1)) * 16;
+    from = ((pos >> p.c.block_log2) - blk0) & 31;
+    page = __shfl_sync(~0u, cur.page, from);
+    return page >= 0 && pos < it.len;
+  }
+  // Asks for the codes of tile t.
   template <int kD>
-  __device__ __forceinline__ void issue(const Kv8AttnParams& p, const CUtensorMap* tk, const CUtensorMap* tv, uint8_t* stage,
-                                        float4* factor, uint64_t* full) {
+  __device__ __forceinline__ void codes(const Kv8AttnParams& p, int t, const CUtensorMap* tk, const CUtensorMap* tv,
+                                        uint8_t* stage, uint64_t* full) const {
     const int lane = threadIdx.x & 31;
-    const int pos = tile * kTile + (lane & (kGroups - 1)) * 16;  // of a 16-token group
-    const int from = ((pos >> p.c.block_log2) - blk0) & 31;
-    const int page = __shfl_sync(~0u, cur.page, from);
-    const float key = __shfl_sync(~0u, cur.key, from), log2v = __shfl_sync(~0u, cur.log2v, from);
-    const float inv = __shfl_sync(~0u, cur.inv, from);
-    const bool there = page >= 0 && pos < it.len;
-    if (lane < kGroups) factor[lane] = make_float4(key, log2v, there ? inv : 0.0f, 0.0f);
+    int pos, page, from;
+    const bool there = group_of(p, t, pos, page, from);
     // one box per page of the tile; the first 16-token group of it stands for it
     const int sub = min(p.c.block_log2, kTileLog2);
     const bool load = lane < kGroups && there && (lane & ((1 << (sub - 4)) - 1)) == 0;
@@ -269,8 +277,19 @@ struct Loader {
       tma_load_3d(tk, full, stage + lane * 16 * kD, 0, y, page);
       tma_load_3d(tv, full, stage + (kTile + lane * 16) * kD, 0, y, page);
     }
-    ++tile;
-    ++x;
+  }
+  // Writes what the softmax needs for tile t.
+  __device__ __forceinline__ void factors(const Kv8AttnParams& p, int t, float4* factor) const {
+    int pos, page, from;
+    const bool there = group_of(p, t, pos, page, from);
+    const float key = __shfl_sync(~0u, cur.ks, from), log2v = __shfl_sync(~0u, cur.log2v, from);
+    const float inv = __shfl_sync(~0u, cur.inv, from);
+    if ((threadIdx.x & 31) < kGroups) factor[threadIdx.x & 31] = make_float4(key, log2v, there ? inv : 0.0f, 0.0f);
+  }
+  // n tiles on, none of them beyond te.
+  __device__ __forceinline__ void advance(const Kv8AttnParams& p, int n) {
+    tile += n;
+    x += n;
     if (x < x1 && tile == te) {
       look_ahead(p);
       if (tile == t1) {
@@ -278,6 +297,7 @@ struct Loader {
         tile = 0;
         t1 = min(it.tiles, x1 - x);
       }
+      nxt.factors(p);
       take(p, nxt);
     }
   }
@@ -380,6 +400,10 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort_flag;
 
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmap_k);
+    prefetch_tmap(&tmap_v);
+  }
   // this CTA's share [c0, c1) of the list, and of it this warp's, [x0, x1)
   const int total = total_tiles(p), items = p.batch * p.c.kv_heads * p.row_blocks;
   const int ctas = min(static_cast<int>(gridDim.x), max(items, total / least_share(total, items)));
@@ -406,9 +430,27 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
   uint8_t* ring = rings + warp * p.stages * kTileBytes;
   Loader loader;
   loader.start(p, it, tile, x0, x1);
-  for (int i = 0; i < p.stages && loader.x < x1; ++i)
-    loader.issue<kD>(p, &tmap_k, &tmap_v, ring + i * kTileBytes, s.factor[warp][i], &s.full[warp][i]);
-  if (loader.x < x1) loader.look_ahead(p);
+  {
+    // the first page batch's codes as soon as its pages are known, and then their scales; the queries meanwhile
+    const int n = min(p.stages, loader.te - loader.tile);
+    for (int i = 0; i < n; ++i) loader.codes<kD>(p, tile + i, &tmap_k, &tmap_v, ring + i * kTileBytes, &s.full[warp][i]);
+    const int r = it.rb * kRows + (lane >> 2);
+    if (r < p.rows) {
+      const int gi = r / p.queries;
+      const uint16_t* q = static_cast<const uint16_t*>(p.q) + it.b * p.q_sb + (it.h * p.group + gi) * p.q_sh + (r - gi * p.queries) * p.q_ss;
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(q + (lane & 3) * (kD / 4)));
+    }
+    loader.cur.factors(p);
+    for (int i = 0; i < n; ++i) loader.factors(p, tile + i, s.factor[warp][i]);
+    loader.advance(p, n);
+    for (int i = n; i < p.stages && loader.x < x1; ++i) {
+      loader.codes<kD>(p, loader.tile, &tmap_k, &tmap_v, ring + i * kTileBytes, &s.full[warp][i]);
+      loader.factors(p, loader.tile, s.factor[warp][i]);
+      loader.advance(p, 1);
+    }
+    if (loader.x < x1) loader.look_ahead(p);
+    __syncwarp();
+  }
 
   const int gid = lane >> 2, c = lane & 3;
   // Fragment addresses within a tile. Keys: 16 (or twice 16) bytes of token gid, channels c * kD / 4 .. Values: the
@@ -596,8 +638,11 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
       }
       __syncwarp();
       if (loader.x < x1) {
-        loader.issue<kD>(p, &tmap_k, &tmap_v, ring + st * kTileBytes, s.factor[warp][st], &s.full[warp][st]);
+        loader.codes<kD>(p, loader.tile, &tmap_k, &tmap_v, ring + st * kTileBytes, &s.full[warp][st]);
+        loader.factors(p, loader.tile, s.factor[warp][st]);
+        loader.advance(p, 1);
         if (loader.x < x1) loader.look_ahead(p);
+        __syncwarp();
       }
       if (++st == p.stages) st = 0, phase ^= 1u;
     }
