@@ -57,6 +57,12 @@ int64_t kv8_ticket_bytes() {
 namespace {
 
 // ------------------------------------------------------------------ append
+//
+// What bounds it: each new value is read once (2 bytes) and written once (1 byte), so
+// HBM. A page and head is one CTA's work, held in registers between the maximum and
+// the codes. The chain length -> page -> values -> maximum -> codes is all latency, so
+// where there are enough CTAs to fill the SMs one takes several heads of its page, with
+// the next head's values on their way meanwhile.
 
 struct AppendSide {
   const void* x;         // new keys or values, [batch, kv_heads, tokens, head_dim] view
@@ -71,17 +77,31 @@ struct AppendParams {
   const int32_t* lens;
   const int32_t* fresh;  // new tokens of each sequence, or NULL: all
   int tokens;
+  int heads_per_cta;
 };
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendVecs = 4;  // 16-byte vectors per thread, at most (8 KB per 128 threads)
 
-// One CTA per touched page of one KV head, for the keys or the values
-// (blockIdx.y = head, blockIdx.z = batch * 2 + side).
-template <int kFmt, int kDtype, int kD>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const AppendParams p) {
+// Larger of two packed pairs, lane by lane; NaN where both are.
+template <int kDtype>
+__device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (kDtype == WBK_DT_F16) asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <int kDtype>
+__device__ __forceinline__ float half_word_value(uint32_t bits) {
+  return pair_to_float2<kDtype>(bits & 0xFFFFu).x;
+}
+
+// One CTA per touched page and heads_per_cta KV heads, for the keys or the values
+// (blockIdx.y: heads, blockIdx.z: batch * 2 + side); kThreads threads hold a page of kThreads * kVec 16-byte vectors.
+template <int kFmt, int kDtype, int kD, int kThreads, int kVec>
+__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams p) {
+  constexpr int kWarps = kThreads / 32;
   const int b = blockIdx.z >> 1;
   const AppendSide& s = p.side[blockIdx.z & 1];
-  const int h = blockIdx.y;
   const int len = kv8_len(p.lens, b, p.c);
   const int n = p.fresh != nullptr ? min(max(p.fresh[b], 0), p.tokens) : p.tokens;
   const int block = p.c.block;
@@ -92,61 +112,113 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   if (slot1 <= slot0) return;
   const int64_t page = kv8_page(p.c, b, blk);
   if (page < 0) return;
-  const int64_t ph = page * p.c.kv_heads + h;
-  uint8_t* codes = s.cache + ph * block * kD;
-  const uint16_t* x = static_cast<const uint16_t*>(s.x) + b * s.sb + h * s.sh + static_cast<int64_t>(start + slot0 - len) * s.ss;
-
-  constexpr int kVec = kD / 8;  // 16-byte vectors per token
-  const int vecs = (slot1 - slot0) * kVec;
-  float amax = 0.0f;
-  for (int i = threadIdx.x; i < vecs; i += kAppendThreads) {
-    const uint4 v = *reinterpret_cast<const uint4*>(x + (i / kVec) * s.ss + (i % kVec) * 8);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = pair_to_float2<kDtype>(w[j]);
-      if (isfinite(f.x)) amax = fmaxf(amax, fabsf(f.x));
-      if (isfinite(f.y)) amax = fmaxf(amax, fabsf(f.y));
+  const int h0 = blockIdx.y * p.heads_per_cta, h1 = min(h0 + p.heads_per_cta, p.c.kv_heads);
+  constexpr int kPer = kD / 8;  // vectors per token
+  const int vecs = (slot1 - slot0) * kPer;
+  const uint16_t* x = static_cast<const uint16_t*>(s.x) + b * s.sb + static_cast<int64_t>(start + slot0 - len + threadIdx.x / kPer) * s.ss +
+                      (threadIdx.x % kPer) * 8;
+  const int64_t step = static_cast<int64_t>(kThreads / kPer) * s.ss;  // a thread's vectors lie in the same column
+  auto load = [&](uint4 (&v)[kVec], int h) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (static_cast<int>(threadIdx.x) + i * kThreads < vecs) v[i] = ld_stream16(x + h * s.sh + i * step);
     }
-  }
-  __shared__ uint32_t red[kAppendThreads / 32];
-  const uint32_t wmax = warp_max_u32(__float_as_uint(amax));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = wmax;
-  __syncthreads();
-  for (int i = 0; i < kAppendThreads / 32; ++i) amax = fmaxf(amax, __uint_as_float(red[i]));
-  float scale = kv8_pow2(kv8_scale_exp<kFmt>(amax));
-  if (slot0 > 0) {
-    const float old = s.scale[ph];
-    if (scale > old) {
-      const float shift = old / scale;
-      for (int i = threadIdx.x; i < slot0 * kD / 2; i += kAppendThreads) {
-        uint16_t* at = reinterpret_cast<uint16_t*>(codes) + i;
-        const float2 f = __half22float2(kv8_half2<kFmt>(*at));
-        *at = static_cast<uint16_t>(kv8_codes2<kFmt>(f.x * shift, f.y * shift));
+  };
+  __shared__ uint32_t red[2][kWarps];
+  uint4 v[kVec];
+  load(v, h0);
+  for (int h = h0; h < h1; ++h) {
+    const int64_t ph = page * p.c.kv_heads + h;
+    const float old = slot0 > 0 ? s.scale[ph] : 0.0f;
+    // ---- largest |x|: as 16-bit patterns, whose order is that of the values; NaN is passed over
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      top = pair_max<kDtype>(top, v[i].x & 0x7FFF7FFFu);
+      top = pair_max<kDtype>(top, v[i].y & 0x7FFF7FFFu);
+      top = pair_max<kDtype>(top, v[i].z & 0x7FFF7FFFu);
+      top = pair_max<kDtype>(top, v[i].w & 0x7FFF7FFFu);
+    }
+    const int turn = (h - h0) & 1;
+    top = warp_max_u32(max(top & 0xFFFFu, top >> 16));
+    if ((threadIdx.x & 31) == 0) red[turn][threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) top = max(top, red[turn][i]);
+    float amax = half_word_value<kDtype>(top);
+    if (isinf(amax)) {  // infinities do not count: again, without them (the same way in all threads)
+      amax = 0.0f;
+      for (int i = 0; i < kVec; ++i) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = pair_to_float2<kDtype>(w[j]);
+          if (isfinite(f.x)) amax = fmaxf(amax, fabsf(f.x));
+          if (isfinite(f.y)) amax = fmaxf(amax, fabsf(f.y));
+        }
       }
-    } else {
-      scale = old;
+      const uint32_t bits = warp_max_u32(__float_as_uint(amax));
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) red[turn][threadIdx.x >> 5] = bits;
+      __syncthreads();
+      for (int i = 0; i < kWarps; ++i) amax = fmaxf(amax, __uint_as_float(red[turn][i]));
     }
-  }
-  const float inv = 1.0f / scale;
-  for (int i = threadIdx.x; i < vecs; i += kAppendThreads) {
-    const uint4 v = *reinterpret_cast<const uint4*>(x + (i / kVec) * s.ss + (i % kVec) * 8);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t q[4];
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = pair_to_float2<kDtype>(w[j]);
-      q[j] = kv8_codes2<kFmt>(f.x * inv, f.y * inv);
+    // ---- the page's scale; older codes follow it where it grows
+    uint8_t* codes = s.cache + ph * block * kD;
+    int e = kv8_scale_exp<kFmt>(amax);
+    float scale = kv8_pow2(e), inv = kv8_pow2(-e);
+    if (slot0 > 0) {
+      if (scale > old) {
+        const float shift = old * inv;
+        for (int i = threadIdx.x; i < slot0 * kD / 4; i += kThreads) {
+          uint32_t* at = reinterpret_cast<uint32_t*>(codes) + i;
+          const uint32_t w = *at;
+          const float2 f = __half22float2(kv8_half2<kFmt>(w)), g = __half22float2(kv8_half2<kFmt>(w >> 16));
+          *at = kv8_codes2<kFmt>(f.x * shift, f.y * shift) | (kv8_codes2<kFmt>(g.x * shift, g.y * shift) << 16);
+        }
+      } else {
+        scale = old;
+        inv = 1.0f / old;
+      }
     }
-    *reinterpret_cast<uint2*>(codes + slot0 * kD + i * 8) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+    // ---- codes; the next head's values take the registers as they become free
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int id = threadIdx.x + i * kThreads;
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      uint32_t q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = f2_mul(pair_to_float2<kDtype>(w[j]), make_float2(inv, inv));
+        q[j] = kv8_codes2<kFmt>(f.x, f.y);
+      }
+      if (id < vecs) {
+        *reinterpret_cast<uint2*>(codes + slot0 * kD + id * 8) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+        if (h + 1 < h1) v[i] = ld_stream16(x + (h + 1) * s.sh + i * step);
+      }
+    }
+    // with old tokens every thread has read the old scale: the sums' barrier lies in between
+    if (threadIdx.x == 0) s.scale[ph] = scale;
   }
-  __syncthreads();  // every thread has read the old scale
-  if (threadIdx.x == 0) s.scale[ph] = scale;
 }
 
-template <int kFmt, int kDtype>
-int launch_append(const AppendParams& p, int head_dim, dim3 grid, cudaStream_t stream) {
-  if (head_dim == 64) kv8_append_kernel<kFmt, kDtype, 64><<<grid, kAppendThreads, 0, stream>>>(p);
-  else kv8_append_kernel<kFmt, kDtype, 128><<<grid, kAppendThreads, 0, stream>>>(p);
+template <int kFmt, int kDtype, int kD>
+int launch_append(const AppendParams& p, dim3 grid, cudaStream_t stream) {
+  switch (p.c.block * kD / 8 / 128) {
+    case 1: kv8_append_kernel<kFmt, kDtype, kD, 128, 1><<<grid, 128, 0, stream>>>(p); break;
+    case 2: kv8_append_kernel<kFmt, kDtype, kD, 128, 2><<<grid, 128, 0, stream>>>(p); break;
+    case 4: kv8_append_kernel<kFmt, kDtype, kD, 128, kAppendVecs><<<grid, 128, 0, stream>>>(p); break;
+    case 8: kv8_append_kernel<kFmt, kDtype, kD, 256, kAppendVecs><<<grid, 256, 0, stream>>>(p); break;
+    default: kv8_append_kernel<kFmt, kDtype, kD, 256, 8><<<grid, 256, 0, stream>>>(p); break;
+  }
   return cuda_check(cudaGetLastError(), "kv8 append launch");
+}
+
+template <int kFmt>
+int dispatch_append(const AppendParams& p, int dtype, int head_dim, dim3 grid, cudaStream_t stream) {
+  if (dtype == WBK_DT_F16)
+    return head_dim == 64 ? launch_append<kFmt, WBK_DT_F16, 64>(p, grid, stream) : launch_append<kFmt, WBK_DT_F16, 128>(p, grid, stream);
+  return head_dim == 64 ? launch_append<kFmt, WBK_DT_BF16, 64>(p, grid, stream) : launch_append<kFmt, WBK_DT_BF16, 128>(p, grid, stream);
 }
 
 }  // namespace
@@ -190,14 +262,14 @@ int wbk_kv8_append(const void* k, const void* v, int dtype, int64_t batch, int64
   p.tokens = static_cast<int>(tokens);
   // a run of `tokens` positions touches at most this many pages
   const int64_t touched = std::min<int64_t>((tokens + block - 2) / block + 1, max_blocks);
-  const dim3 grid(static_cast<unsigned>(touched), static_cast<unsigned>(kv_heads), static_cast<unsigned>(batch * 2));
+  // several heads per CTA once that still leaves the SMs two rounds of CTAs
+  const int64_t units = touched * kv_heads * batch * 2, room = static_cast<int64_t>(sm_count() > 0 ? sm_count() : 148) * 16 * 2;
+  p.heads_per_cta = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kv_heads, units / room)));
+  const dim3 grid(static_cast<unsigned>(touched), static_cast<unsigned>((kv_heads + p.heads_per_cta - 1) / p.heads_per_cta),
+                  static_cast<unsigned>(batch * 2));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int d = static_cast<int>(head_dim);
-  if (fmt == WBK_FMT_E4M3)
-    return dtype == WBK_DT_F16 ? launch_append<WBK_FMT_E4M3, WBK_DT_F16>(p, d, grid, st)
-                               : launch_append<WBK_FMT_E4M3, WBK_DT_BF16>(p, d, grid, st);
-  return dtype == WBK_DT_F16 ? launch_append<WBK_FMT_E5M2, WBK_DT_F16>(p, d, grid, st)
-                             : launch_append<WBK_FMT_E5M2, WBK_DT_BF16>(p, d, grid, st);
+  return fmt == WBK_FMT_E4M3 ? dispatch_append<WBK_FMT_E4M3>(p, dtype, static_cast<int>(head_dim), grid, st)
+                             : dispatch_append<WBK_FMT_E5M2>(p, dtype, static_cast<int>(head_dim), grid, st);
 }
 
 }  // extern "C"
