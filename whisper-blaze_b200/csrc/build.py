@@ -3,7 +3,8 @@
     python whisper-blaze_b200/csrc/build.py [--force] [--verbose]
 
 Objects go to whisper-blaze_b200/_build/, the library to
-whisper-blaze_b200/lib/libwbk.so. The CUDA runtime is linked statically so the
+whisper-blaze_b200/lib/libwbk.so, the Python extension with the short way to the
+decoder-step calls to whisper-blaze_b200/lib/_wbk_calls.so. The CUDA runtime is linked statically so the
 library does not depend on which libcudart the host process loaded first.
 The quantiser unit is compiled with --use_fast_math, the flag set of the
 reference's own quantiser build (setup.py:41-54); its scale division is the
@@ -13,10 +14,12 @@ defaults, like every other unit) shares.
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -24,6 +27,7 @@ PKG = os.path.dirname(HERE)
 REPO = os.path.dirname(PKG)
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "lib", "libwbk.so")
+CALLS = os.path.join(PKG, "lib", "_wbk_calls.so")
 INCLUDE = os.path.join(REPO, "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -75,11 +79,30 @@ def _compile(src: str, flags: list[str], force: bool, verbose: bool) -> tuple[st
     return obj, (r.stdout + r.stderr) if verbose else ""
 
 
+def _compile_calls(force: bool) -> None:
+    """The extension module of wbk_calls.cpp, against this interpreter and the torch it imports."""
+    src = os.path.join(HERE, "wbk_calls.cpp")
+    if not force and not _stale(CALLS, [src, os.path.join(INCLUDE, "wbk.h"), __file__]):
+        return
+    root = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    inc = [INCLUDE, sysconfig.get_paths()["include"], os.path.join(root, "include"),
+           os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include")]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=1"]
+    cmd += [f"-I{d}" for d in inc] + [src, "-o", CALLS, f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch_cpu",
+                                      "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(os.path.dirname(LIB), exist_ok=True)
-    with ThreadPoolExecutor(max_workers=len(UNITS)) as ex:
+    with ThreadPoolExecutor(max_workers=len(UNITS) + 1) as ex:
+        calls = ex.submit(_compile_calls, force)
         results = list(ex.map(lambda kv: _compile(kv[0], kv[1], force, verbose), UNITS.items()))
+        calls.result()
     objs = [o for o, _ in results]
     for _, log in results:
         if log:

@@ -6,6 +6,8 @@ there is no fallback: if it is missing, every op raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import re
 import threading
@@ -14,6 +16,7 @@ import torch
 
 _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG_ROOT, "lib", "libwbk.so")
+CALLS_PATH = os.path.join(_PKG_ROOT, "lib", "_wbk_calls.so")
 HEADER_PATH = os.path.join(os.path.dirname(_PKG_ROOT), "include", "wbk.h")
 
 WBK_OK = 0
@@ -100,6 +103,21 @@ def lib() -> ctypes.CDLL:
                     fn.argtypes = args
                 _lib = L
     return _lib
+
+
+_CALLS = ("wbk_kv8_append", "wbk_attention_kv8", "wbk_attention_kv8_ws_bytes", "wbk_sample")
+
+
+def calls():
+    """The extension module with the short way to the decoder-step calls (csrc/wbk_calls.cpp), bound to the loaded
+    libwbk.so; None where it is not built."""
+    if not os.path.exists(CALLS_PATH):
+        return None
+    loader = importlib.machinery.ExtensionFileLoader("_wbk_calls", CALLS_PATH)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_wbk_calls", loader))
+    loader.exec_module(module)
+    module.bind(*(ctypes.cast(getattr(lib(), name), _vp).value for name in _CALLS))
+    return module
 
 
 def header_symbols() -> list[str]:

@@ -294,7 +294,7 @@ def _scale_arg(scale: Scale, name: str, device) -> tuple[float, Optional[int]]:
 
 
 _SPLITK_WS: dict = {}
-_KV8_WS: dict = {}
+_KV8_WS: list = []  # by device index
 
 
 @_lib.on_device_timeout
@@ -302,8 +302,8 @@ def _zero_shared_workspaces(device_index: int) -> None:
     """After a device-side timeout a kernel may have left the sync words or split-K tickets of
     the device's shared workspace non-zero; zero it again so the next call starts clean.
     (Workspaces passed by the caller are the caller's to zero, as wbk.h states.)"""
-    for shared in (_SPLITK_WS, _KV8_WS):
-        ws = shared.get(torch.device("cuda", device_index))
+    shared = _KV8_WS[device_index] if device_index < len(_KV8_WS) else None
+    for ws in (_SPLITK_WS.get(torch.device("cuda", device_index)), shared):
         if ws is not None:
             ws.zero_()
 
@@ -477,8 +477,18 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[t
 
 # ------------------------------------------------------ 8-bit key/value cache
 
-# The calls below are made once per layer and token, so what they do on the host is kept short: device indexes
-# instead of device objects, the raw stream, no device guard where the device is current already.
+# The calls below are made once per layer and token, so what they do on the host is kept short. Each first offers its
+# arguments to the extension module of csrc/wbk_calls.cpp, which makes the call if they are all as the entry point needs
+# them; what it hands back (None) goes through the checks here, which say what is wrong, or make the call.
+
+_SHORT: list = []  # [the module, or None]
+
+
+def _short():
+    if not _SHORT:
+        _SHORT.append(_lib.calls())
+    return _SHORT[0]
+
 
 _DT16 = {torch.float16: DT_F16, torch.bfloat16: DT_BF16}
 _F8_DTYPE = {FMT_E4M3: torch.float8_e4m3fn, FMT_E5M2: torch.float8_e5m2}
@@ -572,12 +582,14 @@ def _kv8_ws_bytes(index: int, batch: int, heads: int, kv_heads: int, queries: in
         return int(lib().wbk_attention_kv8_ws_bytes(batch, heads, kv_heads, queries, head_dim))
 
 
-def kv8_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """The per-device workspace of attention_kv8 (zero-filled once, grown on demand), shared by its calls on the
-    device: calls that may run at the same time need workspaces of their own."""
-    ws = _KV8_WS.get(device)
+def kv8_workspace(index: int, nbytes: int) -> torch.Tensor:
+    """The workspace of attention_kv8 on CUDA device `index` (zero-filled once, grown on demand), shared by its calls
+    there: calls that may run at the same time need workspaces of their own."""
+    while len(_KV8_WS) <= index:
+        _KV8_WS.append(None)
+    ws = _KV8_WS[index]
     if ws is None or ws.numel() < nbytes:
-        ws = _KV8_WS[device] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        ws = _KV8_WS[index] = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
     return ws
 
 
@@ -596,6 +608,13 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
     one, the page's older codes are rescaled. Tokens past the table, or whose page
     is outside the pool, are not stored. seq_lens is not changed.
     """
+    short = _short()
+    if short is not None:
+        status = short.kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, new_lens, fmt)
+        if status is not None:
+            check(status, "kv8_append")
+            LAUNCHES[0] += 1
+            return
     dt, index, shape, ks3 = _require_bhsd(k, "k")
     vdt, vindex, vshape, vs3 = _require_bhsd(v, "v")
     if vdt != dt or vshape != shape or vindex != index:
@@ -630,6 +649,15 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     shared one, so such calls must not run concurrently on different streams
     without a workspace of their own.
     """
+    short = _short()
+    if short is not None:
+        got = short.attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, q_lens, causal, scale, fmt,
+                                  out, workspace, _KV8_WS)
+        if got is not None:
+            if type(got) is int:
+                check(got, "attention_kv8")
+            LAUNCHES[0] += 1
+            return got
     dt, index, shape, qs3 = _require_bhsd(q, "q")
     B, H, T, D = shape
     f, pages, kv_heads, block, width, ts = _require_cache(index, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
@@ -648,7 +676,7 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
             raise RuntimeError(f"out must be a {q.dtype} view of shape {tuple(shape)} on {q.device}")
     need = _kv8_ws_bytes(index, B, H, kv_heads, T, D)
     if workspace is None:
-        workspace = kv8_workspace(q.device, need)
+        workspace = kv8_workspace(index, need)
     else:
         _require_on(index, workspace, "workspace")
     _launch(lib().wbk_attention_kv8,
@@ -702,6 +730,14 @@ def sample(logits: torch.Tensor, noise: torch.Tensor, temperature=1.0, top_k=0, 
     under the unfiltered softmax of the logits as given. A row with no logit above
     -inf gives token -1 and logprob -inf.
     """
+    short = _short()
+    if short is not None and tokens_out is None and logprobs_out is None:
+        got = short.sample(logits, noise, temperature, top_k, top_p, min_p)
+        if got is not None:
+            if type(got) is int:
+                check(got, "sample")
+            LAUNCHES[0] += 1
+            return got
     index = logits.get_device()
     if index < 0:
         require_cuda(logits, "logits")
