@@ -35,8 +35,41 @@ int kv8_prompt_read_device_error(uint32_t* v, bool clear);
 // (0 = not set: the WBK_WAIT_TIMEOUT_MS / 4 s default applies).
 uint64_t wait_timeout_override_ns();
 
+// Whether the decoder-step kernels are launched with programmatic stream serialization (WBK_PDL, default on): such a
+// kernel may be set up while the one before it in the stream still runs, and calls griddep_wait() before it touches
+// memory.
+bool programmatic_launch();
+
 inline bool aligned(const void* p, size_t a) {
   return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
+}
+
+// Launch of `kernel` with that attribute, and with clusters of `cluster` CTAs where it is above 1.
+template <class... Params, class... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+                         unsigned cluster, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (programmatic_launch()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // ---------------------------------------------------------------- device side

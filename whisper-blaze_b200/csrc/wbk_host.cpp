@@ -2,6 +2,8 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
+#include <cstring>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -38,6 +40,14 @@ int current_device() {
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess) return -1;
   return dev;
+}
+
+bool programmatic_launch() {
+  static const bool on = [] {
+    const char* e = std::getenv("WBK_PDL");
+    return e == nullptr || std::strcmp(e, "0") != 0;
+  }();
+  return on;
 }
 
 int sm_count() {

@@ -100,6 +100,8 @@ __device__ __forceinline__ float half_word_value(uint32_t bits) {
 template <int kFmt, int kDtype, int kD, int kThreads, int kVec>
 __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams p) {
   constexpr int kWarps = kThreads / 32;
+  griddep_launch_dependents();
+  griddep_wait();
   const int b = blockIdx.z >> 1;
   const AppendSide& s = p.side[blockIdx.z & 1];
   const int len = kv8_len(p.lens, b, p.c);
@@ -204,14 +206,15 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
 
 template <int kFmt, int kDtype, int kD>
 int launch_append(const AppendParams& p, dim3 grid, cudaStream_t stream) {
+  cudaError_t e;
   switch (p.c.block * kD / 8 / 128) {
-    case 1: kv8_append_kernel<kFmt, kDtype, kD, 128, 1><<<grid, 128, 0, stream>>>(p); break;
-    case 2: kv8_append_kernel<kFmt, kDtype, kD, 128, 2><<<grid, 128, 0, stream>>>(p); break;
-    case 4: kv8_append_kernel<kFmt, kDtype, kD, 128, kAppendVecs><<<grid, 128, 0, stream>>>(p); break;
-    case 8: kv8_append_kernel<kFmt, kDtype, kD, 256, kAppendVecs><<<grid, 256, 0, stream>>>(p); break;
-    default: kv8_append_kernel<kFmt, kDtype, kD, 256, 8><<<grid, 256, 0, stream>>>(p); break;
+    case 1: e = launch_after(kv8_append_kernel<kFmt, kDtype, kD, 128, 1>, grid, 128, 0, stream, 1, p); break;
+    case 2: e = launch_after(kv8_append_kernel<kFmt, kDtype, kD, 128, 2>, grid, 128, 0, stream, 1, p); break;
+    case 4: e = launch_after(kv8_append_kernel<kFmt, kDtype, kD, 128, kAppendVecs>, grid, 128, 0, stream, 1, p); break;
+    case 8: e = launch_after(kv8_append_kernel<kFmt, kDtype, kD, 256, kAppendVecs>, grid, 256, 0, stream, 1, p); break;
+    default: e = launch_after(kv8_append_kernel<kFmt, kDtype, kD, 256, 8>, grid, 256, 0, stream, 1, p); break;
   }
-  return cuda_check(cudaGetLastError(), "kv8 append launch");
+  return cuda_check(e, "kv8 append launch");
 }
 
 template <int kFmt>

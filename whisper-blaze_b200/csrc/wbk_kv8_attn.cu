@@ -403,7 +403,16 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
   if (threadIdx.x == 0) {
     prefetch_tmap(&tmap_k);
     prefetch_tmap(&tmap_v);
+    for (int i = 0; i < kWarps; ++i) {
+      for (int j = 0; j < kMaxStages; ++j) mbar_init(&s.full[i][j], 1);
+      s.tickets[i] = 0;
+    }
+    s.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  griddep_launch_dependents();
+  __syncthreads();
+  griddep_wait();  // nothing below the set-up reads or writes memory that the kernel before may still use
   // this CTA's share [c0, c1) of the list, and of it this warp's, [x0, x1)
   const int total = total_tiles(p), items = p.batch * p.c.kv_heads * p.row_blocks;
   const int ctas = min(static_cast<int>(gridDim.x), max(items, total / least_share(total, items)));
@@ -413,15 +422,6 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
   if (c0 == c1) return;
   const int warps = min(kWarps, c1 - c0);
   const Split own(c1 - c0, warps);
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kWarps; ++i) {
-      for (int j = 0; j < kMaxStages; ++j) mbar_init(&s.full[i][j], 1);
-      s.tickets[i] = 0;
-    }
-    s.abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncthreads();
   if (warp >= warps) return;
   const int x0 = c0 + own.start(warp), x1 = c0 + own.start(warp + 1);
 
@@ -768,8 +768,7 @@ int launch_step(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParam
       configured[dev] = 1;
     }
   }
-  kv8_step_kernel<kFmt, kD><<<grid, kThreads, smem, stream>>>(tk, tv, p);
-  return cuda_check(cudaGetLastError(), "kv8 attention launch");
+  return cuda_check(launch_after(kv8_step_kernel<kFmt, kD>, dim3(grid), kThreads, smem, stream, 1, tk, tv, p), "kv8 attention launch");
 }
 
 }  // namespace

@@ -427,6 +427,8 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
+  griddep_launch_dependents();
+  griddep_wait();  // nothing above reads or writes memory that the kernel before may still use
 
   // this CTA's share [x0, x1) of the list
   const int64_t total = total_tiles(p);
@@ -860,8 +862,8 @@ int launch_prompt(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMa
       configured[dev] = 1;
     }
   }
-  kv8_prompt_kernel<kFmt, kD, kBf16><<<grid, kThreads, smem, stream>>>(tq, tk, tv, p);
-  return cuda_check(cudaGetLastError(), "kv8 prompt launch");
+  return cuda_check(launch_after(kv8_prompt_kernel<kFmt, kD, kBf16>, dim3(grid), kThreads, smem, stream, 1, tq, tk, tv, p),
+                    "kv8 prompt launch");
 }
 
 template <int kFmt, int kD>

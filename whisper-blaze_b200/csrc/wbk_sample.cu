@@ -427,6 +427,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
   const int64_t row = blockIdx.x / cluster.num_blocks();
   constexpr int kItem = kDtype == WBK_DT_F32 ? 4 : 2, kVec = 16 / kItem;
   int turn = 0;
+  griddep_launch_dependents();
+  griddep_wait();
   const uint8_t* logits = static_cast<const uint8_t*>(p.logits) + row * p.logits_stride * kItem;
   Row<kDtype, kResident> r;
   r.noise = p.noise + row * p.noise_stride;
@@ -629,19 +631,9 @@ int launch_sample(const SampleParams& p, int64_t rows, int ctas, cudaStream_t st
       configured[dev] = 1;
     }
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = kFixed + (kResident ? p.slice * 4 + 32 : 0);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_check(cudaLaunchKernelEx(&cfg, sample_kernel<kDtype, kResident>, p), "sample launch");
+  return cuda_check(launch_after(sample_kernel<kDtype, kResident>, dim3(static_cast<unsigned>(rows * ctas)), kThreads,
+                                 kFixed + (kResident ? p.slice * 4 + 32 : 0), stream, static_cast<unsigned>(ctas), p),
+                    "sample launch");
 }
 
 template <int kDtype>
