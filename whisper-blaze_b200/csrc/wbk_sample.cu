@@ -56,7 +56,9 @@ constexpr int kSliceElems = 25600;      // most tokens per CTA kept in shared me
 constexpr int kList = 2048;             // most tokens that one CTA gathers
 constexpr int kBins = kThreads;
 constexpr float kBinsPerUnit = 16.0f;
-constexpr int kNearBins = 128;          // of the first count: tokens within 8 of the maximum
+constexpr int kNearBins = 256;          // of the first count: tokens within 16 of the maximum
+constexpr int kFew = 64;                // tokens whose order is found by comparing all pairs
+static_assert(kFew * 2 <= kBins, "they lie where the counts were");
 constexpr int kRounds = 6;
 constexpr int kAhead = 8;               // loads in flight per thread
 // Error of the approximate race in log2 units: two roundings of a product up to 150 (tokens below 2^-149 have
@@ -134,6 +136,7 @@ struct SampleSmem {
   int bins[kBins];          // this CTA's counts
   int all[kBins];           // the row's, summed up within each 32
   int count;                // of rank 0: entries of its list
+  int base;                 // this CTA's first in that
   float scan[kWarps];
   uint64_t list[kList];     // of rank 0: places
 };
@@ -210,7 +213,7 @@ __device__ __forceinline__ Message exchange(const Message& m, const R& r, Sample
 template <bool kFirst, int kDtype, bool kResident>
 __device__ __forceinline__ uint64_t race(const Row<kDtype, kResident>& r, uint64_t limit, float least, bool mass,
                                          SampleSmem& s, float& raw, float& all) {
-  float best = -INFINITY, second = -INFINITY;
+  float best = -INFINITY, second = -INFINITY, best_e = 1.0f;
   int best_i = r.end;
   for (int i0 = r.begin + static_cast<int>(threadIdx.x); i0 < r.end; i0 += kAhead * kThreads) {
     float e[kAhead];
@@ -231,7 +234,7 @@ __device__ __forceinline__ uint64_t race(const Row<kDtype, kResident>& r, uint64
       float t = power - lg2(fmaxf(e[j], kMinNoise));
       if (power < least || (limit != 0 && place_of(l, i) <= limit)) t = -INFINITY;
       second = fmaxf(second, fminf(t, best));
-      if (t > best) best = t, best_i = i;
+      if (t > best) best = t, best_i = i, best_e = e[j];
     }
   }
   // the CTA's largest, then full evaluation of all that come near it
@@ -242,7 +245,7 @@ __device__ __forceinline__ uint64_t race(const Row<kDtype, kResident>& r, uint64
   for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s.scan[i]);
   uint64_t won = 0;
   if (best > -INFINITY && best >= top - kNear) {
-    won = score_place(r.score(r.logit(best_i), best_i), best_i);
+    won = score_place(r.weight(r.logit(best_i)) / fmaxf(best_e, kMinNoise), best_i);
     if (second >= top - kNear) {  // two of this thread's tokens are near: look at all of them again
       for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
         const float l = r.logit(i);
@@ -377,6 +380,23 @@ __device__ __forceinline__ uint64_t finish(const Row<kDtype, kResident>& r, int 
       hi = to;
       if (above + cut.upto == top_k) break;
       above += cut.before;
+      if (cut.upto - cut.before <= kFew) {  // few in this bin: count for each how many of them come before it
+        uint64_t* few = reinterpret_cast<uint64_t*>(s.bins);
+        if (threadIdx.x == 0) s.base = 0;
+        __syncthreads();  // also: the counts were read
+#pragma unroll
+        for (int m = 0; m < kPer; ++m)
+          if (v[m] > lo && v[m] <= hi) few[atomicAdd(&s.base, 1)] = v[m];
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < kPer; ++m)
+          if (v[m] > lo && v[m] <= hi) {
+            int place = above;
+            for (int i = 0; i < cut.upto - cut.before; ++i) place += few[i] > v[m];
+            if (place >= top_k) v[m] = 0;
+          }
+        break;
+      }
     }
 #pragma unroll
     for (int m = 0; m < kPer; ++m)
@@ -580,20 +600,37 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
       }
     }
     if (gather) {
-      // ---- what is left goes to rank 0, in any order
-      uint64_t* list = cluster.map_shared_rank(&s.list[0], 0);
-      int* count = cluster.map_shared_rank(&s.count, 0);
-      for (int i0 = r.begin; i0 < r.end; i0 += kThreads) {
-        const int i = i0 + static_cast<int>(threadIdx.x);
-        const float l = i < r.end ? r.logit(i) : 0.0f;
-        const bool in = i < r.end && (cut.bin < kBins ? (r.top - l) * kBinsPerUnit < cut.bin + 1 : place_of(l, i) > limit);
-        const uint32_t who = __ballot_sync(~0u, in);
-        if (who == 0) continue;
-        const int lane = threadIdx.x & 31;
-        int at = 0;
-        if (lane == __ffs(who) - 1) at = atomicAdd(count, __popc(who));
-        at = __shfl_sync(~0u, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
-        if (in && at < kList) list[at] = place_of(l, i);
+      // ---- what is left goes to rank 0, in any order: counted first, so that a CTA asks for its room in the list once
+      const auto in = [&](int i, float l) {
+        return cut.bin < kBins ? (r.top - l) * kBinsPerUnit < cut.bin + 1 : place_of(l, i) > limit;
+      };
+      int mine = 0;
+      for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) mine += in(i, r.logit(i));
+      int upto = mine;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(~0u, upto, o);
+        if ((threadIdx.x & 31) >= o) upto += y;
+      }
+      __syncthreads();
+      if ((threadIdx.x & 31) == 31) s.warp[threadIdx.x >> 5].c = upto;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        int sum = 0;
+        for (int i = 0; i < kWarps; ++i) {
+          const int c = s.warp[i].c;
+          s.warp[i].c = sum;
+          sum += c;
+        }
+        s.base = sum > 0 ? atomicAdd(cluster.map_shared_rank(&s.count, 0), sum) : 0;
+      }
+      __syncthreads();
+      if (mine > 0) {
+        uint64_t* list = cluster.map_shared_rank(&s.list[0], 0);
+        int at = s.base + s.warp[threadIdx.x >> 5].c + upto - mine;
+        for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
+          const float l = r.logit(i);
+          if (in(i, l) && at < kList) list[at++] = place_of(l, i);
+        }
       }
       cluster.sync();
       if (rank == 0) {
