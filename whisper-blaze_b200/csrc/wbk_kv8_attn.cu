@@ -98,6 +98,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
+// A try_wait may suspend for longer than a tile takes to come, so a limit below kFineTimeoutNs goes without.
+__device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns) {
+  if (timeout_ns >= kFineTimeoutNs && mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_slow(bar, parity, abort_flag, timeout_ns, KSITE_TILE);
+}
+
 // Tiles of a CTA's share, at least, where the SMs are not full: two per warp, and more for long items. An item of L
 // tiles in P parts takes about a * L / P + b * P, with a the time of a tile in a CTA and b that of joining a part
 // (0.18 and 0.45 us), least at a share of L / P = sqrt(L * b / a).
@@ -390,7 +396,6 @@ template <int kFmt, int kD>
 __global__ void __launch_bounds__(kThreads, kD == 64 ? 4 : 3)
 kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                 const Kv8AttnParams p) {
-  constexpr int kKSteps = kD / 16;  // of a score product
   constexpr int kMTiles = kD / 16;  // of an output product
   constexpr int kTileBytes = 2 * kTile * kD;
   extern __shared__ uint8_t smem_raw[];
@@ -526,7 +531,7 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
     for (int t = tile; t < t1; ++t) {
-      if (!__all_sync(~0u, mbar_wait(&s.full[warp][st], phase, abort_flag, p.timeout_ns, KSITE_TILE))) {
+      if (!__all_sync(~0u, tile_wait(&s.full[warp][st], phase, abort_flag, p.timeout_ns))) {
         // Give up: copies in flight land before the CTA ends (this tile's, and those of the stages after it).
         int dummy = 0;
         if (lane == 0) {

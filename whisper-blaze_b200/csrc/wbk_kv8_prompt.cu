@@ -55,6 +55,7 @@ constexpr int kFactors = 8;      // slots of per-tile factors: more tiles than t
 constexpr int kBlockBytes = kTile * 128;  // 64 channels of a 16-bit tile
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRaise = 8.0f;   // log2 units
+constexpr uint64_t kDrainNs = 100000000ull;  // least limit of the waits for what is in flight at the end
 constexpr int kTickets = 8;      // per CTA: one for each 32 rows
 static_assert(kTickets <= kKv8TicketsPerSm, "workspace layout");
 enum : uint32_t {
@@ -446,6 +447,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const int sub = min(p.a.c.block_log2, kTileLog2);  // log2 of tokens per TMA box
       const int cover = 32 << p.a.c.block_log2;          // tokens that 32 pages hold
       uint32_t unit = 0, g = 0, q_loads = 0;
+      int q_last = nq;  // query tiles of the last load
       bool ok = true;
       while (x < x1 && ok) {
         const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
@@ -492,7 +494,10 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           if (t == tile) {
             for (int qt = 0; qt < nq && ok; ++qt) {
               ok = warp_wait(&s.q_empty[qt], (q_loads & 1u) ^ 1u, abort_flag, p.timeout_ns, PSITE_PRODUCER);
-              if (!ok) break;
+              if (!ok) {
+                q_last = qt;
+                break;
+              }
               if (lane == 0) {
                 mbar_arrive_expect_tx(&s.q_full[qt], static_cast<uint32_t>(p.tile_pos * p.a.group * kD * 2));
                 for (int i = 0; i < C::kBlocks; ++i)
@@ -510,11 +515,13 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       // The CTA ends only when what was issued has landed and been used: every unit and query tile given back.
       if (lane == 0) {
         int dummy = 0;
-        const uint64_t limit = ok ? p.timeout_ns : 100000000ull;
+        const uint64_t limit = max(p.timeout_ns, kDrainNs);
         for (uint32_t i = unit > C::kRawUnits ? unit - C::kRawUnits : 0; i < unit; ++i)
           mbar_wait(&s.raw_full[i % C::kRawUnits], (i / C::kRawUnits) & 1u, &dummy, limit, PSITE_DRAIN);
-        if (q_loads > 0)
-          for (int qt = 0; qt < nq; ++qt) mbar_wait(&s.q_full[qt], (q_loads - 1) & 1u, &dummy, limit, PSITE_DRAIN);
+        for (int qt = 0; qt < nq; ++qt) {
+          const uint32_t n = q_loads - (qt >= q_last ? 1u : 0u);
+          if (n > 0) mbar_wait(&s.q_full[qt], (n - 1) & 1u, &dummy, limit, PSITE_DRAIN);
+        }
         if (ok) {  // and no commit to these barriers is still on its way
           if (q_loads > 0)
             for (int qt = 0; qt < nq; ++qt) mbar_wait(&s.q_empty[qt], (q_loads - 1) & 1u, abort_flag, limit, PSITE_DRAIN);
@@ -610,7 +617,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       // TMEM and the barriers are in use until every product issued has finished.
       commit(&s.drain[t]);
       int dummy = 0;
-      mbar_wait(&s.drain[t], 0, &dummy, ok ? p.timeout_ns : 100000000ull, PSITE_DRAIN);
+      mbar_wait(&s.drain[t], 0, &dummy, max(p.timeout_ns, kDrainNs), PSITE_DRAIN);
     }
   } else if (warp >= 10) {
     // ---------------------------------------------------------- converters
@@ -688,6 +695,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         if (hh > 2 * tile && __any_sync(~0u, alpha != 1.0f)) {
           // the sums are free once the previous half's product is done
           if (!warp_wait(&s.pv_done[t][h ^ 1], (h == 1 ? g : g - 1) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) {
+            tmem_st_wait();
             ok = false;
             break;
           }

@@ -308,6 +308,11 @@ def _zero_shared_workspaces(device_index: int) -> None:
             ws.zero_()
 
 
+def _zeros(nbytes: int, device: torch.device) -> torch.Tensor:
+    with torch.inference_mode(False):  # a tensor made in inference mode could not be zeroed again outside it
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+
 def splitk_workspace(device, nbytes: int) -> Optional[torch.Tensor]:
     """The per-device split-K workspace (zero-filled once, grown on demand).
 
@@ -319,7 +324,7 @@ def splitk_workspace(device, nbytes: int) -> Optional[torch.Tensor]:
     dev = torch.device(device)
     ws = _SPLITK_WS.get(dev)
     if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+        ws = _zeros(nbytes, dev)
         _SPLITK_WS[dev] = ws
     return ws
 
@@ -582,15 +587,18 @@ def _kv8_ws_bytes(index: int, batch: int, heads: int, kv_heads: int, queries: in
         return int(lib().wbk_attention_kv8_ws_bytes(batch, heads, kv_heads, queries, head_dim))
 
 
-def kv8_workspace(index: int, nbytes: int) -> torch.Tensor:
-    """The workspace of attention_kv8 on CUDA device `index` (zero-filled once, grown on demand), shared by its calls
-    there: calls that may run at the same time need workspaces of their own."""
+def kv8_workspace(index: int) -> torch.Tensor:
+    """The workspace of attention_kv8 on CUDA device `index`, shared by its calls there: calls that may run at the
+    same time need workspaces of their own. Made on first use (outside a capture, whose replays alone would zero it),
+    of the size that the largest call needs, and kept, so that captured graphs can hold its address."""
     while len(_KV8_WS) <= index:
         _KV8_WS.append(None)
-    ws = _KV8_WS[index]
-    if ws is None or ws.numel() < nbytes:
-        ws = _KV8_WS[index] = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
-    return ws
+    if _KV8_WS[index] is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first attention_kv8 on a device must run before a capture, or be given a workspace")
+        nbytes = max(_kv8_ws_bytes(index, 1, 1, 1, rows, 128) for rows in (8, 1024))
+        _KV8_WS[index] = _zeros(nbytes, torch.device("cuda", index))
+    return _KV8_WS[index]
 
 
 def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -674,9 +682,8 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         odt, oindex, oshape, os3 = _require_bhsd(o, "out")
         if odt != dt or oindex != index or oshape != shape:
             raise RuntimeError(f"out must be a {q.dtype} view of shape {tuple(shape)} on {q.device}")
-    need = _kv8_ws_bytes(index, B, H, kv_heads, T, D)
     if workspace is None:
-        workspace = kv8_workspace(index, need)
+        workspace = kv8_workspace(index)
     else:
         _require_on(index, workspace, "workspace")
     _launch(lib().wbk_attention_kv8,
