@@ -15,14 +15,16 @@
 // What bounds it: the row's logits and random numbers are read once, and everything
 // after that is latency -- a row is a chain of reductions. So a row is a cluster of
 // CTAs that keep their slices of the logits in shared memory and exchange sums and
-// maxima through distributed shared memory, and no step sorts the vocabulary:
+// maxima through distributed shared memory (each CTA writes to all others before
+// their one barrier), and no step sorts the vocabulary:
 //   1. the row's maximum M;
 //   2. sum of exp(l - M), for the log-probability, and either
-//      a. top_k up to kList: a count of the tokens by floor((M - l) * 16); the bins that
-//         hold the first top_k tokens (found by finer counts where these are not
-//         enough) are gathered by one CTA, which applies every filter and runs the
-//         race among the few kept (the random numbers of all other tokens are not
-//         read); or
+//      a. top_k up to kList: where as many threads' maxima lie as top_k asks for, there
+//         are as many tokens, and few more as a rule; these (or where that rule does
+//         not apply those of the first bins of a count by floor((M - l) * 16), or of
+//         finer counts) are gathered by one CTA, which applies every filter and runs
+//         the race among the few kept (the random numbers of all other tokens are
+//         not read); or
 //      b. the race among all tokens. Its winner is the answer if it is kept. If it
 //         is not, nothing after it in the order is kept either, so the race is run
 //         again among the tokens before it: gathered by one CTA as in a. once they
@@ -30,9 +32,17 @@
 //         what is left, so rounds are few; after kRounds of them (random numbers
 //         made to defeat this) the cut is found by halving instead.
 //
-// The race compares log2(p_i) - log2(e_i), one multiply-add and one approximate
-// logarithm per token, and evaluates p_i / e_i in full only for the tokens within
-// kNear of the largest: the answer is that of the full evaluation.
+// The race compares log2(p_i) - log2(e_i) with a log2 that is linear between powers
+// of two (no special-function instruction: the exponentials of step 2 keep that unit
+// busy), takes the largest of kAhead tokens at a time, and evaluates p_i / e_i in
+// full only for the tokens within kNear of the largest: the answer is that of the
+// full evaluation.
+//
+// Measured (logits in fp16, everything in L2): one row of 51866 4.2 us greedy, 6.2 us
+// without filters, 8.5 us with top_k 40, 8.4 us with top_p 0.9; 64 such rows 7.4, 10.9,
+// 13.6 and 21.6 us (20 MB are 3.0 us of HBM's time; each exchange takes 1.2 us, a pass over
+// a slice 1 to 4 us). 256 rows of 131072 in fp32 come in seven waves of clusters: 70,
+// 107, 106 and 154 us (268 MB are 41 us of HBM's time).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -56,14 +66,16 @@ constexpr int kSliceElems = 25600;      // most tokens per CTA kept in shared me
 constexpr int kList = 2048;             // most tokens that one CTA gathers
 constexpr int kBins = kThreads;
 constexpr float kBinsPerUnit = 16.0f;
-constexpr int kNearBins = 256;          // of the first count: tokens within 16 of the maximum
 constexpr int kFew = 64;                // tokens whose order is found by comparing all pairs
 static_assert(kFew * 2 <= kBins, "they lie where the counts were");
 constexpr int kRounds = 6;
-constexpr int kAhead = 8;               // loads in flight per thread
-// Error of the approximate race in log2 units: two roundings of a product up to 150 (tokens below 2^-149 have
-// p = 0), 1.8e-5, and of a logarithm up to 126, 0.8e-5, plus the approximate logarithm's 2^-22.
-constexpr float kNear = 1e-4f;
+constexpr int kAhead = 4;               // a thread's tokens of one step of the race, loaded one step ahead
+constexpr int kVecs = 4;                // 16-byte loads of logits in flight per thread
+// Error of the approximate race in log2 units: log2_below() is at most 0.08608 too small, and two roundings of values
+// below 2^10 and its 23 of 31 bits make 2e-4.
+constexpr float kNear = 0.0863f;
+// Of a log2 p below 150 and of an approximate logarithm.
+constexpr float kSlack = 1e-4f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMinNoise = 1.17549435e-38f;
 
@@ -111,6 +123,11 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// log2 of a positive normal number, linear between the powers of two (Mitchell 1962): its exponent and mantissa bits
+// read as a fixed-point number, the upper 23 of them as the mantissa of 2^23 + them. + 383.
+__device__ __forceinline__ float log2_below_383(float x) {
+  return __uint_as_float(__byte_perm(__float_as_uint(x), 0x4B000000u, 0x7321)) * 3.0517578125e-5f;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -132,11 +149,10 @@ struct Message {
 };
 struct SampleSmem {
   Message warp[kWarps];
-  Message said[2];          // exchanges alternate between the two
+  Message said[2][kMaxCluster];  // what each CTA said; exchanges alternate between the two
   int bins[kBins];          // this CTA's counts
   int all[kBins];           // the row's, summed up within each 32
-  int count;                // of rank 0: entries of its list
-  int base;                 // this CTA's first in that
+  int base;
   float scan[kWarps];
   uint64_t list[kList];     // of rank 0: places
 };
@@ -160,7 +176,6 @@ struct Row {
     else return load_logit<kDtype>(x, i);
   }
   __device__ __forceinline__ float weight(float l) const { return expf((l - top) / temperature); }
-  __device__ __forceinline__ float score(float l, int i) const { return weight(l) / fmaxf(noise[i], kMinNoise); }
 };
 
 __device__ __forceinline__ Message warp_join(Message m) {
@@ -171,10 +186,13 @@ __device__ __forceinline__ Message warp_join(Message m) {
   return m;
 }
 
-// Joins every thread's (max u, sum f, sum g, sum c) over the CTA, and says it to the
-// cluster: complete after the next cluster.sync().
+// Joins every thread's (max u, sum f, sum g, sum c) over the CTA and tells it to every CTA of the cluster; returns what
+// they all said, joined, and in `prior` the sum of c over the CTAs of lower rank. s.warp keeps the warps' parts. A
+// message is overwritten two exchanges later, when every CTA has passed the cluster.sync() in between.
 template <class R>
-__device__ __forceinline__ void say(Message m, const R& r, SampleSmem& s, int turn) {
+__device__ __forceinline__ Message exchange(Message m, const R& r, SampleSmem& s, cg::cluster_group& cluster, int& turn,
+                                            int& prior) {
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   m = warp_join(m);
   if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5] = m;
   __syncthreads();
@@ -182,60 +200,75 @@ __device__ __forceinline__ void say(Message m, const R& r, SampleSmem& s, int tu
     m = warp_join(threadIdx.x < kWarps ? s.warp[threadIdx.x] : Message{0, 0.0f, 0.0f, 0, 0.0f});
     const int token = place_index(m.u);
     m.l = token >= r.begin && token < r.end ? r.logit(token) : 0.0f;
-    if (threadIdx.x == 0) s.said[turn] = m;
+    if (static_cast<int>(threadIdx.x) < ctas) *cluster.map_shared_rank(&s.said[turn][rank], threadIdx.x) = m;
   }
-}
-// What the cluster said, joined. A message is overwritten two exchanges later, when
-// every CTA has passed the cluster.sync() in between.
-__device__ __forceinline__ Message hear(SampleSmem& s, cg::cluster_group& cluster, int& turn) {
-  Message r{0, 0.0f, 0.0f, 0, 0.0f};
-  for (unsigned i = 0; i < cluster.num_blocks(); ++i) {
-    const Message o = *cluster.map_shared_rank(&s.said[turn], i);
-    if (o.u > r.u) r.u = o.u, r.l = o.l;
-    r.f += o.f;
-    r.g += o.g;
-    r.c += o.c;
+  cluster.sync();
+  Message all{0, 0.0f, 0.0f, 0, 0.0f};
+  for (int i = 0; i < ctas; ++i) {
+    const Message o = s.said[turn][i];
+    if (o.u > all.u) all.u = o.u, all.l = o.l;
+    all.f += o.f;
+    all.g += o.g;
+    if (i == rank) prior = all.c;
+    all.c += o.c;
   }
   turn ^= 1;
-  return r;
+  return all;
 }
 template <class R>
 __device__ __forceinline__ Message exchange(const Message& m, const R& r, SampleSmem& s, cg::cluster_group& cluster,
                                             int& turn) {
-  say(m, r, s, turn);
-  cluster.sync();
-  return hear(s, cluster, turn);
+  int prior;
+  return exchange(m, r, s, cluster, turn, prior);
 }
+
+// The random numbers of the thread's kAhead tokens from i0 on.
+template <int kDtype, bool kResident>
+struct Noise {
+  float e[kAhead];
+  __device__ __forceinline__ Noise(const Row<kDtype, kResident>& r, int i0) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * kThreads;
+      e[j] = i < r.end ? r.noise[i] : 1.0f;
+    }
+  }
+};
 
 // The race among the tokens placed before (above) `limit` (0: all): score_place of
 // the CTA's winner in full evaluation, 0 if it has no token there. kFirst: also, per
 // thread, the sums of exp(l - top) and, if asked, of exp((l - top) / temperature).
 template <bool kFirst, int kDtype, bool kResident>
 __device__ __forceinline__ uint64_t race(const Row<kDtype, kResident>& r, uint64_t limit, float least, bool mass,
-                                         SampleSmem& s, float& raw, float& all) {
-  float best = -INFINITY, second = -INFINITY, best_e = 1.0f;
-  int best_i = r.end;
+                                         const Noise<kDtype, kResident>& ahead, SampleSmem& s, float& raw, float& all) {
+  // kAhead tokens at a time: their largest, and which kAhead the thread's largest came from
+  float best = -INFINITY, second = -INFINITY, e[kAhead];
+  int best_at = r.end;
+  const bool filtered = limit != 0 || least > -INFINITY;
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) e[j] = ahead.e[j];
   for (int i0 = r.begin + static_cast<int>(threadIdx.x); i0 < r.end; i0 += kAhead * kThreads) {
-    float e[kAhead];
+    float t[kAhead];
+    const Noise<kDtype, kResident> next(r, i0 + kAhead * kThreads);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int i = i0 + j * kThreads;
-      e[j] = i < r.end ? r.noise[i] : 1.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int i = i0 + j * kThreads;
-      if (i >= r.end) break;
-      const float l = r.logit(i), gap = l - r.top, power = gap * r.scale;
+      const float l = i < r.end ? r.logit(i) : -INFINITY, gap = l - r.top;
       if constexpr (kFirst) {
         raw += ex2(gap * kLog2e);
-        if (mass) all += ex2(power);
+        if (mass) all += ex2(gap * r.scale);
       }
-      float t = power - lg2(fmaxf(e[j], kMinNoise));
-      if (power < least || (limit != 0 && place_of(l, i) <= limit)) t = -INFINITY;
-      second = fmaxf(second, fminf(t, best));
-      if (t > best) best = t, best_i = i, best_e = e[j];
+      t[j] = fmaf(gap, r.scale, 383.0f) - log2_below_383(fmaxf(e[j], kMinNoise));
+      if (filtered && (gap * r.scale < least || (limit != 0 && place_of(l, i) <= limit))) t[j] = -INFINITY;
     }
+#pragma unroll
+    for (int n = kAhead / 2; n > 0; n /= 2)
+#pragma unroll
+      for (int j = 0; j < n; ++j) t[j] = fmaxf(t[j], t[j + n]);
+    second = fmaxf(second, fminf(t[0], best));
+    if (t[0] > best) best = t[0], best_at = i0;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) e[j] = next.e[j];
   }
   // the CTA's largest, then full evaluation of all that come near it
   float top = best;
@@ -245,13 +278,14 @@ __device__ __forceinline__ uint64_t race(const Row<kDtype, kResident>& r, uint64
   for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s.scan[i]);
   uint64_t won = 0;
   if (best > -INFINITY && best >= top - kNear) {
-    won = score_place(r.weight(r.logit(best_i)) / fmaxf(best_e, kMinNoise), best_i);
-    if (second >= top - kNear) {  // two of this thread's tokens are near: look at all of them again
-      for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
-        const float l = r.logit(i);
-        if (l > -INFINITY && (l - r.top) * r.scale >= least && place_of(l, i) > limit)
-          won = max(won, score_place(r.score(l, i), i));
-      }
+    // two of this thread's kAhead are near: look at all its tokens again
+    const int from = second >= top - kNear ? r.begin + static_cast<int>(threadIdx.x) : best_at;
+    const int to = second >= top - kNear ? r.end : min(best_at + kAhead * kThreads, r.end);
+#pragma unroll 4
+    for (int i = from; i < to; i += kThreads) {
+      const float l = r.logit(i), gap = l - r.top, e = fmaxf(r.noise[i], kMinNoise);
+      if (fmaf(gap, r.scale, 383.0f) - log2_below_383(e) >= top - kNear && gap * r.scale >= least && (limit == 0 || place_of(l, i) > limit))
+        won = max(won, score_place(r.weight(l) / e, i));
     }
   }
   return won;
@@ -284,7 +318,10 @@ __device__ __forceinline__ Cut cut_sums(int c, int least, SampleSmem& s) {
 }
 __device__ __forceinline__ Cut cut_bins(int least, SampleSmem& s, cg::cluster_group& cluster) {
   int c = 0;
-  for (unsigned i = 0; i < cluster.num_blocks(); ++i) c += *cluster.map_shared_rank(&s.bins[threadIdx.x], i);
+  const int ctas = static_cast<int>(cluster.num_blocks());
+#pragma unroll
+  for (int i = 0; i < kMaxCluster; ++i)
+    if (i < ctas) c += *cluster.map_shared_rank(&s.bins[threadIdx.x], i);
   return cut_sums(c, least, s);
 }
 
@@ -355,12 +392,18 @@ __device__ __forceinline__ uint64_t finish(const Row<kDtype, kResident>& r, int 
                                            float top_p, float min_p, float whole, SampleSmem& s) {
   constexpr int kPer = kList / kThreads;
   uint64_t v[kPer];  // 0: none, or out
+  float e[kPer];
 #pragma unroll
   for (int m = 0; m < kPer; ++m) {
     const int i = m * kThreads + static_cast<int>(threadIdx.x);
     v[m] = i < n ? s.list[i] : 0;
+    e[m] = i < n ? fmaxf(r.noise[place_index(v[m])], kMinNoise) : 1.0f;
   }
-  if (n > top_k) {
+  if (n > top_k && n <= kFew) {  // count for each how many come before it
+    int place = 0;
+    for (int i = 0; i < n; ++i) place += s.list[i] > v[0];
+    if (place >= top_k) v[0] = 0;
+  } else if (n > top_k) {
     // the place that top_k tokens lie above, as in kth_limit
     int above = 0;
 #pragma unroll
@@ -410,8 +453,7 @@ __device__ __forceinline__ uint64_t finish(const Row<kDtype, kResident>& r, int 
     own += w[m];
     score[m] = 0;
     if (v[m] != 0 && w[m] >= min_p && place_logit(v[m]) > -INFINITY) {
-      const int token = place_index(v[m]);
-      score[m] = score_place(w[m] / fmaxf(r.noise[token], kMinNoise), token);
+      score[m] = score_place(w[m] / e[m], place_index(v[m]));
     }
   }
   if (whole < 0.0f && top_p < 1.0f) whole = block_sum(own, s);
@@ -447,6 +489,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
   const int64_t row = blockIdx.x / cluster.num_blocks();
   constexpr int kItem = kDtype == WBK_DT_F32 ? 4 : 2, kVec = 16 / kItem;
   int turn = 0;
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   griddep_launch_dependents();
   griddep_wait();
   const uint8_t* logits = static_cast<const uint8_t*>(p.logits) + row * p.logits_stride * kItem;
@@ -463,13 +506,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
   float* held = reinterpret_cast<float*>(smem_raw + (sizeof(SampleSmem) + 15) / 16 * 16) + (kVec - head) % kVec;
   const uint8_t* from = logits + static_cast<int64_t>(r.begin + head) * kItem;
   float top = -INFINITY;
-  for (int v0 = threadIdx.x; v0 < vecs; v0 += kAhead / 2 * kThreads) {
-    uint4 v[kAhead / 2];
+  for (int v0 = threadIdx.x; v0 < vecs; v0 += kVecs * kThreads) {
+    uint4 v[kVecs];
 #pragma unroll
-    for (int j = 0; j < kAhead / 2; ++j)
+    for (int j = 0; j < kVecs; ++j)
       if (v0 + j * kThreads < vecs) v[j] = reinterpret_cast<const uint4*>(from)[v0 + j * kThreads];
 #pragma unroll
-    for (int j = 0; j < kAhead / 2; ++j) {
+    for (int j = 0; j < kVecs; ++j) {
       if (v0 + j * kThreads >= vecs) break;
       float f[kVec];
 #pragma unroll
@@ -493,17 +536,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
   }
   r.x = kResident ? static_cast<const void*>(held) : logits;
   s.bins[threadIdx.x] = 0;
-  if (threadIdx.x == 0) s.count = 0;
   const float temperature = p.temperature != nullptr ? p.temperature[row] : p.temperature_all;
   const float top_p = p.top_p != nullptr ? p.top_p[row] : p.top_p_all;
   const float min_p = p.min_p != nullptr ? p.min_p[row] : p.min_p_all;
   const int k_given = p.top_k != nullptr ? p.top_k[row] : p.top_k_all;
   const int top_k = k_given > 0 && k_given < p.vocab ? k_given : p.vocab;
-  r.temperature = temperature;
-  r.scale = fminf(kLog2e / temperature, 3e38f);
+  r.temperature = fminf(temperature, 1e30f);  // an infinite one, too, leaves masked tokens at p = 0
+  r.scale = fminf(kLog2e / r.temperature, 3e38f);
   const Message none{0, 0.0f, 0.0f, 0, 0.0f};
   Message m = none;
   m.u = place_of(top, -1);  // no token's place
+  const Noise<kDtype, kResident> first(r, r.begin + static_cast<int>(threadIdx.x));  // for the race, on its way meanwhile
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // every CTA of the cluster has started
   r.top = place_logit(exchange(m, r, s, cluster, turn).u);
 
   uint64_t winner = 0;  // a place
@@ -521,35 +565,51 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
     winner = m.u;
     raw = m.f;
   } else if (!empty) {
-    const float least = min_p > 0.0f ? lg2(min_p) - kNear : -INFINITY;  // of log2 p, for the race
+    const float least = min_p > 0.0f ? lg2(min_p) - kSlack : -INFINITY;  // of log2 p, for the race
     uint64_t limit = 0;    // every token at or after this place is out
     int left = p.vocab;    // tokens before it
     float whole = -1.0f;   // the mass top_p refers to
-    Cut cut{kBins, 0, 0};  // or: what is left are the tokens of the bins up to this, cut.before of them in the bins before
+    Cut cut{kBins, 0, 0};  // or: what is left are the tokens of the bins up to this
+    bool tight = false;    // .. and the last of the first top_k lies in the last of them
     bool gather = false;   // what is left fits one CTA's list
+    int mine = -1, prior;  // this thread's tokens of what is left, where they were counted; those of the CTAs before
+    const auto in = [&](int i, float l) {
+      return cut.bin < kBins ? (r.top - l) * kBinsPerUnit < cut.bin + 1 : place_of(l, i) > limit;
+    };
     if (top_k <= kList && top_k < p.vocab) {
-      // ---- 2a. count by distance from the maximum; the few tokens near it are enough as a rule
+      // ---- 2a. bins by distance from the maximum. Up to where as many threads' maxima lie as top_k there are at least
+      // as many tokens, and not many more where these are few.
+      if (top_k <= static_cast<int>(cluster.num_blocks()) * kThreads / 2) {
+        const float bin = (r.top - top) * kBinsPerUnit;
+        if (bin < kBins) atomicAdd(&s.bins[static_cast<int>(bin)], 1);
+        cluster.sync();
+        cut = cut_bins(top_k, s, cluster);
+      }
       m = none;
       for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
         const float gap = r.top - r.logit(i);
         m.f += ex2(-gap * kLog2e);
-        const float bin = gap * kBinsPerUnit;
-        if (bin < kNearBins) atomicAdd(&s.bins[static_cast<int>(bin)], 1);
+        m.c += gap * kBinsPerUnit < cut.bin + 1;
       }
-      raw = exchange(m, r, s, cluster, turn).f;
-      cut = cut_bins(top_k, s, cluster);
-      if (cut.bin == kBins) {  // the tokens further away, too
-        cluster.sync();
+      mine = m.c;
+      m = exchange(m, r, s, cluster, turn, prior);
+      raw = m.f;
+      left = m.c;
+      gather = true;
+      if (cut.bin == kBins || left > kList) {  // count the tokens
+        mine = -1;
+        s.bins[threadIdx.x] = 0;
+        __syncthreads();
         for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
           const float bin = (r.top - r.logit(i)) * kBinsPerUnit;
-          if (bin >= kNearBins && bin < kBins) atomicAdd(&s.bins[static_cast<int>(bin)], 1);
+          if (bin < kBins) atomicAdd(&s.bins[static_cast<int>(bin)], 1);
         }
         cluster.sync();
         cut = cut_bins(top_k, s, cluster);
+        tight = cut.bin < kBins && cut.upto <= kList;
+        if (tight) left = cut.upto;
+        else cut.bin = kBins, limit = kth_limit(r, top_k, s, cluster, left);  // still further, or many ties
       }
-      gather = true;
-      if (cut.bin < kBins && cut.upto <= kList) left = cut.upto;
-      else cut.bin = kBins, limit = kth_limit(r, top_k, s, cluster, left);  // still further, or many ties
     } else {
       if (top_k < p.vocab) {
         limit = kth_limit(r, top_k, s, cluster, left);
@@ -560,12 +620,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
         float all = 0.0f;
         Message w = none;
         if (round == 0) {
-          w.u = race<true>(r, limit, least, top_p < 1.0f && whole < 0.0f, s, w.f, w.g);
+          w.u = race<true>(r, limit, least, top_p < 1.0f && whole < 0.0f, first, s, w.f, w.g);
           w = exchange(w, r, s, cluster, turn);
           raw = w.f;
           if (whole < 0.0f) whole = w.g;
         } else {
-          w.u = race<false>(r, limit, least, false, s, all, all);
+          w.u = race<false>(r, limit, least, false, first, s, all, all);
           w = exchange(w, r, s, cluster, turn);
         }
         winner = place_of(w.l, place_index(w.u));
@@ -592,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
           if (gather) break;
           // every token before `limit` is kept: one more race decides
           w = none;
-          w.u = race<false>(r, limit, -INFINITY, false, s, all, all);
+          w.u = race<false>(r, limit, -INFINITY, false, first, s, all, all);
           w = exchange(w, r, s, cluster, turn);
           winner = place_of(w.l, place_index(w.u));
           break;
@@ -600,33 +660,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
       }
     }
     if (gather) {
-      // ---- what is left goes to rank 0, in any order: counted first, so that a CTA asks for its room in the list once
-      const auto in = [&](int i, float l) {
-        return cut.bin < kBins ? (r.top - l) * kBinsPerUnit < cut.bin + 1 : place_of(l, i) > limit;
-      };
-      int mine = 0;
-      for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) mine += in(i, r.logit(i));
+      // ---- what is left goes to rank 0: counted first, so that each thread knows its place in the list
+      if (mine < 0) {
+        m = none;
+        for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) m.c += in(i, r.logit(i));
+        mine = m.c;
+        exchange(m, r, s, cluster, turn, prior);
+      }
       int upto = mine;
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(~0u, upto, o);
         if ((threadIdx.x & 31) >= o) upto += y;
       }
-      __syncthreads();
-      if ((threadIdx.x & 31) == 31) s.warp[threadIdx.x >> 5].c = upto;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        int sum = 0;
-        for (int i = 0; i < kWarps; ++i) {
-          const int c = s.warp[i].c;
-          s.warp[i].c = sum;
-          sum += c;
-        }
-        s.base = sum > 0 ? atomicAdd(cluster.map_shared_rank(&s.count, 0), sum) : 0;
-      }
-      __syncthreads();
+      int at = prior + upto - mine;
+      for (int i = 0; i < static_cast<int>(threadIdx.x >> 5); ++i) at += s.warp[i].c;
       if (mine > 0) {
         uint64_t* list = cluster.map_shared_rank(&s.list[0], 0);
-        int at = s.base + s.warp[threadIdx.x >> 5].c + upto - mine;
         for (int i = r.begin + static_cast<int>(threadIdx.x); i < r.end; i += kThreads) {
           const float l = r.logit(i);
           if (in(i, l) && at < kList) list[at++] = place_of(l, i);
@@ -635,8 +684,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
       cluster.sync();
       if (rank == 0) {
         uint64_t hi = place_of(r.top, 0);
-        if (cut.bin < kBins) {  // the last of the first top_k lies in the last bin; one bin more on both sides covers rounding
-          if (cut.bin > 1) hi = place_of(r.top - (cut.bin - 1) / kBinsPerUnit, 0);
+        if (cut.bin < kBins) {  // one bin more on both sides covers rounding
+          if (tight && cut.bin > 1) hi = place_of(r.top - (cut.bin - 1) / kBinsPerUnit, 0);
           limit = static_cast<uint64_t>(order_key(r.top - (cut.bin + 2) / kBinsPerUnit)) << 32;
         }
         winner = finish(r, min(left, kList), top_k, limit, hi, top_p, min_p, whole, s);
@@ -647,7 +696,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const Samp
     p.tokens[row] = empty ? -1 : place_index(winner);
     p.logprobs[row] = empty ? -INFINITY : (place_logit(winner) - r.top) - logf(raw);
   }
-  cluster.sync();  // no CTA ends while another may read its shared memory
 }
 
 template <int kDtype, bool kResident>
