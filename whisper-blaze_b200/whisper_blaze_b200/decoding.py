@@ -142,8 +142,9 @@ class Kv8Decoder:
         if self.own is None or self.own.batch != B:
             self._step = None  # the captured step holds the addresses of the caches being replaced
             args = (cfg.layers, B, cfg.heads, cfg.head_dim)
-            self.own = Kv8Cache(*args, cfg.max_tokens, self.device, self.block, self.fmt)
-            self.source = Kv8Cache(*args, cfg.source_tokens, self.device, self.block, self.fmt)
+            with torch.inference_mode(False):  # caches that a caller may write to outside it, too
+                self.own = Kv8Cache(*args, cfg.max_tokens, self.device, self.block, self.fmt)
+                self.source = Kv8Cache(*args, cfg.source_tokens, self.device, self.block, self.fmt)
         self.own.lens.zero_()
         self.source.lens.zero_()
         x = states.reshape(B * S, cfg.d_model)
