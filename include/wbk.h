@@ -351,9 +351,15 @@ int wbk_kv8_append(const void* k, const void* v, int dtype, int64_t batch, int64
  * rounded to fp16 before they multiply the (exact) fp16 values of the codes.
  * What lies in the cache behind a sequence's length is never used, whatever its
  * codes. A NaN code among the visible tokens makes its head's rows NaN.
- * workspace: wbk_attention_kv8_ws_bytes(...) bytes of device memory, 256-byte
- * aligned, zero-filled before first use and left reusable by each call, not used
- * by two calls at once; may be NULL where that is 0. */
+ * scale: positive and finite, or 0 (the mean of the visible values).
+ * workspace: wbk_attention_kv8_ws_bytes(...) bytes of device memory (every shape
+ * needs some), 256-byte aligned, zero-filled before first use and left reusable
+ * by each call, not used by two calls at once; after a WBK_ERR_DEVICE_TIMEOUT it
+ * must be zero-filled again. Its size does not depend on the lengths.
+ * Limits (WBK_ERR_UNSUPPORTED beyond): batch 32767, heads 65535, queries 16384,
+ * 2^30 tokens per table row, and for up to 32 rows per KV head (heads / kv_heads
+ * * queries) 2^31 tiles of 32 tokens that the table can hold in one call.
+ * Equal inputs give equal outputs, bit for bit. */
 int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
                       int64_t queries, int64_t head_dim, const int64_t* strides, int fmt, const void* k_cache,
                       const void* v_cache, const float* k_scale, const float* v_scale, int64_t pages,

@@ -222,8 +222,20 @@ def test_workspace_of_ones_own(cuda_device):
     assert torch.equal(ops.attention_kv8(*args, workspace=own), ops.attention_kv8(*args))
     with pytest.raises((RuntimeError, ValueError), match="workspace"):
         ops.attention_kv8(*args, workspace=own[:need - 256])
-    with pytest.raises((RuntimeError, ValueError), match="scale"):
-        ops.attention_kv8(*args, scale=-0.5)
+    for scale in (-0.5, float("inf"), float("nan")):
+        with pytest.raises((RuntimeError, ValueError), match="scale"):
+            ops.attention_kv8(*args, scale=scale)
+
+
+@pytest.mark.parametrize("queries", [1, 40])
+def test_a_scale_of_zero_gives_the_mean(cuda_device, queries):
+    q, kc, vc, ks, vs, table, lens = _long(cuda_device, queries)
+    y = ops.attention_kv8(q, kc, vc, ks, vs, table, lens, causal=False, scale=0.0)
+    v = vc.view(torch.float8_e4m3fn).double() * vs.double()[..., None, None]
+    for b, n in enumerate(lens.tolist()):
+        mean = v[table[b].long()].transpose(0, 1).reshape(2, -1, 64)[:, :n].mean(1)
+        # equal weights are exact; fp32 sums of at most 3840 positive values, and the output rounded to 11 bits
+        assert ((y[b].double() - mean.repeat_interleave(4, 0)[:, None]).abs() <= 2.0 ** -10 * mean.repeat_interleave(4, 0)[:, None]).all()
 
 
 def test_the_short_call_path_and_the_checked_one_agree(cuda_device, monkeypatch):

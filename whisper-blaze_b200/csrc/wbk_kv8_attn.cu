@@ -132,35 +132,42 @@ __device__ __forceinline__ int total_tiles(const Kv8AttnParams& p) {
   return __reduce_add_sync(~0u, sum) * p.c.kv_heads * p.row_blocks;
 }
 
-// The item and tile at place x of the list, by a converged warp.
-__device__ __forceinline__ Item locate(const Kv8AttnParams& p, int x, int& tile) {
-  const int lane = threadIdx.x & 31, per = p.c.kv_heads * p.row_blocks;
-  Item it{};
-  for (int b0 = 0;; b0 += 32) {
-    int len = 0, n = 0;
-    const int t = b0 + lane < p.batch ? tiles_of(p, b0 + lane, len, n) : 0;
-    int upto = t * per;
+// 32 sequences of the list, one per lane of a converged warp.
+struct Scan {
+  int b0 = -1, base;     // the first of them, places of the list before it
+  int len, n, t, upto;   // of this lane's sequence: as in Item; places up to its end, from base
+  __device__ __forceinline__ void load(const Kv8AttnParams& p, int first, int places) {
+    const int lane = threadIdx.x & 31;
+    b0 = first;
+    base = places;
+    len = n = t = 0;
+    if (b0 + lane < p.batch) t = tiles_of(p, b0 + lane, len, n);
+    upto = t * p.c.kv_heads * p.row_blocks;
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(~0u, upto, o);
       if (lane >= o) upto += y;
     }
-    const uint32_t past = __ballot_sync(~0u, upto > x);
-    if (past == 0 && b0 + 32 < p.batch) {
-      x -= __shfl_sync(~0u, upto, 31);
-      continue;
-    }
-    const int src = past != 0 ? __ffs(past) - 1 : 31;
-    x -= __shfl_sync(~0u, upto - t * per, src);
-    it.b = b0 + src;
-    it.len = __shfl_sync(~0u, len, src);
-    it.n = __shfl_sync(~0u, n, src);
-    it.tiles = __shfl_sync(~0u, t, src);
-    const int hr = x / it.tiles;
-    tile = x - hr * it.tiles;
-    it.h = hr / p.row_blocks;
-    it.rb = hr - it.h * p.row_blocks;
-    return it;
   }
+};
+
+// The item and tile at place x of the list, by a converged warp; `s` keeps what it looked at for the next place.
+__device__ __forceinline__ Item locate(const Kv8AttnParams& p, int x, int& tile, Scan& s) {
+  if (s.b0 < 0 || x < s.base) s.load(p, 0, 0);
+  uint32_t past;
+  while ((past = __ballot_sync(~0u, s.base + s.upto > x)) == 0 && s.b0 + 32 < p.batch)
+    s.load(p, s.b0 + 32, s.base + __shfl_sync(~0u, s.upto, 31));
+  const int src = past != 0 ? __ffs(past) - 1 : 31;
+  Item it{};
+  it.b = s.b0 + src;
+  it.len = __shfl_sync(~0u, s.len, src);
+  it.n = __shfl_sync(~0u, s.n, src);
+  it.tiles = __shfl_sync(~0u, s.t, src);
+  x -= s.base + __shfl_sync(~0u, s.upto, src) - it.tiles * p.c.kv_heads * p.row_blocks;
+  const int hr = x / it.tiles;
+  tile = x - hr * it.tiles;
+  it.h = hr / p.row_blocks;
+  it.rb = hr - it.h * p.row_blocks;
+  return it;
 }
 
 // `total` places dealt to n owners in contiguous shares, the first `r` of them one longer.
@@ -179,11 +186,11 @@ struct Split {
 __device__ __forceinline__ bool splits(int tiles, int share) { return tiles > min(share, kWhole); }
 
 // Where CTA k's share begins: at the nearer end of an item that is not to be split.
-__device__ __forceinline__ int share_start(const Kv8AttnParams& p, const Split& split, int k, int ctas, int total) {
+__device__ __forceinline__ int share_start(const Kv8AttnParams& p, const Split& split, int k, int ctas, int total, Scan& s) {
   if (k == 0 || k == ctas) return k == 0 ? 0 : total;
   int tile;
   const int x = split.start(k);
-  const Item it = locate(p, x, tile);
+  const Item it = locate(p, x, tile, s);
   if (splits(it.tiles, split.q)) return x;
   return 2 * tile < it.tiles ? x - tile : x - tile + it.tiles;
 }
@@ -423,7 +430,8 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
   const int ctas = min(static_cast<int>(gridDim.x), max(items, total / least_share(total, items)));
   if (blockIdx.x >= ctas) return;
   const Split split(total, ctas);
-  const int c0 = share_start(p, split, blockIdx.x, ctas, total), c1 = share_start(p, split, blockIdx.x + 1, ctas, total);
+  Scan scan;
+  const int c0 = share_start(p, split, blockIdx.x, ctas, total, scan), c1 = share_start(p, split, blockIdx.x + 1, ctas, total, scan);
   if (c0 == c1) return;
   const int warps = min(kWarps, c1 - c0);
   const Split own(c1 - c0, warps);
@@ -431,7 +439,7 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
   const int x0 = c0 + own.start(warp), x1 = c0 + own.start(warp + 1);
 
   int tile = 0;
-  Item it = locate(p, x0, tile);
+  Item it = locate(p, x0, tile, scan);
   uint8_t* ring = rings + warp * p.stages * kTileBytes;
   Loader loader;
   loader.start(p, it, tile, x0, x1);
@@ -847,7 +855,8 @@ int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_
     return fail(WBK_ERR_INVALID_ARG, "wbk_attention_kv8: q_lens misaligned");
   if (!aligned(q, 16) || !aligned(out, 16))
     return fail(WBK_ERR_UNSUPPORTED, "wbk_attention_kv8: q and out must be 16-byte aligned");
-  if (!(scale >= 0.0f)) return fail(WBK_ERR_INVALID_ARG, "wbk_attention_kv8: scale %g is negative", static_cast<double>(scale));
+  if (!(scale >= 0.0f && scale <= 3.402823466e38f))
+    return fail(WBK_ERR_INVALID_ARG, "wbk_attention_kv8: scale %g is negative or not finite", static_cast<double>(scale));
   for (int i = 0; i < 6; ++i)
     if (!kv8_stride_ok(strides[i]))
       return fail(WBK_ERR_UNSUPPORTED, "wbk_attention_kv8: stride[%d] = %lld is not a multiple of 8 elements", i,
