@@ -63,6 +63,13 @@ namespace {
 // the codes. The chain length -> page -> values -> maximum -> codes is all latency, so
 // where there are enough CTAs to fill the SMs one takes several heads of its page, with
 // the next head's values on their way meanwhile.
+//
+// Measured: 64 sequences of 1500 tokens, 20 heads of 64 (737 MB moved) 131 to 134 us,
+// 5.5 to 5.6 TB/s, 0.85 of a plain copy's rate; one head per CTA, a page in two passes
+// through shared memory: 146. 16 sequences of up to 1021 tokens, 8 heads of 128, into half-full
+// pages (64 MB) 16 us, 4.0 TB/s. One token for each of 64 sequences 4.5 us, launch and
+// that chain. The maximum is taken on 16-bit pairs as they are (exact), and a value's
+// code is its one rounding: fp16 / bf16 times a power of two is exact in fp32.
 
 struct AppendSide {
   const void* x;         // new keys or values, [batch, kv_heads, tokens, head_dim] view

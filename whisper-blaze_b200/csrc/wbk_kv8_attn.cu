@@ -26,7 +26,18 @@
 // m a running maximum of x_j + log2 vs, at most 2^8 too small (raising it rescales
 // the sums, so it is raised only when needed). The output is sum w_j code_j /
 // sum (w_j / vs). So w_j, rounded to fp16, is relative to the largest product of
-// weight and value scale, and pages of small scale lose nothing.
+// weight and value scale, and pages of small scale lose nothing. The rounding is an
+// error of 2^-11 of each weight, as fp16 codes need fp16 weights; totals take the fp32
+// weights. Queries in bf16 become fp16 by an exact power of two per row.
+//
+// Measured, head size 64: 64 sequences of 1500 tokens, 20 heads, one query (246 MB) 54 us:
+// HBM's rate (6.5 TB/s) from the first tile at 5 to 8 us to the first warps' end at
+// 42 us, and then the others' ends and joins. The same with 45 to 448 tokens (41 MB)
+// 20 us; one sequence of 224 tokens 7.4 us (launch, lengths, pages, codes, join: each
+// waits for the one before). Head size 128: 16 sequences of up to 32768 tokens, 8 KV heads for
+// 32 query heads (738 MB) 136 us, 5.4 TB/s, 0.83 of a plain copy's rate. Longer shares
+// for the CTAs that an SM gets first, which end first, gave nothing (54.4 -> 55.2 to
+// 57.5 us): HBM is busy meanwhile.
 #include <algorithm>
 #include <climits>
 #include <mutex>

@@ -26,6 +26,14 @@
 //     then bring its next scores (the order of products with different accumulators is
 //     not guaranteed, so the issuer waits for the first).
 //
+// Measured: 2011 queries of 32 heads (8 KV heads) of 128 behind 16000 cached tokens (0.49
+// TFLOP) 575 to 600 us, 0.82 to 0.86 PFLOP/s, half the rate of a plain bf16 product. The
+// tensor pipe is busy 44 % of the time, the exponentials' unit 45 %, issue slots 49 %:
+// a softmax warp waits for its own chain of loads, maxima, exponentials and stores.
+// Whole 128-token score tiles took 660 us; setmaxnreg in favour of the softmax, and part
+// of the exponentials as polynomials, gave nothing. 8 prompts of 223 tokens, 20 heads of 64:
+// 22 us (two tiles of work per SM; launch, set-up and join are most of it).
+//
 // The softmax is that of the few-rows kernel: running maximum of
 // log2(e) * scale * q.k + log2(value scale), raised when it is passed by 2^8.
 //
