@@ -30,8 +30,8 @@
 // TFLOP) 575 to 600 us, 0.82 to 0.86 PFLOP/s, half the rate of a plain bf16 product. The
 // tensor pipe is busy 44 % of the time, the exponentials' unit 45 %, issue slots 49 %:
 // a softmax warp waits for its own chain of loads, maxima, exponentials and stores.
-// Whole 128-token score tiles took 660 us; setmaxnreg in favour of the softmax, and part
-// of the exponentials as polynomials, gave nothing. 8 prompts of 223 tokens, 20 heads of 64:
+// Whole 128-token score tiles took 660 us; part of the exponentials as polynomials gave
+// nothing. 8 prompts of 223 tokens, 20 heads of 64:
 // 22 us (two tiles of work per SM; launch, set-up and join are most of it).
 //
 // The softmax is that of the few-rows kernel: running maximum of

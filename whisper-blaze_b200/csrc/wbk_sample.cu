@@ -62,7 +62,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kCtasPerSm = 2;
 constexpr int kLeastSlice = 2048;       // tokens per CTA, below which a row is not split further
-constexpr int kSliceElems = 25600;      // most tokens per CTA kept in shared memory (two CTAs per SM)
+constexpr int kSliceElems = 25600;      // most tokens per CTA kept in shared memory (two CTAs per SM up to 22000)
 constexpr int kList = 2048;             // most tokens that one CTA gathers
 constexpr int kBins = kThreads;
 constexpr float kBinsPerUnit = 16.0f;
