@@ -387,7 +387,7 @@ __device__ __forceinline__ float weights(uint32_t (&y)[32], const float4* factor
   return sum;
 }
 
-template <int kFmt, int kD, bool kBf16>
+template <int kFmt, int kD, bool kBf16, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
 kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                   const __grid_constant__ CUtensorMap tmap_v, const PromptParams p) {
@@ -397,7 +397,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                                                          ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort_flag;
-  const int nq = p.tiles_q;
+  const int nq = kSplit ? 2 : p.tiles_q;
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
@@ -417,9 +417,9 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.k_full[i], kConvThreads / 32);
-      mbar_init(&s.k_empty[i], static_cast<uint32_t>(nq));  // one per issuer
+      mbar_init(&s.k_empty[i], kSplit ? 1u : static_cast<uint32_t>(nq));  // one per issuer that uses it
       mbar_init(&s.v_full[i], kConvThreads / 32);
-      mbar_init(&s.v_empty[i], static_cast<uint32_t>(nq));
+      mbar_init(&s.v_empty[i], kSplit ? 1u : static_cast<uint32_t>(nq));
     }
     for (int i = 0; i < kFactors; ++i) mbar_init(&s.factor_full[i], 1);
     s.abort_flag = 0;
@@ -439,38 +439,55 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   griddep_launch_dependents();
   griddep_wait();  // nothing above reads or writes memory that the kernel before may still use
 
-  // this CTA's share [x0, x1) of the list
+  // this CTA's share of the list, or where the query tiles split it (kSplit) that of each, as of twice as many CTAs
   const int64_t total = total_tiles(p);
-  const int64_t active = max(min(static_cast<int64_t>(gridDim.x), total / 2), static_cast<int64_t>(1));
-  const int64_t x0 = blockIdx.x < active ? blockIdx.x * total / active : 0;
-  const int64_t x1 = blockIdx.x < active ? (blockIdx.x + 1) * total / active : 0;
-  int tile = 0;
-  Item it{};
-  if (x0 < x1) it = locate(p, x0, tile);
-  int64_t x = x0;
+  const int owners = static_cast<int>(gridDim.x) * (kSplit ? 2 : 1);
+  const int64_t active = max(min(static_cast<int64_t>(owners), total / 2), static_cast<int64_t>(1));
+  auto owner_of = [&](int t) { return static_cast<int>(blockIdx.x) + (kSplit ? t * static_cast<int>(gridDim.x) : 0); };
+  auto share = [&](int owner) { return owner < active ? owner * total / active : total; };  // its start
+  // Place of a query tile's i-th tile in the rings: its own count where they share all tiles, else in turn.
+  auto slot_of = [](uint32_t i, int t) { return kSplit ? 2 * i + static_cast<uint32_t>(t) : i; };
 
   if (warp == 8 || warp == 9 || warp == 14) {
     if (warp == 8) {
       // -------------------------------------------------------- producer
       const int sub = min(p.a.c.block_log2, kTileLog2);  // log2 of tokens per TMA box
       const int cover = 32 << p.a.c.block_log2;          // tokens that 32 pages hold
-      uint32_t unit = 0, g = 0, q_loads = 0;
-      int q_last = nq;  // query tiles of the last load
+      constexpr int kStreams = kSplit ? 2 : 1;  // kSplit: the two shares' tiles in turn
+      uint32_t unit = 0, tiles[kStreams] = {}, q_loads[2] = {0, 0};
       bool ok = true;
-      while (x < x1 && ok) {
-        const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
-        int blk0 = 0, te = tile;
-        PageLane pages{-1, 0.0f, 1.0f};
-        for (int t = tile; t < t1 && ok; ++t, ++g) {
-          if (t == te) {
-            blk0 = (t * kTile) >> p.a.c.block_log2;
-            pages = fetch_page(p, it, blk0 + lane);
-            te = ((blk0 << p.a.c.block_log2) + cover) >> kTileLog2;
+      Item its[kStreams];
+      int64_t xs[kStreams], ends[kStreams];
+      int ts[kStreams], t1s[kStreams], blk0s[kStreams], tes[kStreams];
+      PageLane held[kStreams];
+#pragma unroll
+      for (int u = 0; u < kStreams; ++u) {
+        xs[u] = share(owner_of(u)), ends[u] = share(owner_of(u) + 1);
+        if (owner_of(u) >= active) ends[u] = xs[u];
+        ts[u] = t1s[u] = 0;
+        if (xs[u] < ends[u]) {
+          its[u] = locate(p, xs[u], ts[u]);
+          t1s[u] = static_cast<int>(min(static_cast<int64_t>(its[u].tiles), ts[u] + (ends[u] - xs[u])));
+          tes[u] = ts[u];
+        }
+      }
+      bool fresh[kStreams] = {};  // a segment's first tile is done: its queries are loaded
+      while (ok && (xs[0] < ends[0] || xs[kStreams - 1] < ends[kStreams - 1])) {
+#pragma unroll
+        for (int u = 0; u < kStreams; ++u) {
+          if (!ok || xs[u] >= ends[u]) continue;
+          Item& it = its[u];
+          PageLane& pages = held[u];
+          const int t = ts[u];
+          if (t == tes[u]) {
+            blk0s[u] = (t * kTile) >> p.a.c.block_log2;
+            pages = fetch_page(p, it, blk0s[u] + lane);
+            tes[u] = ((blk0s[u] << p.a.c.block_log2) + cover) >> kTileLog2;
           }
           // ---- the tile's factors, before its codes
-          const int slot = static_cast<int>(g % kFactors);
+          const int slot = static_cast<int>(slot_of(tiles[u], u) % kFactors);
           const int pos = t * kTile + (lane & (kGroups - 1)) * 16;
-          const int from = ((pos >> p.a.c.block_log2) - blk0) & 31;
+          const int from = ((pos >> p.a.c.block_log2) - blk0s[u]) & 31;
           const int64_t page = __shfl_sync(~0u, pages.page, from);
           const float ks = __shfl_sync(~0u, pages.ks, from), vs = __shfl_sync(~0u, pages.vs, from);
           const bool there = page >= 0 && pos < it.len;
@@ -490,35 +507,39 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           const int y = (it.h << p.a.c.block_log2) + (pos & (p.a.c.block - 1));
 #pragma unroll 1
           for (int kv = 0; kv < 2; ++kv, ++unit) {
-            const int u = static_cast<int>(unit % C::kRawUnits);
-            if (ok) ok = warp_wait(&s.raw_empty[u], ((unit / C::kRawUnits) & 1u) ^ 1u, abort_flag, p.timeout_ns, PSITE_PRODUCER);
+            const int r = static_cast<int>(unit % C::kRawUnits);
+            if (ok) ok = warp_wait(&s.raw_empty[r], ((unit / C::kRawUnits) & 1u) ^ 1u, abort_flag, p.timeout_ns, PSITE_PRODUCER);
             if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[u], bytes);
+            if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[r], bytes);
             __syncwarp();
-            if (load) tma_load_3d(kv == 0 ? &tmap_k : &tmap_v, &s.raw_full[u], s.raw[u] + lane * 16 * kD, 0, y, static_cast<int>(page));
+            if (load) tma_load_3d(kv == 0 ? &tmap_k : &tmap_v, &s.raw_full[r], s.raw[r] + lane * 16 * kD, 0, y, static_cast<int>(page));
           }
           if (!ok) break;
+          ++tiles[u];
           // ---- queries, behind the item's first codes
-          if (t == tile) {
-            for (int qt = 0; qt < nq && ok; ++qt) {
-              ok = warp_wait(&s.q_empty[qt], (q_loads & 1u) ^ 1u, abort_flag, p.timeout_ns, PSITE_PRODUCER);
-              if (!ok) {
-                q_last = qt;
-                break;
-              }
+          if (!fresh[u]) {
+            fresh[u] = true;
+            for (int qt = kSplit ? u : 0; qt < (kSplit ? u + 1 : nq); ++qt) {
+              ok = warp_wait(&s.q_empty[qt], (q_loads[qt] & 1u) ^ 1u, abort_flag, p.timeout_ns, PSITE_PRODUCER);
+              if (!ok) break;
               if (lane == 0) {
                 mbar_arrive_expect_tx(&s.q_full[qt], static_cast<uint32_t>(p.tile_pos * p.a.group * kD * 2));
                 for (int i = 0; i < C::kBlocks; ++i)
-                  tma_load_5d(&tmap_q, &s.q_full[qt], s.q[qt] + i * kBlockBytes, i * 64, 0, (it.pb * nq + qt) * p.tile_pos, it.h, it.b);
+                  tma_load_5d(&tmap_q, &s.q_full[qt], s.q[qt] + i * kBlockBytes, i * 64, 0,
+                              (kSplit ? it.pb : it.pb * nq + qt) * p.tile_pos, it.h, it.b);
               }
               __syncwarp();
+              ++q_loads[qt];
             }
-            ++q_loads;
+          }
+          ++xs[u];
+          if (++ts[u] == t1s[u] && xs[u] < ends[u]) {
+            next_item(p, it);
+            ts[u] = tes[u] = 0;
+            t1s[u] = static_cast<int>(min(static_cast<int64_t>(it.tiles), ends[u] - xs[u]));
+            fresh[u] = false;
           }
         }
-        x += t1 - tile;
-        tile = 0;
-        if (x < x1) next_item(p, it);
       }
       // The CTA ends only when what was issued has landed and been used: every unit and query tile given back.
       if (lane == 0) {
@@ -526,24 +547,30 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         const uint64_t limit = max(p.timeout_ns, kDrainNs);
         for (uint32_t i = unit > C::kRawUnits ? unit - C::kRawUnits : 0; i < unit; ++i)
           mbar_wait(&s.raw_full[i % C::kRawUnits], (i / C::kRawUnits) & 1u, &dummy, limit, PSITE_DRAIN);
-        for (int qt = 0; qt < nq; ++qt) {
-          const uint32_t n = q_loads - (qt >= q_last ? 1u : 0u);
-          if (n > 0) mbar_wait(&s.q_full[qt], (n - 1) & 1u, &dummy, limit, PSITE_DRAIN);
-        }
+        for (int qt = 0; qt < nq; ++qt)
+          if (q_loads[qt] > 0) mbar_wait(&s.q_full[qt], (q_loads[qt] - 1) & 1u, &dummy, limit, PSITE_DRAIN);
         if (ok) {  // and no commit to these barriers is still on its way
-          if (q_loads > 0)
-            for (int qt = 0; qt < nq; ++qt) mbar_wait(&s.q_empty[qt], (q_loads - 1) & 1u, abort_flag, limit, PSITE_DRAIN);
-          for (uint32_t i = g > kStages ? g - kStages : 0; i < g; ++i) {
-            mbar_wait(&s.k_empty[i % kStages], (i / kStages) & 1u, abort_flag, limit, PSITE_DRAIN);
-            mbar_wait(&s.v_empty[i % kStages], (i / kStages) & 1u, abort_flag, limit, PSITE_DRAIN);
-          }
+          for (int qt = 0; qt < nq; ++qt)
+            if (q_loads[qt] > 0) mbar_wait(&s.q_empty[qt], (q_loads[qt] - 1) & 1u, abort_flag, limit, PSITE_DRAIN);
+#pragma unroll
+          for (int u = 0; u < kStreams; ++u)
+            for (uint32_t i = tiles[u] > kStages / kStreams ? tiles[u] - kStages / kStreams : 0; i < tiles[u]; ++i) {
+              const uint32_t g = slot_of(i, u);
+              mbar_wait(&s.k_empty[g % kStages], (g / kStages) & 1u, abort_flag, limit, PSITE_DRAIN);
+              mbar_wait(&s.v_empty[g % kStages], (g / kStages) & 1u, abort_flag, limit, PSITE_DRAIN);
+            }
         }
       }
     } else {
       // ------------------------------------- MMA issuers: warp 9 query tile 0, warp 14 query tile 1
       const int t = warp == 9 ? 0 : 1;
       uint32_t g = 0, ui = 0;
-      bool ok = t < nq;
+      bool ok = t < nq && owner_of(t) < active;
+      int tile = 0;
+      int64_t x = share(owner_of(t));
+      const int64_t x1 = share(owner_of(t) + 1);
+      Item it{};
+      if (ok) it = locate(p, x, tile);
       const uint32_t tm = static_cast<uint32_t>(uniform(static_cast<int>(tmem)));
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (ok) ok = warp_wait(bar, parity, abort_flag, p.timeout_ns, PSITE_MMA);
@@ -555,7 +582,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       };
       const int qt = uniform(t);
       auto issue_s = [&](int h, uint32_t gj) {
-        const int st = uniform(static_cast<int>(gj % kStages)), qh = uniform(h);
+        const int st = uniform(static_cast<int>(slot_of(gj, t) % kStages)), qh = uniform(h);
         if (elect_one()) {
           const uint32_t d = tm + s_col(qt, qh);
 #pragma unroll
@@ -570,7 +597,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         __syncwarp();
       };
       auto issue_pv = [&](int h, uint32_t gj, bool first) {
-        const int st = uniform(static_cast<int>(gj % kStages)), qh = uniform(h);
+        const int st = uniform(static_cast<int>(slot_of(gj, t) % kStages)), qh = uniform(h);
         const uint32_t onto = static_cast<uint32_t>(uniform(first ? 0 : 1));
         if (elect_one()) {
           const uint64_t vd = value_desc(s.v[st] + qh * (kHalf * 128));
@@ -591,7 +618,8 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll 1
         for (int j = -1; j < n && ok; ++j) {
           const uint32_t gj = g + static_cast<uint32_t>(j), gn = gj + 1;
-          if (j >= 0) wait(&s.v_full[gj % kStages], (gj / kStages) & 1u);
+          const uint32_t sj = slot_of(gj, t), sn = slot_of(gn, t);
+          if (j >= 0) wait(&s.v_full[sj % kStages], (sj / kStages) & 1u);
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
             if (j >= 0) {
@@ -602,7 +630,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
               issue_pv(h, gj, j == 0 && h == 0);
             }
             if (j + 1 < n) {
-              if (h == 0) wait(&s.k_full[gn % kStages], (gn / kStages) & 1u);
+              if (h == 0) wait(&s.k_full[sn % kStages], (sn / kStages) & 1u);
               if (gn > 0) wait(&s.pv_done[t][h], gj & 1u);
               if (!ok) break;
               tc_fence_after();
@@ -610,9 +638,9 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             }
           }
           if (!ok) break;
-          if (j >= 0) commit(&s.v_empty[gj % kStages]);
+          if (j >= 0) commit(&s.v_empty[sj % kStages]);
           if (j + 1 < n) {
-            commit(&s.k_empty[gn % kStages]);
+            commit(&s.k_empty[sn % kStages]);
             if (j + 2 == n) commit(&s.q_empty[t]);  // the item's last scores are issued
           }
         }
@@ -631,8 +659,12 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     // ---------------------------------------------------------- converters
     uint32_t unit = 0;
     bool ok = true;
-    const int64_t mine = x1 - x0;
-    for (int64_t i = 0; i < mine && ok; ++i) {
+    int64_t mine[2] = {0, 0};
+    for (int u = 0; u < (kSplit ? 2 : 1); ++u)
+      if (owner_of(u) < active) mine[u] = share(owner_of(u) + 1) - share(owner_of(u));
+    const int64_t rounds = kSplit ? 2 * max(mine[0], mine[1]) : mine[0];
+    for (int64_t i = 0; i < rounds && ok; ++i) {
+      if (kSplit && (i >> 1) >= mine[i & 1]) continue;
       const uint32_t g = static_cast<uint32_t>(i);
       const int st = static_cast<int>(g % kStages), slot = static_cast<int>(g % kFactors);
       const uint32_t empty = ((g / kStages) & 1u) ^ 1u;
@@ -656,17 +688,23 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     uint32_t g = 0;
-    bool ok = t < nq;
+    bool ok = t < nq && owner_of(t) < active;
+    int tile = 0;
+    int64_t x = share(owner_of(t));
+    const int64_t x1 = share(owner_of(t) + 1);
+    Item it{};
+    if (ok) it = locate(p, x, tile);
     while (x < x1 && ok) {
       const int t1 = static_cast<int>(min(static_cast<int64_t>(it.tiles), tile + (x1 - x)));
-      const int i = (it.pb * nq + t) * p.tile_pos + r / p.a.group, gi = r % p.a.group;  // query position and head
+      const int i = (kSplit ? it.pb : it.pb * nq + t) * p.tile_pos + r / p.a.group, gi = r % p.a.group;  // query position and head
       const bool real = r < p.tile_pos * p.a.group && i < p.a.queries;
       const int seq = kv8_len(p.a.lens, it.b, p.a.c);
       const int vis = i >= it.n ? 0 : p.a.causal ? max(seq - it.n + i + 1, 0) : seq;
       float m = -INFINITY, l = 0.0f;
       for (int hh = 2 * tile; hh < 2 * t1; ++hh) {  // 64 tokens at a time
-        const int h = hh & 1, slot = static_cast<int>(g % kFactors);
-        if ((h == 0 && !warp_wait(&s.factor_full[slot], (g / kFactors) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) ||
+        const uint32_t place = slot_of(g, t);
+        const int h = hh & 1, slot = static_cast<int>(place % kFactors);
+        if ((h == 0 && !warp_wait(&s.factor_full[slot], (place / kFactors) & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) ||
             !warp_wait(&s.s_full[t][h], g & 1u, abort_flag, p.timeout_ns, PSITE_SOFTMAX)) {
           ok = false;
           break;
@@ -761,27 +799,31 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       if (!whole) {
         part[256 * kD + row] = m;
         part[256 * kD + 256 + row] = l;
-        // the CTAs that this item lies in; the last of them to finish these 32 rows joins them
+        // the shares that this item lies in; the last of them to finish these 32 rows joins them
         const int64_t begin = x - tile, end = begin + it.tiles;
         const int first = static_cast<int>(((begin + 1) * active - 1) / total), last = static_cast<int>((end * active - 1) / total);
         __threadfence();
         __syncwarp();
         uint32_t before = 0;
         if (lane == 0) {
-          uint32_t* ticket = &p.tickets[first * kTickets + warp];
+          uint32_t* ticket = &p.tickets[kSplit ? first * 4 + quarter : first * kTickets + warp];
           before = atomicAdd(ticket, 1u);
           if (before == static_cast<uint32_t>(last - first)) *ticket = 0u;
         }
         if (__shfl_sync(~0u, before, 0) == static_cast<uint32_t>(last - first)) {
           __threadfence();
-          const float* base = p.parts + static_cast<int64_t>(first) * 2 * part_floats(kD);
           const int count = last - first + 1;
-          auto at = [&](int k) { return base + (k == 0 ? 1 : 2 * static_cast<int64_t>(k)) * part_floats(kD); };
+          // the part of the k-th share; in units of float4, a row's place in it is that of this thread's row
+          auto at = [&](int k) {
+            const int owner = first + k, cta = kSplit && owner >= static_cast<int>(gridDim.x) ? owner - gridDim.x : owner;
+            return p.parts + (static_cast<int64_t>(cta) * 2 + (k == 0 ? 1 : 0)) * part_floats(kD);
+          };
+          auto row_in = [&](int k) { return kSplit ? r + (first + k >= static_cast<int>(gridDim.x) ? kTile : 0) : row; };
           float top = -INFINITY, tot = 0.0f;
-          for (int k = 0; k < count; ++k) top = fmaxf(top, __ldcg(at(k) + 256 * kD + row));
+          for (int k = 0; k < count; ++k) top = fmaxf(top, __ldcg(at(k) + 256 * kD + row_in(k)));
           for (int k = 0; k < count; ++k) {
-            const float mk = __ldcg(at(k) + 256 * kD + row);
-            tot = fmaf(mk == -INFINITY ? 0.0f : ex2(mk - top), __ldcg(at(k) + 256 * kD + 256 + row), tot);
+            const float mk = __ldcg(at(k) + 256 * kD + row_in(k));
+            tot = fmaf(mk == -INFINITY ? 0.0f : ex2(mk - top), __ldcg(at(k) + 256 * kD + 256 + row_in(k)), tot);
           }
           const float invt = tot == 0.0f ? 0.0f : 1.0f / tot;
 #pragma unroll 1
@@ -790,10 +832,10 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll
             for (int k = 0; k < 32; ++k) o[k] = 0.0f;
             for (int k = 0; k < count; ++k) {
-              const float mk = __ldcg(at(k) + 256 * kD + row), f = mk == -INFINITY ? 0.0f : ex2(mk - top);
+              const float mk = __ldcg(at(k) + 256 * kD + row_in(k)), f = mk == -INFINITY ? 0.0f : ex2(mk - top);
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
-                const float4 y = __ldcg(reinterpret_cast<const float4*>(at(k)) + (c * 8 + e) * 256 + row);
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(at(k)) + (c * 8 + e) * 256 + row_in(k));
                 o[4 * e] = fmaf(f, y.x, o[4 * e]), o[4 * e + 1] = fmaf(f, y.y, o[4 * e + 1]);
                 o[4 * e + 2] = fmaf(f, y.z, o[4 * e + 2]), o[4 * e + 3] = fmaf(f, y.w, o[4 * e + 3]);
               }
@@ -858,7 +900,7 @@ int prompt_sms() {
   return n > 0 ? n : 148;
 }
 
-template <int kFmt, int kD, bool kBf16>
+template <int kFmt, int kD, bool kBf16, bool kSplit>
 int launch_prompt(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PromptParams& p, int grid,
                   cudaStream_t stream) {
   constexpr size_t smem = sizeof(PromptSmem<kD>) + 1024;
@@ -871,22 +913,25 @@ int launch_prompt(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMa
     std::lock_guard<std::mutex> lock(mu);
     if (static_cast<int>(configured.size()) <= dev) configured.resize(dev + 1, 0);
     if (!configured[dev]) {
-      if (int e = cuda_check(cudaFuncSetAttribute(kv8_prompt_kernel<kFmt, kD, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      if (int e = cuda_check(cudaFuncSetAttribute(kv8_prompt_kernel<kFmt, kD, kBf16, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                   static_cast<int>(smem)),
                              "kv8 prompt smem attribute"))
         return e;
       configured[dev] = 1;
     }
   }
-  return cuda_check(launch_after(kv8_prompt_kernel<kFmt, kD, kBf16>, dim3(grid), kThreads, smem, stream, 1, tq, tk, tv, p),
+  return cuda_check(launch_after(kv8_prompt_kernel<kFmt, kD, kBf16, kSplit>, dim3(grid), kThreads, smem, stream, 1, tq, tk, tv, p),
                     "kv8 prompt launch");
 }
 
 template <int kFmt, int kD>
 int dispatch_type(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PromptParams& p, int grid,
                   cudaStream_t stream) {
-  return p.a.bf16 ? launch_prompt<kFmt, kD, true>(tq, tk, tv, p, grid, stream)
-                  : launch_prompt<kFmt, kD, false>(tq, tk, tv, p, grid, stream);
+  if (p.tiles_q == 1)
+    return p.a.bf16 ? launch_prompt<kFmt, kD, true, true>(tq, tk, tv, p, grid, stream)
+                    : launch_prompt<kFmt, kD, false, true>(tq, tk, tv, p, grid, stream);
+  return p.a.bf16 ? launch_prompt<kFmt, kD, true, false>(tq, tk, tv, p, grid, stream)
+                  : launch_prompt<kFmt, kD, false, false>(tq, tk, tv, p, grid, stream);
 }
 
 }  // namespace
