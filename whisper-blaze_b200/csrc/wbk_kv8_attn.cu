@@ -774,9 +774,8 @@ int64_t step_ctas(const StepShape& s) { return static_cast<int64_t>(step_sms()) 
 
 // Many rows per KV head go to the kernel of wbk_kv8_prompt.cu, which converts each tile of codes once for up to 256 of
 // them; the one here takes time for each 8. us for 24, 32, 48 and 64 rows, here / there: 16 sequences of up to 16384
-// tokens, 8 KV heads, head size 64: 125 155 222 287 / 201 201 201 192, head size 128: 186 237 339 453 / 220 220 220 208;
-// 32 of up to 512: 28 30 32 34 / 29 29 29 28 and 28 32 39 47 / 34 34 34 33; 2 of up to 4096: 27 26 29 31 / 29 29 29 28
-// and 28 28 32 35 / 42 41 42 42.
+// tokens, 8 KV heads, head size 64: 125 155 222 287 / 155 for each, head size 128: 186 237 339 453 / 184; 32 of up to
+// 512: 28 30 32 34 / 28 and 28 32 39 47 / 35; 2 of up to 4096: 27 26 29 31 / 31 and 28 28 32 35 / 45.
 bool prompt_kernel(int64_t group, int64_t queries) { return group <= 128 && group * queries > 32; }
 
 template <int kFmt, int kD>

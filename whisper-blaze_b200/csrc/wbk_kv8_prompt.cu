@@ -18,6 +18,11 @@
 //     share of it, so causal triangles, ragged lengths and few long items fill the
 //     SMs alike. An item that lies in several CTAs is joined by the last of them,
 //     per 32 rows, in the order of the list.
+//   * Up to 128 rows (one query tile per item): a CTA takes two shares of the list, one
+//     for each of its softmax warpgroups, whose tiles come in turn. (16 sequences of
+//     up to 16384 tokens, 8 KV heads, 64 rows, head size 64 / 128: 155 / 184 us; one share
+//     with one warpgroup 192 / 209; the shares' keys and values in plain order, so that
+//     one share's keys wait for the other's products: 193 / 248.)
 //   * Warps 0-3 and 4-7: softmax of one query tile each, a row per thread; 8: TMA
 //     producer; 9 and 14: tcgen05 issuers, one per query tile; 10-13: converters.
 //   * Scores are computed for 64 tokens at a time, in two sets of TMEM columns per
@@ -27,7 +32,7 @@
 //     not guaranteed, so the issuer waits for the first).
 //
 // Measured: 2011 queries of 32 heads (8 KV heads) of 128 behind 16000 cached tokens (0.49
-// TFLOP) 575 to 600 us, 0.82 to 0.86 PFLOP/s, half the rate of a plain bf16 product. The
+// TFLOP) 546 to 570 us, 0.87 to 0.90 PFLOP/s, 0.55 of the rate of a plain bf16 product. The
 // tensor pipe is busy 44 % of the time, the exponentials' unit 45 %, issue slots 49 %:
 // a softmax warp waits for its own chain of loads, maxima, exponentials and stores.
 // Whole 128-token score tiles took 660 us; part of the exponentials as polynomials gave
@@ -59,7 +64,7 @@ constexpr int kThreads = 480;
 constexpr int kConvThreads = 128;
 constexpr int kConvWarp = 10;  // the first of them
 constexpr int kStages = 2;       // converted tiles of keys, and of values
-constexpr int kFactors = 8;      // slots of per-tile factors: more tiles than the ring lets the producer be ahead
+constexpr int kFactors = 8;      // slots of per-tile factors: more tiles than the rings let the producer be ahead
 constexpr int kBlockBytes = kTile * 128;  // 64 channels of a 16-bit tile
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRaise = 8.0f;   // log2 units
@@ -472,10 +477,29 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         }
       }
       bool fresh[kStreams] = {};  // a segment's first tile is done: its queries are loaded
-      while (ok && (xs[0] < ends[0] || xs[kStreams - 1] < ends[kStreams - 1])) {
+      // kSplit: values go one tile behind, so that no share's next keys wait for the other's products
+      bool vload[kStreams] = {};
+      uint32_t vbytes[kStreams] = {};
+      int vy[kStreams], vpage[kStreams];
+      auto issue = [&](const CUtensorMap* map, bool load, uint32_t bytes, int y, int page) {
+        const int r = static_cast<int>(unit % C::kRawUnits);
+        ok = warp_wait(&s.raw_empty[r], ((unit / C::kRawUnits) & 1u) ^ 1u, abort_flag, p.timeout_ns, PSITE_PRODUCER);
+        if (!ok) return;
+        if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[r], bytes);
+        __syncwarp();
+        if (load) tma_load_3d(map, &s.raw_full[r], s.raw[r] + lane * 16 * kD, 0, y, page);
+        ++unit;
+      };
+      bool behind[kStreams] = {};  // kSplit: the last values are still to come
+      while (ok && (xs[0] < ends[0] || xs[kStreams - 1] < ends[kStreams - 1] || behind[0] || behind[kStreams - 1])) {
 #pragma unroll
         for (int u = 0; u < kStreams; ++u) {
-          if (!ok || xs[u] >= ends[u]) continue;
+          if (!ok) break;
+          if (xs[u] >= ends[u]) {
+            if (behind[u]) issue(&tmap_v, vload[u], vbytes[u], vy[u], vpage[u]);
+            behind[u] = false;
+            continue;
+          }
           Item& it = its[u];
           PageLane& pages = held[u];
           const int t = ts[u];
@@ -501,21 +525,21 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&s.factor_full[slot]);
-          // ---- keys, then values: one box per page, which its first group stands for
+          // ---- keys, then values: one box per page, which the page's first group in the tile stands for
           const bool load = lane < kGroups && there && (lane & ((1 << (sub - 4)) - 1)) == 0;
           const uint32_t bytes = __popc(__ballot_sync(~0u, load)) * (static_cast<uint32_t>(kD) << sub);
           const int y = (it.h << p.a.c.block_log2) + (pos & (p.a.c.block - 1));
+          if constexpr (kSplit) {
+            issue(&tmap_k, load, bytes, y, static_cast<int>(page));
+            if (ok && tiles[u] > 0) issue(&tmap_v, vload[u], vbytes[u], vy[u], vpage[u]);
+            vload[u] = load, vbytes[u] = bytes, vy[u] = y, vpage[u] = static_cast<int>(page);
+          } else {
 #pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv, ++unit) {
-            const int r = static_cast<int>(unit % C::kRawUnits);
-            if (ok) ok = warp_wait(&s.raw_empty[r], ((unit / C::kRawUnits) & 1u) ^ 1u, abort_flag, p.timeout_ns, PSITE_PRODUCER);
-            if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[r], bytes);
-            __syncwarp();
-            if (load) tma_load_3d(kv == 0 ? &tmap_k : &tmap_v, &s.raw_full[r], s.raw[r] + lane * 16 * kD, 0, y, static_cast<int>(page));
+            for (int kv = 0; kv < 2 && ok; ++kv) issue(kv == 0 ? &tmap_k : &tmap_v, load, bytes, y, static_cast<int>(page));
           }
           if (!ok) break;
           ++tiles[u];
+          behind[u] = kSplit;
           // ---- queries, behind the item's first codes
           if (!fresh[u]) {
             fresh[u] = true;
@@ -662,15 +686,17 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     int64_t mine[2] = {0, 0};
     for (int u = 0; u < (kSplit ? 2 : 1); ++u)
       if (owner_of(u) < active) mine[u] = share(owner_of(u) + 1) - share(owner_of(u));
-    const int64_t rounds = kSplit ? 2 * max(mine[0], mine[1]) : mine[0];
+    // kSplit: of each share in turn the next keys, then values; otherwise keys and values in turn
+    const int64_t rounds = kSplit ? 2 * (max(mine[0], mine[1]) + 1) : mine[0];
     for (int64_t i = 0; i < rounds && ok; ++i) {
-      if (kSplit && (i >> 1) >= mine[i & 1]) continue;
-      const uint32_t g = static_cast<uint32_t>(i);
-      const int st = static_cast<int>(g % kStages), slot = static_cast<int>(g % kFactors);
-      const uint32_t empty = ((g / kStages) & 1u) ^ 1u;
-      ok = warp_wait(&s.factor_full[slot], (g / kFactors) & 1u, abort_flag, p.timeout_ns, PSITE_CONVERT);
 #pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv, ++unit) {
+      for (int kv = 0; kv < 2; ++kv) {
+        const int64_t own = kSplit ? (i >> 1) - kv : i;  // tile of the share
+        if (kSplit && (own < 0 || own >= mine[i & 1])) continue;
+        const uint32_t g = kSplit ? slot_of(static_cast<uint32_t>(own), static_cast<int>(i & 1)) : static_cast<uint32_t>(i);
+        const int st = static_cast<int>(g % kStages), slot = static_cast<int>(g % kFactors);
+        const uint32_t empty = ((g / kStages) & 1u) ^ 1u;
+        if (kSplit || kv == 0) ok = warp_wait(&s.factor_full[slot], (g / kFactors) & 1u, abort_flag, p.timeout_ns, PSITE_CONVERT);
         const int u = static_cast<int>(unit % C::kRawUnits);
         if (ok) ok = warp_wait(&s.raw_full[u], (unit / C::kRawUnits) & 1u, abort_flag, p.timeout_ns, PSITE_CONVERT);
         if (ok) ok = warp_wait(kv == 0 ? &s.k_empty[st] : &s.v_empty[st], empty, abort_flag, p.timeout_ns, PSITE_CONVERT);
@@ -681,6 +707,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         else convert_tile<kFmt, kD, false>(s.raw[u], to, &s.raw_empty[u], clear, s.factor[slot], s.limit[slot]);
         fence_async_smem();
         warp_arrive(kv == 0 ? &s.k_full[st] : &s.v_full[st]);
+        ++unit;
       }
     }
   } else {
