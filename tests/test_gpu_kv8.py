@@ -291,6 +291,28 @@ def test_a_long_cache_and_equal_bits(cuda_device, T):
         assert torch.equal(ops.attention_kv8(*args), y)
 
 
+@pytest.mark.parametrize("d,T,group,dtype,fmt", [(64, 9, 4, torch.float16, "e4m3"), (128, 33, 1, torch.bfloat16, "e4m3"),
+                                                 (64, 128, 1, torch.bfloat16, "e5m2"), (128, 15, 8, torch.float16, "e5m2")])
+@pytest.mark.parametrize("causal", [True, False])
+def test_33_to_128_rows(cuda_device, causal, d, T, group, dtype, fmt):
+    """Two shares of the work per CTA: one long sequence in all of them, short ones of a tile or two, one with nothing."""
+    lens, q_lens = [9000, 130, 0, T, 257, 700], [T, T, T, 5, 0, T - 1]
+    c = Cache(cuda_device, len(lens), 2, d, 64, -(-max(lens) // 64), fmt, seed=T)
+    q = _q(cuda_device, 50 + T, len(lens), 2 * group, T, d, dtype=dtype)
+    gpu = c.to_gpu()
+    y = _attention_check(cuda_device, c, q, lens, q_lens, causal, gpu=gpu)
+    for _ in range(3):
+        assert torch.equal(ops.attention_kv8(q, *gpu, _i32(cuda_device, lens), _i32(cuda_device, q_lens), causal=causal,
+                                             fmt=fmt), y)
+
+
+def test_many_items_of_one_tile(cuda_device):
+    """More items than shares, each of one tile of 64 rows."""
+    lens = [1 + i * 3 % 128 for i in range(96)]
+    c = Cache(cuda_device, len(lens), 4, 64, 32, 4, seed=51)
+    _attention_check(cuda_device, c, _q(cuda_device, 52, len(lens), 4, 64, 64), lens, causal=False)
+
+
 def test_offsets_past_32_bits(cuda_device):
     """A pool whose last pages lie beyond 2^32 bytes, filled only where it is read."""
     pages, d, block = (1 << 32) // (128 * 128) + 40, 128, 128
