@@ -348,7 +348,9 @@ int wbk_kv8_append(const void* k, const void* v, int dtype, int64_t batch, int64
  * WBK_DT_BF16, head_dim values contiguous, element strides in the HOST array
  * strides[6] = {q_b, q_h, q_s, o_b, o_h, o_s}, each a multiple of 8; pointers
  * 16-byte aligned. Scores, softmax and sums in fp32; the softmax weights are
- * rounded to fp16 before they multiply the (exact) fp16 values of the codes.
+ * rounded to fp16 before they multiply the (exact) fp16 values of the codes: a
+ * token's term in the output is off by at most 2^-11 of itself and 2^-32 of the
+ * row's largest product of weight and value scale times the code.
  * What lies in the cache behind a sequence's length is never used, whatever its
  * codes. A NaN code among the visible tokens makes its head's rows NaN.
  * scale: positive and finite, or 0 (the mean of the visible values).

@@ -111,6 +111,11 @@ __device__ __forceinline__ uint32_t float2_to_pair(float a, float b) {
   }
 }
 
+// Softmax weights are held relative to 2^(m - kKv8Lift), m the row's running maximum, which is passed by 2^8 at most:
+// the largest is 2^15, the top of fp16's range. Rounded to fp16 a weight is then off by at most 2^-11 of itself and, below
+// fp16's normal range, 2^-25 * 2^-7 of the largest. Sums and totals carry the same factor.
+constexpr float kKv8Lift = 7.0f;
+
 // Length of sequence b, held to what the block table can address.
 __device__ __forceinline__ int kv8_len(const int32_t* lens, int b, const Kv8Pages& c) {
   const int64_t cap = static_cast<int64_t>(c.max_blocks) * c.block;

@@ -22,13 +22,13 @@
 //     product is free, so a lane's fragments are consecutive bytes of one token.
 //
 // Softmax in powers of two: with x_j = log2(e) * scale * q.k_j and a page's value
-// scale vs, the weight that meets the codes of V is w_j = 2^(x_j + log2 vs - m),
+// scale vs, the weight that meets the codes of V is w_j = 2^(x_j + log2 vs - m + 7),
 // m a running maximum of x_j + log2 vs, at most 2^8 too small (raising it rescales
 // the sums, so it is raised only when needed). The output is sum w_j code_j /
 // sum (w_j / vs). So w_j, rounded to fp16, is relative to the largest product of
-// weight and value scale, and pages of small scale lose nothing. The rounding is an
-// error of 2^-11 of each weight, as fp16 codes need fp16 weights; totals take the fp32
-// weights. Queries in bf16 become fp16 by an exact power of two per row.
+// weight and value scale, and pages of small scale lose nothing. The rounding, as fp16
+// codes need fp16 weights, is an error of 2^-11 of each weight and of 2^-32 of the
+// largest product; totals take the fp32 weights. Queries in bf16 become fp16 by an exact power of two per row.
 //
 // Measured, head size 64: 64 sequences of 1500 tokens, 20 heads, one query (246 MB) 54 us:
 // HBM's rate (6.5 TB/s) from the first tile at 5 to 8 us to the first warps' end at
@@ -615,7 +615,7 @@ kv8_step_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constan
           for (int j = 0; j < kMTiles; ++j) o[j][e] *= alpha, o[j][e + 2] *= alpha;
         }
       }
-      const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+      const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0] - kKv8Lift, m[1] == -INFINITY ? 0.0f : m[1] - kKv8Lift};
 #pragma unroll
       for (int gi = 0; gi < kGroups; ++gi) {
         // ---- weights of 16 tokens, transposed: tokens 2c, 2c + 1 (pb0) and 8 further (pb1) of row gid

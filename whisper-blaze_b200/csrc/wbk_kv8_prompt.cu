@@ -40,7 +40,8 @@
 // 22 us (two tiles of work per SM; launch, set-up and join are most of it).
 //
 // The softmax is that of the few-rows kernel: running maximum of
-// log2(e) * scale * q.k + log2(value scale), raised when it is passed by 2^8.
+// log2(e) * scale * q.k + log2(value scale), raised when it is passed by 2^8, and
+// weights 2^7 larger than relative to it.
 //
 // Every mbarrier wait is bounded; one that runs out records WBK_ERR_DEVICE_TIMEOUT,
 // raises the CTA's abort flag and every role leaves its loop; copies and products
@@ -759,7 +760,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           m = mx;
         }
         l *= alpha;
-        const float ref = m == -INFINITY ? 0.0f : m;
+        const float ref = m == -INFINITY ? 0.0f : m - kKv8Lift;
         // ---- weights, in place of their scores
         l += weights(ya, fac, ref);
         tmem_st_x16(sa, ya);
