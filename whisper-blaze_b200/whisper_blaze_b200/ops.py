@@ -294,16 +294,18 @@ def _scale_arg(scale: Scale, name: str, device) -> tuple[float, Optional[int]]:
 
 
 _SPLITK_WS: dict = {}
+_SPLITK_OUTGROWN: dict = {}  # device: workspaces that were too small for a later call
 _KV8_WS: list = []  # by device index
 
 
 @_lib.on_device_timeout
 def _zero_shared_workspaces(device_index: int) -> None:
     """After a device-side timeout a kernel may have left the sync words or split-K tickets of
-    the device's shared workspace non-zero; zero it again so the next call starts clean.
+    the device's shared workspaces non-zero; zero them again so the next call starts clean.
     (Workspaces passed by the caller are the caller's to zero, as wbk.h states.)"""
     shared = _KV8_WS[device_index] if device_index < len(_KV8_WS) else None
-    for ws in (_SPLITK_WS.get(torch.device("cuda", device_index)), shared):
+    dev = torch.device("cuda", device_index)
+    for ws in (_SPLITK_WS.get(dev), shared, *_SPLITK_OUTGROWN.get(dev, ())):
         if ws is not None:
             ws.zero_()
 
@@ -316,6 +318,7 @@ def _zeros(nbytes: int, device: torch.device) -> torch.Tensor:
 def splitk_workspace(device, nbytes: int) -> Optional[torch.Tensor]:
     """The per-device split-K workspace (zero-filled once, grown on demand).
 
+    One that was outgrown is kept: a captured graph may hold its address. Each is at least twice the one before.
     Shared by every short-M GEMM on the device, so such GEMMs must not run
     concurrently on different streams; pass `workspace=` to gemm_fp8 to give a
     stream its own."""
@@ -324,8 +327,12 @@ def splitk_workspace(device, nbytes: int) -> Optional[torch.Tensor]:
     dev = torch.device(device)
     ws = _SPLITK_WS.get(dev)
     if ws is None or ws.numel() < nbytes:
-        ws = _zeros(nbytes, dev)
-        _SPLITK_WS[dev] = ws
+        if ws is not None:
+            nbytes = max(nbytes, 2 * ws.numel())
+        new = _zeros(nbytes, dev)
+        if ws is not None:
+            _SPLITK_OUTGROWN.setdefault(dev, []).append(ws)
+        ws = _SPLITK_WS[dev] = new
     return ws
 
 
