@@ -187,13 +187,16 @@ class Kv8Decoder:
         return ops.sample(x, torch.empty_like(x, dtype=torch.float32).exponential_(), **settings)
 
     def _captured_step(self, settings: dict) -> dict:
+        """The graph of one step. To be called between start() and the prompt: the step that is run before the capture
+        writes at the start of empty sequences' first pages, which the prompt's append then starts afresh. (Behind a
+        prompt it could raise a page's scale and re-code the prompt's tokens.)"""
         key = tuple(sorted((k, v.data_ptr() if isinstance(v, torch.Tensor) else v) for k, v in settings.items()))
         if self._step is None or self._step["key"] != key:
             B = self.own.batch
             token = torch.zeros(B, 1, dtype=torch.int64, device=self.device)
-            lens, draws = self.own.lens.clone(), torch.cuda.get_rng_state(self.device)
-            self.step(token, **settings)  # every first-time initialisation; what it appended lies past the lengths
-            self.own.lens.copy_(lens)
+            draws = torch.cuda.get_rng_state(self.device)
+            self.step(token, **settings)  # every first-time initialisation
+            self.own.lens.zero_()
             torch.cuda.set_rng_state(draws, self.device)  # as if it had not been
             torch.cuda.synchronize(self.device)
             graph = torch.cuda.CUDAGraph()
@@ -220,10 +223,10 @@ class Kv8Decoder:
             self.start(states, state_lens)
             tokens = torch.empty(prompt.shape[0], count, dtype=torch.int64, device=self.device)
             logprobs = torch.empty(prompt.shape[0], count, dtype=torch.float32, device=self.device)
+            s = self._captured_step(settings) if count > 1 else None
             drawn, lp = self.step(prompt, prompt_lens, **settings)
             tokens[:, 0], logprobs[:, 0] = drawn, lp
             if count > 1:
-                s = self._captured_step(settings)
                 s["token"].copy_(drawn.clamp(min=0)[:, None])
                 for i in range(1, count):
                     s["graph"].replay()
