@@ -4,6 +4,7 @@ import torch
 
 from conftest import randn_f16
 from whisper_blaze_b200 import _lib, ops
+from whisper_blaze_b200.decoding import DecoderConfig, Kv8Decoder, random_decoder_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -37,4 +38,34 @@ def test_a_graph_of_linears_outlives_a_larger_call(cuda_device, monkeypatch):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert all(bool((m == 0x5A).all()) for m in marks)
     assert all(torch.equal(a, b) for a, b in zip(ops.linear_fp8(*larger), first))
+    assert _lib.device_error() == 0
+
+
+# ------------------------------------------------------------ two decoders
+
+CFG = DecoderConfig(d_model=256, heads=4, ffn=2048, layers=2, vocab=1003, max_tokens=200, source_tokens=70)
+
+
+def _decoder(dev, seed, batch=3):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    decoder = Kv8Decoder(CFG, random_decoder_weights(CFG, dev, seed=seed, std=0.1), dev)
+    states = torch.randn(batch, CFG.source_tokens, CFG.d_model, generator=g, device=dev).half()
+    prompt = torch.randint(CFG.vocab, (batch, 40), generator=g, device=dev)
+    return decoder, states, prompt
+
+
+def test_two_decoders_on_two_streams(cuda_device):
+    """Issued together they give what each gives alone."""
+    both = [_decoder(cuda_device, 81), _decoder(cuda_device, 82, batch=2)]
+    alone = [d.generate(s, p, 60, temperature=0.0) for d, s, p in both]
+    streams = [torch.cuda.Stream(cuda_device) for _ in both]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for (d, s, p), stream in zip(both, streams):
+            with torch.cuda.stream(stream):
+                got.append(d.generate(s, p, 60, temperature=0.0))
+        torch.cuda.synchronize()
+        for a, b in zip(got, alone):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     assert _lib.device_error() == 0

@@ -17,6 +17,9 @@ Takes the place of the decoder half of HF's WhisperForConditionalGeneration
 """
 from __future__ import annotations
 
+import contextlib
+import functools
+import threading
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Tuple
 
@@ -100,15 +103,50 @@ def random_decoder_weights(cfg: DecoderConfig, device, seed: int = 1234, std: fl
     return w
 
 
+_TURN = threading.RLock()
+_LAST: Dict[int, tuple] = {}  # by device index: the stream of the last decoder call, an event behind it
+
+
+@contextlib.contextmanager
+def _turn(device: torch.device):
+    """Work issued in here runs, on the GPU, after what was issued in here before it for that device, on whatever
+    stream: the decoders of a device share the workspaces of its linears and of its attention, which calls that
+    run at the same time must not, and their grid-wide linears need the SMs that another's could hold."""
+    with _TURN, torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            yield
+            return
+        index, stream = torch.cuda.current_device(), torch.cuda.current_stream()
+        stream_before, event = _LAST.get(index, (stream, None))
+        if stream_before != stream:
+            stream.wait_event(event)
+        try:
+            yield
+        finally:
+            event = torch.cuda.Event()
+            event.record(stream)
+            _LAST[index] = (stream, event)
+
+
+def _in_turn(fn):
+    @functools.wraps(fn)
+    def call(self, *args, **kwargs):
+        with _turn(self.device):
+            return fn(self, *args, **kwargs)
+    return call
+
+
 class Kv8Decoder:
-    """See the module's description. One instance runs one batch at a time, on one stream."""
+    """See the module's description. One instance runs one batch at a time, on one stream. Instances on one device take
+    turns, whatever their streams and threads; other calls of ops.linear_fp8, gemm_fp8 and attention_kv8 that may run
+    at the same time need workspaces of their own."""
 
     def __init__(self, cfg: DecoderConfig, weights: Dict[str, torch.Tensor], device, block: int = 64,
                  fmt: str = "e4m3") -> None:
         self.cfg, self.block, self.fmt = cfg, block, fmt
         self.device = torch.device(device)
         self.w = {k: t.to(self.device) for k, t in weights.items()}
-        with torch.cuda.device(self.device):
+        with _turn(self.device):
             # FP8 once; the fp16 originals of the linears are dropped, the embedding's stays for the lookup
             self.q = {k[:-2]: ops.quantise(t.contiguous()) for k, t in self.w.items() if k.endswith(".w")}
             self.q["vocab"] = ops.quantise(self.w["embed"].contiguous())
@@ -131,6 +169,7 @@ class Kv8Decoder:
         x = x.view(B, -1, parts, self.cfg.heads, self.cfg.head_dim)
         return [x[:, :, i].transpose(1, 2) for i in range(parts)]
 
+    @_in_turn
     @torch.inference_mode()
     def start(self, states: torch.Tensor, state_lens: Optional[torch.Tensor] = None) -> None:
         """Project the encoder's states [B, S, d_model] fp16 into each layer's cross cache and empty the other.
@@ -153,6 +192,7 @@ class Kv8Decoder:
             self.source.append(i, k, v, state_lens)
         self.source.advance(S if state_lens is None else state_lens)
 
+    @_in_turn
     @torch.inference_mode()
     def logits(self, tokens: torch.Tensor, new_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Run tokens [B, T] int64 behind those already held; fp16 logits [B, vocab] after each sequence's last.
@@ -179,6 +219,7 @@ class Kv8Decoder:
         last = h[:, -1] if new_lens is None else h[torch.arange(B, device=self.device), (new_lens.long() - 1).clamp(min=0)]
         return self._linear("vocab", self._norm("ln", last.contiguous()))
 
+    @_in_turn
     @torch.inference_mode()
     def step(self, tokens: torch.Tensor, new_lens: Optional[torch.Tensor] = None,
              **settings) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -208,6 +249,7 @@ class Kv8Decoder:
                           "settings": settings}
         return self._step
 
+    @_in_turn
     @torch.inference_mode()
     def generate(self, states: torch.Tensor, prompt: torch.Tensor, count: int,
                  state_lens: Optional[torch.Tensor] = None, prompt_lens: Optional[torch.Tensor] = None,
@@ -219,16 +261,15 @@ class Kv8Decoder:
         T = prompt.shape[1]
         if count < 1 or T < 1 or T + count - 1 > self.cfg.max_tokens:
             raise ValueError(f"{T} prompt tokens and {count} new ones; the decoder holds {self.cfg.max_tokens}")
-        with torch.cuda.device(self.device):
-            self.start(states, state_lens)
-            tokens = torch.empty(prompt.shape[0], count, dtype=torch.int64, device=self.device)
-            logprobs = torch.empty(prompt.shape[0], count, dtype=torch.float32, device=self.device)
-            s = self._captured_step(settings) if count > 1 else None
-            drawn, lp = self.step(prompt, prompt_lens, **settings)
-            tokens[:, 0], logprobs[:, 0] = drawn, lp
-            if count > 1:
-                s["token"].copy_(drawn.clamp(min=0)[:, None])
-                for i in range(1, count):
-                    s["graph"].replay()
-                    tokens[:, i], logprobs[:, i] = s["drawn"], s["logprob"]
+        self.start(states, state_lens)
+        tokens = torch.empty(prompt.shape[0], count, dtype=torch.int64, device=self.device)
+        logprobs = torch.empty(prompt.shape[0], count, dtype=torch.float32, device=self.device)
+        s = self._captured_step(settings) if count > 1 else None
+        drawn, lp = self.step(prompt, prompt_lens, **settings)
+        tokens[:, 0], logprobs[:, 0] = drawn, lp
+        if count > 1:
+            s["token"].copy_(drawn.clamp(min=0)[:, None])
+            for i in range(1, count):
+                s["graph"].replay()
+                tokens[:, i], logprobs[:, i] = s["drawn"], s["logprob"]
         return tokens, logprobs
