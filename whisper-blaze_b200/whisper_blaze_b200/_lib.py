@@ -110,12 +110,15 @@ _CALLS = ("wbk_kv8_append", "wbk_attention_kv8", "wbk_attention_kv8_ws_bytes", "
 
 def calls():
     """The extension module with the short way to the decoder-step calls (csrc/wbk_calls.cpp), bound to the loaded
-    libwbk.so; None where it is not built."""
+    libwbk.so; None where it is not built or does not load (one of another torch, say): ops.py then goes its own way."""
     if not os.path.exists(CALLS_PATH):
         return None
     loader = importlib.machinery.ExtensionFileLoader("_wbk_calls", CALLS_PATH)
-    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_wbk_calls", loader))
-    loader.exec_module(module)
+    try:
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_wbk_calls", loader))
+        loader.exec_module(module)
+    except ImportError:
+        return None
     module.bind(*(ctypes.cast(getattr(lib(), name), _vp).value for name in _CALLS))
     return module
 
