@@ -16,6 +16,7 @@ from __future__ import annotations
 import argparse
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -28,6 +29,7 @@ REPO = os.path.dirname(PKG)
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "lib", "libwbk.so")
 CALLS = os.path.join(PKG, "lib", "_wbk_calls.so")
+CALLS_FOR = os.path.join(BUILD, "_wbk_calls.for")  # what CALLS was compiled for
 INCLUDE = os.path.join(REPO, "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -79,21 +81,47 @@ def _compile(src: str, flags: list[str], force: bool, verbose: bool) -> tuple[st
     return obj, (r.stdout + r.stderr) if verbose else ""
 
 
+def _torch_root() -> str:
+    return os.path.dirname(importlib.util.find_spec("torch").origin)
+
+
+def calls_for() -> str:
+    """What the extension module is compiled for: an interpreter's and a torch's internals. The module says it too, and
+    _lib.calls compares it."""
+    with open(os.path.join(_torch_root(), "version.py")) as f:
+        version = re.search(r"^__version__ = ['\"](.+)['\"]", f.read(), re.M).group(1)
+    return f"{sysconfig.get_config_var('SOABI')} torch {version}"
+
+
+def _calls_stale(src: str) -> bool:
+    if _stale(CALLS, [src, os.path.join(INCLUDE, "wbk.h"), __file__]) or not os.path.exists(CALLS_FOR):
+        return True
+    with open(CALLS_FOR) as f:
+        return f.read() != calls_for()
+
+
 def _compile_calls(force: bool) -> None:
     """The extension module of wbk_calls.cpp, against this interpreter and the torch it imports."""
     src = os.path.join(HERE, "wbk_calls.cpp")
-    if not force and not _stale(CALLS, [src, os.path.join(INCLUDE, "wbk.h"), __file__]):
+    if not force and not _calls_stale(src):
         return
-    root = os.path.dirname(importlib.util.find_spec("torch").origin)
+    import torch  # for its C++ ABI
+    for old in (CALLS, CALLS_FOR):
+        if os.path.exists(old):
+            os.remove(old)
+    root = _torch_root()
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     inc = [INCLUDE, sysconfig.get_paths()["include"], os.path.join(root, "include"),
            os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include")]
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=1"]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DWBK_CALLS_FOR="{calls_for()}"']
     cmd += [f"-I{d}" for d in inc] + [src, "-o", CALLS, f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch_cpu",
                                       "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    with open(CALLS_FOR, "w") as f:
+        f.write(calls_for())
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

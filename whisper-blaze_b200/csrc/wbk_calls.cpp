@@ -262,4 +262,9 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_wbk_calls", nullptr, -1, g_meth
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__wbk_calls(void) { return PyModule_Create(&g_module); }
+PyMODINIT_FUNC PyInit__wbk_calls(void) {
+  PyObject* m = PyModule_Create(&g_module);
+  // the interpreter and the torch whose internals this was compiled against: the loader uses it with no other
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", WBK_CALLS_FOR) != 0) Py_CLEAR(m);
+  return m;
+}

@@ -10,6 +10,7 @@ import importlib.machinery
 import importlib.util
 import os
 import re
+import sysconfig
 import threading
 
 import torch
@@ -110,7 +111,8 @@ _CALLS = ("wbk_kv8_append", "wbk_attention_kv8", "wbk_attention_kv8_ws_bytes", "
 
 def calls():
     """The extension module with the short way to the decoder-step calls (csrc/wbk_calls.cpp), bound to the loaded
-    libwbk.so; None where it is not built or does not load (one of another torch, say): ops.py then goes its own way."""
+    libwbk.so; None where it is not built, is for another torch or interpreter, whose tensors it would misread, or does not
+    load: ops.py then goes its own way."""
     if not os.path.exists(CALLS_PATH):
         return None
     loader = importlib.machinery.ExtensionFileLoader("_wbk_calls", CALLS_PATH)
@@ -118,6 +120,8 @@ def calls():
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_wbk_calls", loader))
         loader.exec_module(module)
     except ImportError:
+        return None
+    if getattr(module, "built_for", None) != f"{sysconfig.get_config_var('SOABI')} torch {torch.__version__}":
         return None
     module.bind(*(ctypes.cast(getattr(lib(), name), _vp).value for name in _CALLS))
     return module
