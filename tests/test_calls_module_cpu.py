@@ -47,3 +47,25 @@ def test_a_module_for_another_torch_is_done_without_and_built_anew(tmp_path, mon
         assert build._calls_stale(src) is stale
     monkeypatch.setattr(torch, "__version__", "2.0.0")
     assert _lib.calls() is None
+
+
+def test_the_library_is_built_where_the_module_is_not(tmp_path, monkeypatch, capsys):
+    """No g++: everything but the module is linked, and the reason is printed."""
+    build = _build_py()
+    linked = []
+
+    def run(cmd, **_):
+        if cmd[0].endswith("g++"):
+            raise FileNotFoundError("g++")
+        linked.append(cmd)
+        return type("Done", (), {"returncode": 0, "stdout": "", "stderr": ""})
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    monkeypatch.setattr(build, "_calls_stale", lambda src: True)
+    for name, file in (("BUILD", ""), ("LIB", "libwbk.so"), ("CALLS", "_wbk_calls.so"), ("CALLS_FOR", "for")):
+        monkeypatch.setattr(build, name, str(tmp_path / file))
+    (tmp_path / "_wbk_calls.so").write_bytes(b"of another torch")
+    assert build.build() == build.LIB
+    assert "-shared" in linked[-1] and build.LIB in linked[-1]
+    assert not (tmp_path / "_wbk_calls.so").exists()  # a stale one does not stay
+    assert "_wbk_calls.so is not built" in capsys.readouterr().err

@@ -130,7 +130,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=len(UNITS) + 1) as ex:
         calls = ex.submit(_compile_calls, force)
         results = list(ex.map(lambda kv: _compile(kv[0], kv[1], force, verbose), UNITS.items()))
-        calls.result()
+        try:
+            calls.result()
+        except Exception as e:  # no Python headers, no g++, a torch without CUDA: the library does not need it
+            print(f"{CALLS} is not built; kv8_append, attention_kv8 and sample go through ctypes, at 12 to 18 us of host "
+                  f"time each:\n{e}", file=sys.stderr)
     objs = [o for o, _ in results]
     for _, log in results:
         if log:
