@@ -154,6 +154,21 @@ class Kv8Decoder:
         self.own: Optional[Kv8Cache] = None
         self.source: Optional[Kv8Cache] = None
         self._step: Optional[dict] = None
+        self._most = 0  # tokens that the longest sequence holds, at most: the host's count, padding included
+
+    def _make_room(self, T: int, new_lens: Optional[torch.Tensor]) -> None:
+        """Raises if T tokens more, or new_lens of them, are more than the positions of a sequence. The lengths are on the
+        device: they are looked at, and waited for, only where the host's count does not say. (What a caller's own graph
+        of logits() appends in its replays is not counted.)"""
+        if torch.cuda.is_current_stream_capturing():
+            return
+        if self._most + T > self.cfg.max_tokens:
+            most = int((self.own.lens + (T if new_lens is None else new_lens)).max())
+            if most > self.cfg.max_tokens:
+                raise ValueError(f"{T} more tokens make a sequence of {most}; the decoder holds {self.cfg.max_tokens}")
+            self._most = most
+        else:
+            self._most += T
 
     def _linear(self, name: str, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
                 epilogue: str = "none") -> torch.Tensor:
@@ -185,6 +200,7 @@ class Kv8Decoder:
                 self.own = Kv8Cache(*args, cfg.max_tokens, self.device, self.block, self.fmt)
                 self.source = Kv8Cache(*args, cfg.source_tokens, self.device, self.block, self.fmt)
         self.own.lens.zero_()
+        self._most = 0
         self.source.lens.zero_()
         x = states.reshape(B * S, cfg.d_model)
         for i in range(cfg.layers):
@@ -196,9 +212,11 @@ class Kv8Decoder:
     @torch.inference_mode()
     def logits(self, tokens: torch.Tensor, new_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Run tokens [B, T] int64 behind those already held; fp16 logits [B, vocab] after each sequence's last.
-        new_lens [B] int32: how many of the T are real (default: all)."""
+        new_lens [B] int32: how many of the T are real (default: all). ValueError where a sequence would have more
+        than max_tokens."""
         cfg, own, source = self.cfg, self.own, self.source
         B, T = tokens.shape
+        self._make_room(T, new_lens)
         at = own.lens.long()[:, None] + torch.arange(T, device=self.device)
         h = (self.w["embed"][tokens] + self.w["positions"][at.clamp_(max=cfg.max_tokens - 1)]).view(B * T, cfg.d_model)
         held = own.lens + (T if new_lens is None else new_lens)
@@ -238,6 +256,7 @@ class Kv8Decoder:
             draws = torch.cuda.get_rng_state(self.device)
             self.step(token, **settings)  # every first-time initialisation
             self.own.lens.zero_()
+            self._most = 0
             torch.cuda.set_rng_state(draws, self.device)  # as if it had not been
             torch.cuda.synchronize(self.device)
             graph = torch.cuda.CUDAGraph()
@@ -269,6 +288,7 @@ class Kv8Decoder:
         tokens[:, 0], logprobs[:, 0] = drawn, lp
         if count > 1:
             s["token"].copy_(drawn.clamp(min=0)[:, None])
+            self._most += count - 1
             for i in range(1, count):
                 s["graph"].replay()
                 tokens[:, i], logprobs[:, i] = s["drawn"], s["logprob"]
