@@ -61,3 +61,16 @@ def test_what_a_graph_appended_counts(setup):
     decoder.logits(tokens[:, :5])
     with pytest.raises(ValueError, match="holds 24"):
         decoder.logits(tokens[:, :1])
+
+
+def test_counts_beyond_what_is_given_are_all_of_it(setup):
+    """As kv8_append takes them: more than T is T, less than none is none; the lengths say what the caches hold."""
+    decoder, states, tokens = setup
+    decoder.start(states[:, :15], _i32(tokens, [15, 0]))
+    want = decoder.logits(tokens[:, :8], _i32(tokens, [8, 0]))
+    then = decoder.logits(tokens[:, 8:9])
+    decoder.start(states[:, :15], _i32(tokens, [20, -3]))
+    assert decoder.source.lens.tolist() == [15, 0]
+    got = decoder.logits(tokens[:, :8], _i32(tokens, [11, -2]))
+    assert decoder.own.lens.tolist() == [8, 0]
+    assert torch.equal(got, want) and torch.equal(decoder.logits(tokens[:, 8:9]), then)

@@ -202,6 +202,8 @@ class Kv8Decoder:
         self.own.lens.zero_()
         self._most = 0
         self.source.lens.zero_()
+        if state_lens is not None:
+            state_lens = state_lens.clamp(0, S)  # as kv8_append takes them
         x = states.reshape(B * S, cfg.d_model)
         for i in range(cfg.layers):
             k, v = self._heads(self._linear(f"{i}.xkv", x), B, 2)
@@ -216,6 +218,8 @@ class Kv8Decoder:
         than max_tokens."""
         cfg, own, source = self.cfg, self.own, self.source
         B, T = tokens.shape
+        if new_lens is not None:
+            new_lens = new_lens.clamp(0, T)  # as kv8_append takes them
         self._make_room(T, new_lens)
         at = own.lens.long()[:, None] + torch.arange(T, device=self.device)
         h = (self.w["embed"][tokens] + self.w["positions"][at.clamp_(max=cfg.max_tokens - 1)]).view(B * T, cfg.d_model)
