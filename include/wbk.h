@@ -314,7 +314,8 @@ int wbk_linear_fp8_f16(const void* A16, int64_t M, int64_t N, int64_t K, int a_f
  * and a table entry outside [0, pages) names no page: nothing is written there,
  * and attention leaves its tokens out.
  * Scales are powers of two, as wbk_kv8_append writes them; attention takes any
- * positive finite scale. No reference counterpart (the reference caches fp16 keys
+ * scale from 2^-64 (the least that is written) to 2^60 (values up to 2^68; only
+ * bf16 has larger ones). No reference counterpart (the reference caches fp16 keys
  * and values inside Hugging Face's decoder, whisper_blaze/model.py).
  */
 
@@ -349,10 +350,12 @@ int wbk_kv8_append(const void* k, const void* v, int dtype, int64_t batch, int64
  * strides[6] = {q_b, q_h, q_s, o_b, o_h, o_s}, each a multiple of 8; pointers
  * 16-byte aligned. Scores, softmax and sums in fp32; the softmax weights are
  * rounded to fp16 before they multiply the (exact) fp16 values of the codes: a
- * token's term in the output is off by at most 2^-11 of itself and 2^-32 of the
- * row's largest product of weight and value scale times the code.
+ * weight times its value scale is off by at most 2^-11 of itself and 2^-32 of the
+ * row's largest. Where the value scales of a sequence and head are 2^k apart, a
+ * token with less than 2^(k - 133) of another's weight may be left out.
  * What lies in the cache behind a sequence's length is never used, whatever its
- * codes. A NaN code among the visible tokens makes its head's rows NaN.
+ * codes. A NaN or infinite code (wbk_kv8_append writes none) among the tokens of a
+ * sequence can make all rows of its head NaN, causal rows before it included.
  * scale: positive and finite, or 0 (the mean of the visible values).
  * workspace: wbk_attention_kv8_ws_bytes(...) bytes of device memory (every shape
  * needs some), 256-byte aligned, zero-filled before first use and left reusable
@@ -360,7 +363,8 @@ int wbk_kv8_append(const void* k, const void* v, int dtype, int64_t batch, int64
  * must be zero-filled again. Its size does not depend on the lengths.
  * Limits (WBK_ERR_UNSUPPORTED beyond): batch 32767, heads 65535, queries 16384,
  * 2^30 tokens per table row, and for up to 32 rows per KV head (heads / kv_heads
- * * queries) 2^31 tiles of 32 tokens that the table can hold in one call.
+ * * queries), more than 128 query heads per KV head or queries repeated by a stride
+ * of 0, 2^31 tiles of 32 tokens (per 8 rows) that the table can hold in one call.
  * Equal inputs give equal outputs, bit for bit. */
 int wbk_attention_kv8(const void* q, void* out, int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
                       int64_t queries, int64_t head_dim, const int64_t* strides, int fmt, const void* k_cache,
