@@ -65,7 +65,17 @@ constexpr int kThreads = 480;
 constexpr int kConvThreads = 128;
 constexpr int kConvWarp = 10;  // the first of them
 constexpr int kStages = 2;       // converted tiles of keys, and of values
-constexpr int kFactors = 8;      // slots of per-tile factors: more tiles than the rings let the producer be ahead
+// Slots of per-tile factors. The producer writes a tile's factors before it asks for its codes, and nothing tells it that
+// a slot is free: there are more than it can be ahead of the softmax. With R units in the ring of codes:
+//   * One share. At tile i the values of tile i - 1 have been asked for, so those of i - 1 - R / 2 have been converted, so the
+//     product that had their stage, of tile i - 1 - R / 2 - kStages, is done, and the softmax of that tile.
+//   * Two shares, each with half of the slots and one stage, values one tile behind keys. At tile i of a share
+//     its values of tile i - 2 have been asked for. The other share's codes lie in between, so those of i - 3 have been
+//     converted, and the product of i - 4 is done: tiles i - 3 to i may be in use, four slots. A share whose
+//     neighbour has ended would need one more from its second lone tile on, if that is tile 4 or later. There is none such: where
+//     both have tiles they differ by one at most (shares of one list), and where one has none the list is short,
+//     total / 2 shares of 2 or 3 tiles.
+constexpr int kFactors = 8;
 constexpr int kBlockBytes = kTile * 128;  // 64 channels of a 16-bit tile
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRaise = 8.0f;   // log2 units
@@ -86,6 +96,7 @@ struct Cfg {
   static constexpr int kRawBytes = kTile * kD;
   static constexpr int kBlocks = kD / 64;
   static constexpr int kTileBytes = kBlocks * kBlockBytes;
+  static_assert(kFactors > kRawUnits / 2 + kStages && kFactors / 2 > 3 && kRawUnits <= 4, "a slot would be overwritten in use");
 };
 // TMEM columns: scores, then weights, of half h of query tile t; sums of query tile t.
 __device__ __forceinline__ uint32_t s_col(int t, int h) { return static_cast<uint32_t>(t * 128 + h * 64); }
