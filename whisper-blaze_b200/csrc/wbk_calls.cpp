@@ -4,7 +4,7 @@
 // Through ctypes such a call spends 12 to 18 us on the host, more than its kernel runs
 // in a small batch. Here the arguments are looked at in C++: a call whose every
 // argument is as the entry point needs it, on the current device, is made at once
-// (6 to 8 us). Anything else returns None, and ops.py goes its own way: it finds the same
+// (5 to 8 us). Anything else returns None, and ops.py goes its own way: it finds the same
 // things wrong, says what, and raises; so messages and rules have one home.
 //
 // An extension module of the torch that it was compiled with (ops.py imports it if it

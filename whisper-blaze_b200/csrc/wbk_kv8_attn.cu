@@ -10,8 +10,8 @@
 //     batches and one long sequence fill the SMs alike. Warps share nothing but the
 //     items that lie in several of them: such an item is joined first by the last warp
 //     of a CTA to finish, through shared memory, then by the last of its CTAs, through
-//     global memory, always in the order of the list. Short items are not split
-//     between CTAs.
+//     global memory, always in the order of the list. CTAs split an item only if it has
+//     more tiles than min(a CTA's share, kWhole).
 //   * Each warp keeps a ring of tiles in flight with TMA (swizzled, so that the
 //     fragment loads below have no bank conflicts) and looks pages and scales up 32
 //     at a time and one batch ahead.
@@ -30,12 +30,12 @@
 // codes need fp16 weights, is an error of 2^-11 of each weight and of 2^-32 of the
 // largest product; totals take the fp32 weights. Queries in bf16 become fp16 by an exact power of two per row.
 //
-// Measured, head size 64: 64 sequences of 1500 tokens, 20 heads, one query (246 MB) 54 us:
-// HBM's rate (6.5 TB/s) from the first tile at 5 to 8 us to the first warps' end at
-// 42 us, and then the others' ends and joins. The same with 45 to 448 tokens (41 MB)
-// 20 us; one sequence of 224 tokens 7.4 us (launch, lengths, pages, codes, join: each
+// Measured, head size 64: 64 sequences of 1500 tokens, 20 heads, one query (246 MB) 55 us:
+// the first tiles are there at 5 to 11 us, half of the warps have done their last by 42 us
+// (HBM's rate in between), the others by 51, and joins end at 53. The same with 45 to 448 tokens (41 MB)
+// 21 us; one sequence of 224 tokens 7.4 us (launch, lengths, pages, codes, join: each
 // waits for the one before). Head size 128: 16 sequences of up to 32768 tokens, 8 KV heads for
-// 32 query heads (738 MB) 136 us, 5.4 TB/s, 0.83 of a plain copy's rate. Longer shares
+// 32 query heads (738 MB) 135 us, 5.5 TB/s, 0.84 of a plain copy's rate. Longer shares
 // for the CTAs that an SM gets first, which end first, gave nothing (54.4 -> 55.2 to
 // 57.5 us): HBM is busy meanwhile.
 #include <algorithm>

@@ -33,7 +33,7 @@
 //
 // Measured: 2011 queries of 32 heads (8 KV heads) of 128 behind 16000 cached tokens (0.49
 // TFLOP) 546 to 575 us, 0.86 to 0.90 PFLOP/s, 0.52 to 0.55 of the rate of a plain bf16 product. The
-// tensor pipe is busy 44 % of the time, the exponentials' unit 45 %, issue slots 49 %:
+// tensor pipe is busy 47 % of an SM's time, the exponentials' unit 48 %, issue slots 53 %:
 // a softmax warp waits for its own chain of loads, maxima, exponentials and stores.
 // Whole 128-token score tiles took 660 us; part of the exponentials as polynomials gave
 // nothing. 8 prompts of 223 tokens, 20 heads of 64:
