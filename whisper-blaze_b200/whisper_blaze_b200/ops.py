@@ -318,7 +318,8 @@ def _zeros(nbytes: int, device: torch.device) -> torch.Tensor:
 def splitk_workspace(device, nbytes: int) -> Optional[torch.Tensor]:
     """The per-device split-K workspace (zero-filled once, grown on demand).
 
-    One that was outgrown is kept: a captured graph may hold its address. Each is at least twice the one before.
+    One that was outgrown is kept: a captured graph may hold its address. Each is at least twice the one before. A call
+    in a capture that needs a larger one gets it for itself: it lies in the graph's memory, and only the replays zero it.
     Shared by every short-M GEMM on the device, so such GEMMs must not run
     concurrently on different streams; pass `workspace=` to gemm_fp8 to give a
     stream its own."""
@@ -327,6 +328,8 @@ def splitk_workspace(device, nbytes: int) -> Optional[torch.Tensor]:
     dev = torch.device(device)
     ws = _SPLITK_WS.get(dev)
     if ws is None or ws.numel() < nbytes:
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            return _zeros(nbytes, dev)
         if ws is not None:
             nbytes = max(nbytes, 2 * ws.numel())
         new = _zeros(nbytes, dev)
