@@ -173,6 +173,7 @@ def device_error() -> int:
         dev = torch.cuda.current_device()
         for fn in _TIMEOUT_HOOKS:
             fn(dev)
+        torch.cuda.synchronize(dev)  # the next call may be on another stream than what the hooks issued
     return code.value
 
 
